@@ -279,6 +279,75 @@ int kb_attn_bwd(void* dq, void* dk, void* dv, const void* q, const void* k, cons
 int kb_cross_kv(void* k16, void* v16, int ld_out, const void* ctx, int ld_ctx, int ctx_dtype, int L, int N, int K, const void* Wk,
                 const void* Wv, int ldw, const void* kn_w_bf16, float eps, void* workspace, size_t workspace_bytes, void* stream);
 
+/* ---- 4-bit floating point in blocks that share a scale, for a DiT served or LoRA-trained on a 4-bit base (the engine holds bf16 / fp16 weights only).
+ * An element is one of 0, 0.5, 1, 1.5, 2, 3, 4, 6 with a sign (e2m1) times the scale of its block, along a row:
+ *   KB_MX4  blocks of 32, scale 2^(floor(log2 max|x|) - 2), at least 2^-127 (stored as a biased exponent, E8M0); exp must be 0
+ *   KB_NV4  blocks of 16, scale = max|x| 2^-exp / 6 rounded to E4M3, at least 2^-9 and at most 448, times 2^exp of the whole matrix: choose exp so
+ *           that max|x| 2^-exp / 6 of most blocks lies in [2^-6, 448] (weights near 0.02: exp = -9); -64 <= exp <= 64
+ * Elements are x / scale rounded to nearest, ties to even, magnitudes beyond 6 to 6: each is decided exactly, so a matrix has one quantisation. A block
+ * with an infinity or NaN gets a NaN scale, which every product with it shows.
+ *
+ * A 4-bit matrix [rows, cols] is two buffers. codes: rows of ld_codes bytes (a multiple of 16, >= kb_quant4_row_bytes(cols) = 16 ceil(cols / 32)), two
+ * elements per byte, the even column in the low half, zeros up to a multiple of 32 columns. scales: kb_quant4_scale_bytes(rows, cols, fmt) bytes, in pieces of
+ * 512 for 128 rows x 4 blocks: row r, block b at ((r / 128) P + b / 4) 512 + (r % 32) 16 + (r / 32 % 4) 4 + b % 4, P = ceil(blocks / 4); zeros for the blocks
+ * behind the last one of a row, nothing is written for rows behind the last. Rows from a multiple of 128 on are a matrix of their own at the
+ * same ld_codes (scales 512 P bytes per 128 rows further). Both buffers 16-byte aligned. cols up to KB_MAX_Q4_COLS. */
+enum { KB_MX4 = 0, KB_NV4 = 1 };
+#define KB_MAX_Q4_COLS (1 << 24)
+int kb_quant4_row_bytes(int cols);                              /* 0: cols out of range */
+size_t kb_quant4_scale_bytes(int rows, int cols, int fmt);      /* 0: bad argument */
+
+/* x [rows, ld_x] (KB_F16 / KB_BF16 / KB_F32; any stride, any alignment of its elements) to 4 bits, one launch. */
+int kb_quant4(void* codes, int ld_codes, void* scales, const void* x, int ld_x, int dtype, int rows, int cols, int fmt, int exp, void* stream);
+/* The values that a 4-bit matrix stands for: y [rows, ld_y], or with transpose y [cols, ld_y]; rounded once to out_dtype. Any stride and alignment of y.
+ * (An element times its scale has six significant bits: exact in every type within its range; fp16 holds it from 2^-24 to 65504.) */
+int kb_dequant4(void* y, int ld_y, int out_dtype, const void* codes, int ld_codes, const void* scales, int rows, int cols, int fmt, int exp, int transpose,
+                void* stream);
+
+/* kb_linear16 on 4-bit operands: C = epilogue(alpha * A[M,K] . W[N,K]^T), A and W of one format, fp32 sums. alpha carries both matrices' powers of two:
+ * 2^(exp_A + exp_W) (1 for KB_MX4). Epilogues KB_EPI_F32, KB_EPI_F16, KB_EPI_GELU16, KB_EPI_RESID (C += gate[c] * alpha * acc, gate NULL = 1) as there, and
+ *   KB_EPI_GELU4   C = gelu_erf(alpha * acc) in 4 bits of the same format (exp 0): C its codes, ldc their row bytes, C_scales its scales, which no other
+ *                  epilogue takes. What the next kb_linear4 reads: the hidden activations of an MLP never exist in 16 bits.
+ * M, N, K free (K up to KB_MAX_Q4_COLS). C 16-byte aligned, ldc a multiple of 8 (fp16) / 4 (fp32) / 16 (bytes of codes). Repeats are bit-identical. */
+enum { KB_EPI_GELU4 = 5 };
+int kb_linear4(void* C, int ldc, void* C_scales, const void* A, int lda, const void* A_scales, const void* W, int ldw, const void* W_scales, int M, int N,
+               int K, int fmt, int epi, float alpha, const float* gate, void* stream);
+
+/* The gradient of kb_linear4's input (A taken as the values that it was quantised from): dx [M, K] = dy [M, N] . W [N, K], dy fp16, dx fp16 or fp32.
+ * W is decoded, transposed, to fp16 in the workspace (kb_linear4_dx_workspace_bytes(N, K), always required), then multiplied as kb_linear16 does.
+ * N a multiple of 64, K of 8. Frozen weights have no gradient. */
+size_t kb_linear4_dx_workspace_bytes(int N, int K);
+int kb_linear4_dx(void* dx, int ld_dx, int out_dtype, const void* dy_f16, int ld_dy, const void* W, int ldw, const void* W_scales, int M, int N, int K, int fmt,
+                  int exp, void* workspace, size_t workspace_bytes, void* stream);
+
+/* ---- Rotary positions from integers, of n <= 4 tensors (q and k of a block, or their gradients) in one launch. kb_qk_prep and KB_EPI_HEADS16 rotate whole
+ * heads of 128 by fp32 tables; this takes heads of any size up to 256, the first rot_dim elements of them, either layout, and computes the angles:
+ * pair i of row r turns by pos[r % pos_rows][axis[i]] * freq[i] radians, exactly reduced (positions of the whole int range, negative ones too):
+ *   (a, b) -> amplitude * (a cos - b sin, b cos + a sin),  pairs (i, i + rot_dim/2) for KB_ROPE_HALF, (2i, 2i + 1) for KB_ROPE_INTERLEAVED.
+ * The rest of the head is copied. inverse: by the negative angle, which is the gradient.
+ *   out[k] / in[k]: [rows, ld] with head h at columns [h head_dim, ...), heads[k] heads; out[k] may be in[k] (same stride), else they must not overlap
+ *   pos: device, int [pos_rows, ld_pos], n_axes columns used (DiT: frame, row, column); freq, axis: HOST arrays of rot_dim / 2, axis NULL = all 0
+ * The arrays of pointers and sizes are host memory as well and are read before the call returns. Any stride and alignment of elements. */
+enum { KB_ROPE_HALF = 0, KB_ROPE_INTERLEAVED = 1 };
+int kb_rope(int n, void* const* out, const int* ld_out, const void* const* in, const int* ld_in, const int* heads, int dtype, int rows, int head_dim, int rot_dim,
+            int layout, const int* pos, int pos_rows, int ld_pos, int n_axes, const double* freq, const int* axis, float amplitude, int inverse, void* stream);
+/* freq[i] = base^(-2i / rot_dim), i < rot_dim / 2 (at most 128), for contexts stretched by `factor`:
+ *   KB_ROPE_LINEAR  freq / factor (positions interpolated)
+ *   KB_ROPE_BASE    base * factor^(rot_dim / (rot_dim - 2)): the slowest pair is stretched by factor, the fastest not at all
+ *   KB_ROPE_PARTS   by turns over the trained length, trained_len * freq / 2 pi: at most slow_turns: freq / factor, at least fast_turns: freq, between
+ *                   them a linear mixture of both
+ * Host arithmetic, no device needed. Parameters that a scaling does not use are ignored. */
+enum { KB_ROPE_PLAIN = 0, KB_ROPE_LINEAR = 1, KB_ROPE_BASE = 2, KB_ROPE_PARTS = 3 };
+int kb_rope_freqs(double* freq, int rot_dim, double base, int scaling, double factor, double trained_len, double slow_turns, double fast_turns);
+
+/* ---- Dropout with a mask that is never stored, for the input of a LoRA's down-projection: out = keep ? in * s : 0 (+ resid). keep is a function of rng[0]
+ * (seed), rng[1] (offset), row and column alone (Philox4x32-10, dropout.cuh has the mapping), so the gradient is the same call on out's gradient with the same
+ * rng, and `resid` sums it into a gradient from elsewhere. An element is dropped with probability t / 65536, t = p rounded to 16 bits, and s = 65536 / (65536 - t).
+ * rng is device memory (two words, 8-byte aligned), read when the kernel runs: a captured call takes what lies there at each replay.
+ * resid [rows, ld_resid] has out's type; out may be in or resid (same stride and, for in, same type), else must not overlap them. 0 <= p < 1 - 2^-17. */
+int kb_dropout(void* out, int ld_out, int out_dtype, const void* in, int ld_in, int in_dtype, const void* resid, int ld_resid, int rows, int cols, double p,
+               const unsigned long long* rng, void* stream);
+
 /* dst[r * ld + col0 + c] = fp16(scale * src[r, c]) for a bf16 matrix [rows, cols]: builds the stacked operands A_cat
  * (scale 1) and B_cat (the LoRA's scale) of the second product (k_lora_pack, engine/src/kernels.cu:548-554). */
 int kb_lora_pack(void* dst_f16, int ld, int col0, const void* src_bf16, int rows, int cols, float scale, void* stream);

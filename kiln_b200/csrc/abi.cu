@@ -4,6 +4,7 @@
 #include <cuda.h>
 #include <cuda_runtime.h>
 
+#include <math.h>
 #include <string.h>
 
 #include <mutex>
@@ -15,6 +16,10 @@
 #include "selfcheck.cuh"
 #include "gemm_sm100.cuh"
 #include "attn_bwd_sm100.cuh"
+#include "quant4.cuh"
+#include "gemm4_sm100.cuh"
+#include "rope.cuh"
+#include "dropout.cuh"
 #include "routes.h"
 
 namespace {
@@ -84,6 +89,13 @@ int set_gemm_smem() {
     return KB_OK;
 }
 
+template <int EPI>
+int set_gemm4_smem() {
+    int rc;
+    if ((rc = set_smem(gemm4_kernel<EPI, FMT_MX4>, G4_SMEM))) return rc;
+    return set_smem(gemm4_kernel<EPI, FMT_NV4>, G4_SMEM);
+}
+
 int init_device(DeviceState& st, int dev) {
     cudaDeviceProp prop;
     if (cudaGetDeviceProperties(&prop, dev) != cudaSuccess) return KB_ERR_DEVICE;
@@ -112,6 +124,9 @@ int init_device(DeviceState& st, int dev) {
     if ((rc = set_smem(attn_fwd_kernel<MODE_NAG, float>, ATTN_SMEM_NAG))) return rc;
     if ((rc = set_gemm_smem<EPI_F32>()) || (rc = set_gemm_smem<EPI_F16>()) || (rc = set_gemm_smem<EPI_GELU16>()) ||
         (rc = set_gemm_smem<EPI_RESID>()) || (rc = set_gemm_smem<EPI_HEADS16>()))
+        return rc;
+    if ((rc = set_gemm4_smem<EPI_F32>()) || (rc = set_gemm4_smem<EPI_F16>()) || (rc = set_gemm4_smem<EPI_GELU16>()) ||
+        (rc = set_gemm4_smem<EPI_RESID>()) || (rc = set_gemm4_smem<EPI_GELU4>()))
         return rc;
     for (int i = 1; i <= 2; i++) {
         cudaLaunchConfig_t cfg = {};
@@ -959,6 +974,331 @@ int kb_cross_kv(void* k16, void* v16, int ld_out, const void* ctx, int ld_ctx, i
     const void* const hw[2] = {kn_w_bf16, nullptr};
     const int rope_on[2] = {0, 0};
     return linear16_segments(cs, ld_out, x16, ldx, ws, ldw, 2, L, N, K, KB_EPI_HEADS16, nullptr, hw, rope_on, nullptr, nullptr, 0, eps, stream);
+}
+
+}  // extern "C"
+
+// ------------------------------------------------------------------------------------------- 4-bit matrices and their products
+namespace {
+
+constexpr int MAX_Q4_EXP = 64;
+
+inline bool valid_q4(int fmt, int exp) {
+    return fmt == KB_NV4 ? exp >= -MAX_Q4_EXP && exp <= MAX_Q4_EXP : fmt == KB_MX4 && exp == 0;
+}
+
+// a 4-bit matrix as an argument
+int check_q4(const void* codes, int ld, const void* scales, int cols) {
+    if (!codes || !scales) return KB_ERR_ARG;
+    if (!aligned16(codes) || !aligned16(scales) || (ld & 15)) return KB_ERR_ALIGN;
+    if (ld < q4_row_bytes(cols)) return KB_ERR_SHAPE;
+    return KB_OK;
+}
+
+inline size_t elem_size(int dtype) { return dtype == KB_F32 ? 4 : 2; }
+// whether every row starts on 16 bytes, so that a thread may take eight elements at once
+inline bool wide_rows(const void* p, int ld, int dtype) { return aligned16(p) && (ld * elem_size(dtype)) % 16 == 0; }
+
+int quant4_grid(Quant4Params& p, dim3* grid) {
+    p.segs = (p.cols + Q4_SEGS * 256 - 1) / (Q4_SEGS * 256);
+    const long long blocks = ((long long)p.rows * p.segs + Q4_THREADS / 32 - 1) / (Q4_THREADS / 32);
+    if (blocks > 0x7fffffffLL) return KB_ERR_SHAPE;
+    *grid = dim3((unsigned)blocks);
+    return KB_OK;
+}
+
+template <int FMT>
+int launch_quant4(Quant4Params& p, int dtype, cudaStream_t stream) {
+    dim3 grid;
+    int rc;
+    if ((rc = quant4_grid(p, &grid))) return rc;
+    if (dtype == KB_F16) return launch_dependent(quant4_kernel<__half, FMT>, grid, dim3(Q4_THREADS), 0, stream, nullptr, p);
+    if (dtype == KB_BF16) return launch_dependent(quant4_kernel<__nv_bfloat16, FMT>, grid, dim3(Q4_THREADS), 0, stream, nullptr, p);
+    return launch_dependent(quant4_kernel<float, FMT>, grid, dim3(Q4_THREADS), 0, stream, nullptr, p);
+}
+
+template <int FMT, typename T>
+int launch_dequant4_t(Quant4Params& p, bool transpose, cudaStream_t stream) {
+    dim3 grid;
+    int rc;
+    if (transpose) {
+        const long long blocks = (((long long)p.rows + Q4_TILE - 1) / Q4_TILE) * ((p.cols + Q4_TILE - 1) / Q4_TILE);
+        if (blocks > 0x7fffffffLL) return KB_ERR_SHAPE;
+        return launch_dependent(dequant4_t_kernel<T, FMT>, dim3((unsigned)blocks), dim3(256), 0, stream, nullptr, p);
+    }
+    if ((rc = quant4_grid(p, &grid))) return rc;
+    return launch_dependent(dequant4_kernel<T, FMT>, grid, dim3(Q4_THREADS), 0, stream, nullptr, p);
+}
+
+template <int FMT>
+int launch_dequant4(Quant4Params& p, int dtype, bool transpose, cudaStream_t stream) {
+    if (dtype == KB_F16) return launch_dequant4_t<FMT, __half>(p, transpose, stream);
+    if (dtype == KB_BF16) return launch_dequant4_t<FMT, __nv_bfloat16>(p, transpose, stream);
+    return launch_dequant4_t<FMT, float>(p, transpose, stream);
+}
+
+// codes [rows][row bytes]: box 128 bytes x 128 rows
+int make_tmap_codes(CUtensorMap* tm, const void* ptr, int rows, int cols, int ld) {
+    const cuuint64_t dims[3] = {(cuuint64_t)q4_row_bytes(cols), (cuuint64_t)rows, 1};
+    const cuuint64_t strides[2] = {(cuuint64_t)ld, (cuuint64_t)rows * (cuuint64_t)ld};
+    const cuuint32_t box[3] = {128, 128, 1};
+    const cuuint32_t estr[3] = {1, 1, 1};
+    CUresult r = g_encode(tm, CU_TENSOR_MAP_DATA_TYPE_UINT8, 3, const_cast<void*>(ptr), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                          CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    return r == CUDA_SUCCESS ? KB_OK : KB_ERR_CUDA;
+}
+// scales [row block][piece][128 words]: box = the pieces of one k step of one row block
+int make_tmap_scales(CUtensorMap* tm, const void* ptr, int rows, int cols, int fmt) {
+    const int pieces = q4_pieces(cols, fmt);
+    const cuuint64_t dims[3] = {128, (cuuint64_t)pieces, (cuuint64_t)((rows + 127) / 128)};
+    const cuuint64_t strides[2] = {512, (cuuint64_t)pieces * 512};
+    const cuuint32_t box[3] = {128, (cuuint32_t)(G4_K / (4 * q4_block(fmt))), 1};
+    const cuuint32_t estr[3] = {1, 1, 1};
+    CUresult r = g_encode(tm, CU_TENSOR_MAP_DATA_TYPE_UINT32, 3, const_cast<void*>(ptr), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                          CU_TENSOR_MAP_SWIZZLE_NONE, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    return r == CUDA_SUCCESS ? KB_OK : KB_ERR_CUDA;
+}
+
+template <int EPI, int FMT>
+int launch_gemm4(DeviceState* st, const Gemm4Maps& maps, Gemm4Params p, cudaStream_t stream) {
+    p.tiles_m = (p.M + 127) / 128;
+    p.tiles_n = (p.N + 127) / 128;
+    const long long n_tiles = (long long)p.tiles_m * p.tiles_n;
+    if (n_tiles > 0x3fffffffLL) return KB_ERR_SHAPE;
+    const unsigned grid = (unsigned)(n_tiles < st->sm_count ? n_tiles : st->sm_count);
+    return launch_dependent(gemm4_kernel<EPI, FMT>, dim3(grid), dim3(G_THREADS), G4_SMEM, stream, nullptr, maps, p);
+}
+
+template <int FMT>
+int launch_gemm4_epi(DeviceState* st, int epi, const Gemm4Maps& maps, const Gemm4Params& p, cudaStream_t stream) {
+    switch (epi) {
+        case KB_EPI_F32: return launch_gemm4<EPI_F32, FMT>(st, maps, p, stream);
+        case KB_EPI_F16: return launch_gemm4<EPI_F16, FMT>(st, maps, p, stream);
+        case KB_EPI_GELU16: return launch_gemm4<EPI_GELU16, FMT>(st, maps, p, stream);
+        case KB_EPI_RESID: return launch_gemm4<EPI_RESID, FMT>(st, maps, p, stream);
+        default: return launch_gemm4<EPI_GELU4, FMT>(st, maps, p, stream);
+    }
+}
+
+}  // namespace
+
+extern "C" {
+
+int kb_quant4_row_bytes(int cols) { return cols > 0 && cols <= KB_MAX_Q4_COLS ? q4_row_bytes(cols) : 0; }
+
+size_t kb_quant4_scale_bytes(int rows, int cols, int fmt) {
+    if (rows <= 0 || cols <= 0 || cols > KB_MAX_Q4_COLS || (fmt != KB_MX4 && fmt != KB_NV4)) return 0;
+    return (((size_t)rows + 127) / 128) * q4_pieces(cols, fmt) * 512;
+}
+
+int kb_quant4(void* codes, int ld_codes, void* scales, const void* x, int ld_x, int dtype, int rows, int cols, int fmt, int exp, void* stream_) {
+    cudaStream_t stream = static_cast<cudaStream_t>(stream_);
+    if (!x || rows < 0 || cols <= 0 || !valid_in_dtype(dtype) || !valid_q4(fmt, exp)) return KB_ERR_ARG;
+    if (cols > KB_MAX_Q4_COLS || ld_x < cols) return KB_ERR_SHAPE;
+    if (reinterpret_cast<uintptr_t>(x) % elem_size(dtype)) return KB_ERR_ALIGN;
+    int rc;
+    if ((rc = check_q4(codes, ld_codes, scales, cols))) return rc;
+    DeviceState* st;
+    if ((rc = get_state(&st))) return rc;
+    if (rows == 0) return KB_OK;
+    Quant4Params p = {};
+    p.x = x; p.codes = static_cast<uint8_t*>(codes); p.scales = static_cast<uint8_t*>(scales);
+    p.rows = rows; p.cols = cols; p.ld_x = ld_x; p.ld = ld_codes; p.pieces = q4_pieces(cols, fmt); p.exp = exp;
+    p.wide = wide_rows(x, ld_x, dtype);
+    ProfScope ps(st, KB_PROF_LINEAR, stream);
+    return fmt == KB_MX4 ? launch_quant4<FMT_MX4>(p, dtype, stream) : launch_quant4<FMT_NV4>(p, dtype, stream);
+}
+
+int kb_dequant4(void* y, int ld_y, int out_dtype, const void* codes, int ld_codes, const void* scales, int rows, int cols, int fmt, int exp,
+                int transpose, void* stream_) {
+    cudaStream_t stream = static_cast<cudaStream_t>(stream_);
+    if (!y || rows < 0 || cols <= 0 || !valid_in_dtype(out_dtype) || !valid_q4(fmt, exp)) return KB_ERR_ARG;
+    if (cols > KB_MAX_Q4_COLS || ld_y < (transpose ? rows : cols)) return KB_ERR_SHAPE;
+    if (reinterpret_cast<uintptr_t>(y) % elem_size(out_dtype)) return KB_ERR_ALIGN;
+    int rc;
+    if ((rc = check_q4(codes, ld_codes, scales, cols))) return rc;
+    DeviceState* st;
+    if ((rc = get_state(&st))) return rc;
+    if (rows == 0) return KB_OK;
+    Quant4Params p = {};
+    p.y = y; p.codes = static_cast<uint8_t*>(const_cast<void*>(codes)); p.scales = static_cast<uint8_t*>(const_cast<void*>(scales));
+    p.rows = rows; p.cols = cols; p.ld_x = ld_y; p.ld = ld_codes; p.pieces = q4_pieces(cols, fmt); p.exp = exp;
+    p.wide = wide_rows(y, ld_y, out_dtype);
+    ProfScope ps(st, KB_PROF_LINEAR, stream);
+    return fmt == KB_MX4 ? launch_dequant4<FMT_MX4>(p, out_dtype, transpose != 0, stream) : launch_dequant4<FMT_NV4>(p, out_dtype, transpose != 0, stream);
+}
+
+int kb_linear4(void* C, int ldc, void* C_scales, const void* A, int lda, const void* A_scales, const void* W, int ldw, const void* W_scales, int M,
+               int N, int K, int fmt, int epi, float alpha, const float* gate, void* stream_) {
+    cudaStream_t stream = static_cast<cudaStream_t>(stream_);
+    if (!C || M < 0 || N <= 0 || K <= 0 || !valid_q4(fmt, 0)) return KB_ERR_ARG;
+    const bool out4 = epi == KB_EPI_GELU4, out32 = epi == KB_EPI_F32 || epi == KB_EPI_RESID;
+    if (!out4 && !out32 && epi != KB_EPI_F16 && epi != KB_EPI_GELU16) return KB_ERR_ARG;
+    if ((gate && epi != KB_EPI_RESID) || (C_scales && !out4)) return KB_ERR_ARG;
+    if (K > KB_MAX_Q4_COLS || N > KB_MAX_Q4_COLS) return KB_ERR_SHAPE;
+    int rc;
+    if ((rc = check_q4(A, lda, A_scales, K)) || (rc = check_q4(W, ldw, W_scales, K))) return rc;
+    if (out4) {
+        if ((rc = check_q4(C, ldc, C_scales, N))) return rc;
+    } else {
+        if (!aligned16(C) || (ldc & (out32 ? 3 : 7))) return KB_ERR_ALIGN;
+        if (ldc < N) return KB_ERR_SHAPE;
+    }
+    if (reinterpret_cast<uintptr_t>(gate) % 4) return KB_ERR_ALIGN;
+    DeviceState* st;
+    if ((rc = get_state(&st))) return rc;
+    if (M == 0) return KB_OK;
+    Gemm4Maps maps;
+    memset(&maps, 0, sizeof(maps));
+    if ((rc = make_tmap_codes(&maps.a, A, M, K, lda)) || (rc = make_tmap_codes(&maps.w, W, N, K, ldw)) ||
+        (rc = make_tmap_scales(&maps.sa, A_scales, M, K, fmt)) || (rc = make_tmap_scales(&maps.sw, W_scales, N, K, fmt)) ||
+        (!out4 && (rc = make_tmap_out(&maps.c, C, M, N, ldc, out32, false, false))))
+        return rc;
+    Gemm4Params p = {};
+    p.M = M; p.N = N; p.K = K; p.alpha = alpha; p.C = C; p.ldc = ldc; p.gate = gate; p.status = st->status;
+    if (out4) { p.codes = static_cast<uint8_t*>(C); p.scales = static_cast<uint8_t*>(C_scales); p.ld_codes = ldc; p.pieces = q4_pieces(N, fmt); }
+    ProfScope ps(st, KB_PROF_LINEAR, stream);
+    return fmt == KB_MX4 ? launch_gemm4_epi<FMT_MX4>(st, epi, maps, p, stream) : launch_gemm4_epi<FMT_NV4>(st, epi, maps, p, stream);
+}
+
+size_t kb_linear4_dx_workspace_bytes(int N, int K) { return N > 0 && K > 0 ? (size_t)N * (size_t)K * 2 : 0; }
+
+int kb_linear4_dx(void* dx, int ld_dx, int out_dtype, const void* dy_f16, int ld_dy, const void* W, int ldw, const void* W_scales, int M, int N, int K,
+                  int fmt, int exp, void* workspace, size_t workspace_bytes, void* stream_) {
+    cudaStream_t stream = static_cast<cudaStream_t>(stream_);
+    if (!dx || !dy_f16 || M < 0 || N <= 0 || K <= 0 || !valid_q4(fmt, exp) || (out_dtype != KB_F16 && out_dtype != KB_F32)) return KB_ERR_ARG;
+    if (!aligned16(dx) || !aligned16(dy_f16) || (ld_dy & 7) || (ld_dx & (out_dtype == KB_F32 ? 3 : 7))) return KB_ERR_ALIGN;
+    if ((N % GB_K) || (K % 8) || K > KB_MAX_Q4_COLS || ld_dy < N || ld_dx < K) return KB_ERR_SHAPE;
+    int rc;
+    if ((rc = check_q4(W, ldw, W_scales, K))) return rc;
+    if (M == 0) return KB_OK;
+    if (!workspace || workspace_bytes < kb_linear4_dx_workspace_bytes(N, K)) return KB_ERR_WORKSPACE;
+    if (!aligned16(workspace)) return KB_ERR_ALIGN;
+    // the transposed weight in fp16 (4-bit values with their scales are fp16 numbers, see the header), then the fp16 product
+    if ((rc = kb_dequant4(workspace, N, KB_F16, W, ldw, W_scales, N, K, fmt, exp, 1, stream_))) return rc;
+    void* const cs[1] = {dx};
+    const void* const ws[1] = {workspace};
+    const void* const hw[1] = {nullptr};
+    const int rope_on[1] = {0};
+    return linear16_segments(cs, ld_dx, dy_f16, ld_dy, ws, N, 1, M, K, N, out_dtype == KB_F32 ? KB_EPI_F32 : KB_EPI_F16, nullptr, hw, rope_on, nullptr, nullptr,
+                             0, 0.f, stream);
+}
+
+// ------------------------------------------------------------------------------------------- rotary positions, dropout
+int kb_rope_freqs(double* freq, int rot_dim, double base, int scaling, double factor, double trained_len, double slow_turns, double fast_turns) {
+    if (!freq || rot_dim <= 0 || (rot_dim & 1) || rot_dim > 2 * ROPE_MAX_PAIRS || !(base > 0.0) || !isfinite(base)) return KB_ERR_ARG;
+    if (scaling < KB_ROPE_PLAIN || scaling > KB_ROPE_PARTS) return KB_ERR_ARG;
+    if (scaling != KB_ROPE_PLAIN && (!(factor > 0.0) || !isfinite(factor))) return KB_ERR_ARG;
+    if (scaling == KB_ROPE_PARTS && (!(trained_len > 0.0) || !isfinite(trained_len) || !(fast_turns > slow_turns) || !isfinite(fast_turns) || !isfinite(slow_turns)))
+        return KB_ERR_ARG;
+    if (scaling == KB_ROPE_BASE && rot_dim > 2) base *= pow(factor, (double)rot_dim / (rot_dim - 2));
+    for (int i = 0; i < rot_dim / 2; i++) {
+        double f = pow(base, -2.0 * i / rot_dim);
+        if (scaling == KB_ROPE_LINEAR) f /= factor;
+        if (scaling == KB_ROPE_PARTS) {
+            double keep = (trained_len * f / 6.283185307179586 - slow_turns) / (fast_turns - slow_turns);
+            keep = keep < 0.0 ? 0.0 : keep > 1.0 ? 1.0 : keep;
+            f = f * keep + f / factor * (1.0 - keep);
+        }
+        freq[i] = f;
+    }
+    return KB_OK;
+}
+
+}  // extern "C"
+
+namespace {
+
+template <typename T>
+int launch_rope_t(const RopeParams& p, bool half, bool vec, unsigned blocks, cudaStream_t stream) {
+    const dim3 grid(blocks), block(ROPE_THREADS);
+    if (half) {
+        if (vec) return launch_dependent(rope_kernel<T, true, true>, grid, block, 0, stream, nullptr, p);
+        return launch_dependent(rope_kernel<T, true, false>, grid, block, 0, stream, nullptr, p);
+    }
+    if (vec) return launch_dependent(rope_kernel<T, false, true>, grid, block, 0, stream, nullptr, p);
+    return launch_dependent(rope_kernel<T, false, false>, grid, block, 0, stream, nullptr, p);
+}
+
+template <typename InT>
+int launch_dropout_t(const DropoutParams& p, int out_dtype, unsigned blocks, cudaStream_t stream) {
+    if (out_dtype == KB_F16) return launch_dependent(dropout_kernel<InT, __half>, dim3(blocks), dim3(DROP_THREADS), 0, stream, nullptr, p);
+    if (out_dtype == KB_BF16) return launch_dependent(dropout_kernel<InT, __nv_bfloat16>, dim3(blocks), dim3(DROP_THREADS), 0, stream, nullptr, p);
+    return launch_dependent(dropout_kernel<InT, float>, dim3(blocks), dim3(DROP_THREADS), 0, stream, nullptr, p);
+}
+
+}  // namespace
+
+extern "C" {
+
+int kb_rope(int n, void* const* out, const int* ld_out, const void* const* in, const int* ld_in, const int* heads, int dtype, int rows, int head_dim,
+            int rot_dim, int layout, const int* pos, int pos_rows, int ld_pos, int n_axes, const double* freq, const int* axis, float amplitude, int inverse,
+            void* stream_) {
+    cudaStream_t stream = static_cast<cudaStream_t>(stream_);
+    if (n < 1 || n > ROPE_MAX_TENSORS || !out || !ld_out || !in || !ld_in || !heads || !pos || !freq || !valid_in_dtype(dtype)) return KB_ERR_ARG;
+    if (rows < 0 || head_dim <= 0 || rot_dim <= 0 || (rot_dim & 1) || pos_rows <= 0 || n_axes < 1 || (layout != KB_ROPE_HALF && layout != KB_ROPE_INTERLEAVED))
+        return KB_ERR_ARG;
+    if (head_dim > 2 * ROPE_MAX_PAIRS || rot_dim > head_dim || n_axes > 255 || ld_pos < n_axes) return KB_ERR_SHAPE;
+    if (reinterpret_cast<uintptr_t>(pos) % 4) return KB_ERR_ALIGN;
+    RopeParams p = {};
+    p.wide = head_dim % 8 == 0;
+    for (int i = 0; i < n; i++) {
+        if (!out[i] || !in[i] || heads[i] <= 0) return KB_ERR_ARG;
+        if (heads[i] > MAX_HEADS || ld_in[i] < heads[i] * head_dim || ld_out[i] < heads[i] * head_dim) return KB_ERR_SHAPE;
+        if (reinterpret_cast<uintptr_t>(out[i]) % elem_size(dtype) || reinterpret_cast<uintptr_t>(in[i]) % elem_size(dtype)) return KB_ERR_ALIGN;
+        p.t[i].x = in[i]; p.t[i].y = out[i]; p.t[i].heads = heads[i]; p.t[i].ld_x = ld_in[i]; p.t[i].ld_y = ld_out[i];
+        p.wide = p.wide && wide_rows(in[i], ld_in[i], dtype) && wide_rows(out[i], ld_out[i], dtype);
+    }
+    for (int i = 0; i < rot_dim / 2; i++) {
+        const int ax = axis ? axis[i] : 0;
+        if (ax < 0 || ax >= n_axes || !isfinite(freq[i])) return KB_ERR_ARG;
+        const long double turns = (long double)freq[i] / 6.283185307179586476925286766559005768L, part = turns - floorl(turns);
+        p.freq[i] = part < 1.0L ? (unsigned long long)(part * 18446744073709551616.0L) : 0ull;
+        p.axis[i] = (unsigned char)ax;
+    }
+    DeviceState* st;
+    int rc;
+    if ((rc = get_state(&st))) return rc;
+    if (rows == 0) return KB_OK;
+    p.pos = pos; p.n = n; p.rows = rows; p.pos_rows = pos_rows; p.ld_pos = ld_pos; p.dim = head_dim; p.rot = rot_dim; p.inverse = inverse != 0;
+    p.amplitude = amplitude;
+    const int pairs = rot_dim / 2;
+    p.block_rows = ROPE_SLOTS / pairs < 4 ? ROPE_SLOTS / pairs : 4;
+    const unsigned blocks = (unsigned)(((long long)rows + p.block_rows - 1) / p.block_rows);
+    const bool half = layout == KB_ROPE_HALF, vec = p.wide && (!half || pairs % 8 == 0);
+    ProfScope ps(st, KB_PROF_NORM_ROPE, stream);
+    if (dtype == KB_F16) return launch_rope_t<__half>(p, half, vec, blocks, stream);
+    if (dtype == KB_BF16) return launch_rope_t<__nv_bfloat16>(p, half, vec, blocks, stream);
+    return launch_rope_t<float>(p, half, vec, blocks, stream);
+}
+
+int kb_dropout(void* out, int ld_out, int out_dtype, const void* in, int ld_in, int in_dtype, const void* resid, int ld_resid, int rows, int cols, double p_drop,
+               const unsigned long long* rng, void* stream_) {
+    cudaStream_t stream = static_cast<cudaStream_t>(stream_);
+    if (!out || !in || !rng || rows < 0 || cols <= 0 || !valid_in_dtype(in_dtype) || !valid_in_dtype(out_dtype) || !(p_drop >= 0.0 && p_drop < 1.0))
+        return KB_ERR_ARG;
+    const unsigned t = (unsigned)(65536.0 * p_drop + 0.5);
+    if (t >= 65536u) return KB_ERR_ARG;
+    if (ld_in < cols || ld_out < cols || (resid && ld_resid < cols)) return KB_ERR_SHAPE;
+    if (reinterpret_cast<uintptr_t>(out) % elem_size(out_dtype) || reinterpret_cast<uintptr_t>(in) % elem_size(in_dtype) ||
+        reinterpret_cast<uintptr_t>(resid) % elem_size(out_dtype) || reinterpret_cast<uintptr_t>(rng) % 8)
+        return KB_ERR_ALIGN;
+    DeviceState* st;
+    int rc;
+    if ((rc = get_state(&st))) return rc;
+    if (rows == 0) return KB_OK;
+    DropoutParams p = {};
+    p.x = in; p.resid = resid; p.y = out; p.rng = rng;
+    p.cols = cols; p.groups = (cols + 7) / 8; p.units = (long long)rows * p.groups;
+    p.ld_x = ld_in; p.ld_r = ld_resid; p.ld_y = ld_out;
+    p.t = t; p.scale = (float)(65536.0 / (65536.0 - t));
+    p.wide = wide_rows(in, ld_in, in_dtype) && wide_rows(out, ld_out, out_dtype) && (!resid || wide_rows(resid, ld_resid, out_dtype));
+    const long long blocks = (p.units + DROP_THREADS - 1) / DROP_THREADS;
+    if (blocks > 0x7fffffffLL) return KB_ERR_SHAPE;
+    ProfScope ps(st, KB_PROF_LINEAR, stream);
+    if (in_dtype == KB_F16) return launch_dropout_t<__half>(p, out_dtype, (unsigned)blocks, stream);
+    if (in_dtype == KB_BF16) return launch_dropout_t<__nv_bfloat16>(p, out_dtype, (unsigned)blocks, stream);
+    return launch_dropout_t<float>(p, out_dtype, (unsigned)blocks, stream);
 }
 
 int kb_lora_pack(void* dst_f16, int ld, int col0, const void* src_bf16, int rows, int cols, float scale, void* stream) {

@@ -1,0 +1,254 @@
+// 4-bit floating point in blocks (e2m1: 0, 0.5, 1, 1.5, 2, 3, 4, 6 with a sign) that share a scale: to and from it.
+//   MX4  blocks of 32 columns, a = max |x|, s = 2^(floor(log2 a) - 2) (no less than 2^-127), stored as its exponent + 127 (E8M0)
+//   NV4  blocks of 16 columns, y = x 2^-exp, s = max |y| / 6 rounded to E4M3 (no less than 2^-9, no more than 448); `exp` belongs to the whole matrix
+// and each element is x / s (y / s) rounded to the nearest of the eight values, ties to the even code, beyond 6 to 6. Every one of these is
+// decided exactly, so a value has one code whatever computes it: the quotients take one step of correction (Markstein, 1990:
+// q0 = y r, q = q0 + r (y - q0 s) with a fused remainder), which makes a y that lies on a border (1.25 s, ...) give the border itself; a y
+// next to one is at least a 24-bit step away from it, more than the rounding of q. A block that holds an infinity or a NaN gets a NaN for its scale.
+//
+// Layout of a matrix [rows, cols]: codes two to a byte, the even column in the low half, rows of `ld` bytes, filled with zeros up to
+// a multiple of 32 columns. Scales in pieces of 512 bytes, 128 rows x 4 blocks, as the tensor cores' copy into TMEM reads them (32 lanes x 16
+// bytes): row r, block b at byte ((r / 128) pieces + b / 4) 512 + (r % 32) 16 + (r / 32 % 4) 4 + b % 4; pieces = ceil(blocks / 4), the
+// scales of blocks behind the last one are zeros, those of rows behind the last one are not touched.
+#pragma once
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+#include <stdint.h>
+
+#include "prep.cuh"   // Io
+#include "ptx.cuh"
+
+namespace kb {
+
+constexpr int FMT_MX4 = 0, FMT_NV4 = 1;
+__host__ __device__ constexpr int q4_block(int fmt) { return fmt == FMT_MX4 ? 32 : 16; }
+__host__ __device__ constexpr int q4_pieces(int cols, int fmt) { return (cols + 4 * q4_block(fmt) - 1) / (4 * q4_block(fmt)); }   // of a row block
+__host__ __device__ constexpr int q4_row_bytes(int cols) { return (cols + 31) / 32 * 16; }
+__device__ __forceinline__ size_t q4_scale_at(int row, int piece, int pieces) {   // the four scales of a piece
+    return ((size_t)(row >> 7) * pieces + piece) * 512 + (row & 31) * 16 + ((row >> 5) & 3) * 4;
+}
+
+// 2^e, e in [-126, 127]
+__device__ __forceinline__ float pow2f(int e) { return __uint_as_float((uint32_t)(e + 127) << 23); }
+
+// four pairs of codes from eight numbers (already divided by their scale), element i in bits [4 i, 4 i + 4)
+__device__ __forceinline__ uint32_t e2m1_pack8(const float (&v)[8]) {
+    uint32_t r;
+    asm("{\n\t.reg .b8 a, b, c, d;\n\t"
+        "cvt.rn.satfinite.e2m1x2.f32 a, %2, %1;\n\t"
+        "cvt.rn.satfinite.e2m1x2.f32 b, %4, %3;\n\t"
+        "cvt.rn.satfinite.e2m1x2.f32 c, %6, %5;\n\t"
+        "cvt.rn.satfinite.e2m1x2.f32 d, %8, %7;\n\t"
+        "mov.b32 %0, {a, b, c, d};\n\t}"
+        : "=r"(r)
+        : "f"(v[0]), "f"(v[1]), "f"(v[2]), "f"(v[3]), "f"(v[4]), "f"(v[5]), "f"(v[6]), "f"(v[7]));
+    return r;
+}
+// eight codes as four half2 (every value is one of fp16)
+__device__ __forceinline__ void e2m1_unpack8(uint32_t codes, uint32_t (&h)[4]) {
+    asm("{\n\t.reg .b8 a, b, c, d;\n\t"
+        "mov.b32 {a, b, c, d}, %4;\n\t"
+        "cvt.rn.f16x2.e2m1x2 %0, a;\n\t"
+        "cvt.rn.f16x2.e2m1x2 %1, b;\n\t"
+        "cvt.rn.f16x2.e2m1x2 %2, c;\n\t"
+        "cvt.rn.f16x2.e2m1x2 %3, d;\n\t}"
+        : "=r"(h[0]), "=r"(h[1]), "=r"(h[2]), "=r"(h[3])
+        : "r"(codes));
+}
+__device__ __forceinline__ uint32_t e4m3_byte(float v) {
+    uint16_t r;
+    asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(r) : "f"(0.f), "f"(v));
+    return r & 0xffu;
+}
+__device__ __forceinline__ float e4m3_value(uint32_t byte) {
+    uint32_t h;
+    asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(h) : "h"((uint16_t)byte));
+    return __half2float(__ushort_as_half((uint16_t)h));
+}
+// what a scale byte stands for; MX4's smallest, 2^-127, is a subnormal number
+template <int FMT>
+__device__ __forceinline__ float q4_scale_value(uint32_t byte) {
+    if (FMT == FMT_NV4) return e4m3_value(byte);
+    return byte == 0u ? __uint_as_float(0x00400000u) : byte == 255u ? __uint_as_float(0x7fffffffu) : __uint_as_float(byte << 23);
+}
+
+// The scale of a block whose largest |x| has these bits: its byte, and what elements are divided by (s) and multiplied with (r = 1 / s).
+template <int FMT>
+struct BlockScale {
+    uint32_t byte;
+    float s, r;
+    // down = 2^-exp of the matrix (NV4)
+    __device__ __forceinline__ BlockScale(uint32_t abs_bits, float down) {
+        if (FMT == FMT_MX4) {
+            const uint32_t e = abs_bits >> 23;
+            byte = e > 2u ? e - 2u : 0u;                       // floor(log2 a) + 127 - 2
+            r = __uint_as_float((254u - byte) << 23);
+            s = 0.f;                                           // powers of two: a product is exact
+        } else {
+            const float a = __uint_as_float(abs_bits) * down, sixth = 1.f / 6.f;
+            float q = a * sixth;
+            q = fmaf(fmaf(-q, 6.f, a), sixth, q);
+            byte = max(e4m3_byte(q), 1u);
+            s = e4m3_value(byte);
+            r = __frcp_rn(s);
+        }
+        if (abs_bits >= 0x7f800000u) byte = FMT == FMT_MX4 ? 255u : 127u;
+    }
+    __device__ __forceinline__ float operator()(float x, float down) const {
+        if (FMT == FMT_MX4) return x * r;
+        const float y = x * down, q = y * r;
+        return fmaf(fmaf(-q, s, y), r, q);
+    }
+};
+
+template <typename T> __device__ __forceinline__ float to_f32(T v);
+template <> __device__ __forceinline__ float to_f32<float>(float v) { return v; }
+template <> __device__ __forceinline__ float to_f32<__half>(__half v) { return __half2float(v); }
+template <> __device__ __forceinline__ float to_f32<__nv_bfloat16>(__nv_bfloat16 v) { return __bfloat162float(v); }
+template <typename T> __device__ __forceinline__ T from_f32(float v);
+template <> __device__ __forceinline__ float from_f32<float>(float v) { return v; }
+template <> __device__ __forceinline__ __half from_f32<__half>(float v) { return __float2half_rn(v); }
+template <> __device__ __forceinline__ __nv_bfloat16 from_f32<__nv_bfloat16>(float v) { return __float2bfloat16_rn(v); }
+
+// eight elements from column c of a row, zeros behind the last column; `wide`: every row starts on 16 bytes
+template <typename T>
+__device__ __forceinline__ F8 load8(const T* row, int c, int cols, bool wide) {
+    if (wide && c + 8 <= cols) return Io<T>::ld8(row + c);
+    F8 f;
+#pragma unroll
+    for (int i = 0; i < 8; i++) f.v[i] = c + i < cols ? to_f32(row[c + i]) : 0.f;
+    return f;
+}
+template <typename T>
+__device__ __forceinline__ void store8(T* row, int c, int cols, bool wide, const F8& f) {
+    if (wide && c + 8 <= cols) { Io<T>::st8(row + c, f); return; }
+#pragma unroll
+    for (int i = 0; i < 8; i++)
+        if (c + i < cols) row[c + i] = from_f32<T>(f.v[i]);
+}
+
+struct Quant4Params {
+    const void* x;               // [rows, ld_x]
+    void* y;                     // dequant: [rows, ld_x], transposed [cols, ld_x]
+    uint8_t* codes;
+    uint8_t* scales;
+    int rows, cols, ld_x, ld;    // ld: bytes of a row of codes
+    int pieces, segs;            // pieces of a row block; groups of Q4_SEGS x 256 columns of a row
+    int exp;
+    bool wide;
+};
+
+// A lane takes eight columns, so that a block is two (NV4) or four (MX4) lanes, which meet by shuffles; a warp 256 columns side by side, Q4_SEGS
+// times, its loads first. Bound by memory: 16-bit rows 2 bytes read and 0.56 written per element.
+constexpr int Q4_THREADS = 128, Q4_SEGS = 2;
+
+template <typename T, int FMT>
+__global__ void __launch_bounds__(Q4_THREADS)
+quant4_kernel(const Quant4Params p) {
+    pdl_launch();
+    pdl_wait();
+    const long long unit = (long long)blockIdx.x * (Q4_THREADS / 32) + (threadIdx.x >> 5);
+    const long long row64 = unit / p.segs;
+    if (row64 >= p.rows) return;
+    const int row = (int)row64, lane = threadIdx.x & 31;
+    const int c0 = (int)(unit % p.segs) * (Q4_SEGS * 256) + lane * 8;
+    const T* const src = static_cast<const T*>(p.x) + (size_t)row * p.ld_x;
+    const float down = pow2f(-p.exp);
+    F8 f[Q4_SEGS];
+#pragma unroll
+    for (int i = 0; i < Q4_SEGS; i++) f[i] = load8(src, c0 + i * 256, p.cols, p.wide);
+#pragma unroll
+    for (int i = 0; i < Q4_SEGS; i++) {
+        const int c = c0 + i * 256;
+        uint32_t top = 0u;
+#pragma unroll
+        for (int e = 0; e < 8; e++) top = max(top, __float_as_uint(f[i].v[e]) & 0x7fffffffu);
+        top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
+        if (FMT == FMT_MX4) top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
+        const BlockScale<FMT> bs(top, down);
+        float v[8];
+#pragma unroll
+        for (int e = 0; e < 8; e++) v[e] = bs(f[i].v[e], down);
+        if (c < q4_row_bytes(p.cols) * 2) *reinterpret_cast<uint32_t*>(p.codes + (size_t)row * p.ld + (c >> 1)) = e2m1_pack8(v);
+        // the four scales of a piece, 8 (NV4) or 16 lanes, meet in its first lane
+        constexpr int STEP = q4_block(FMT) / 8;
+        uint32_t word = c < p.cols ? bs.byte << (8 * ((lane / STEP) & 3)) : 0u;
+        word |= __shfl_xor_sync(0xffffffffu, word, STEP);
+        word |= __shfl_xor_sync(0xffffffffu, word, 2 * STEP);
+        const int piece = c / (4 * q4_block(FMT));
+        if (lane % (4 * STEP) == 0 && piece < p.pieces) *reinterpret_cast<uint32_t*>(p.scales + q4_scale_at(row, piece, p.pieces)) = word;
+    }
+}
+
+// eight values from column c (a multiple of 8) of a row, up = 2^exp
+template <int FMT>
+__device__ __forceinline__ F8 q4_values8(const Quant4Params& p, int row, int c, float up) {
+    uint32_t h[4];
+    e2m1_unpack8(*reinterpret_cast<const uint32_t*>(p.codes + (size_t)row * p.ld + (c >> 1)), h);
+    const int b = c / q4_block(FMT);
+    const float s = q4_scale_value<FMT>(p.scales[q4_scale_at(row, b >> 2, p.pieces) + (b & 3)]) * up;
+    F8 f;
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+        const float2 v = __half22float2(*reinterpret_cast<const __half2*>(&h[i]));
+        f.v[2 * i] = v.x * s;
+        f.v[2 * i + 1] = v.y * s;
+    }
+    return f;
+}
+
+template <typename T, int FMT>
+__global__ void __launch_bounds__(Q4_THREADS)
+dequant4_kernel(const Quant4Params p) {
+    pdl_launch();
+    pdl_wait();
+    const long long unit = (long long)blockIdx.x * (Q4_THREADS / 32) + (threadIdx.x >> 5);
+    const long long row64 = unit / p.segs;
+    if (row64 >= p.rows) return;
+    const int row = (int)row64, c0 = (int)(unit % p.segs) * (Q4_SEGS * 256) + (threadIdx.x & 31) * 8;
+    T* const dst = static_cast<T*>(p.y) + (size_t)row * p.ld_x;
+    const float up = pow2f(p.exp);
+#pragma unroll
+    for (int i = 0; i < Q4_SEGS; i++) {
+        const int c = c0 + i * 256;
+        if (c < p.cols) store8(dst, c, p.cols, p.wide, q4_values8<FMT>(p, row, c, up));
+    }
+}
+
+// The transpose [cols, ld_x], through shared memory in tiles of 64 x 64: a thread decodes eight columns of two rows side by side, which become
+// eight pairs along a row of the transpose. What the gradient of a projection's input multiplies with.
+constexpr int Q4_TILE = 64, Q4_TILE_LD = 72;      // elements of a tile row in shared memory: a row starts on 16 bytes, four banks further
+template <typename T, int FMT>
+__global__ void __launch_bounds__(256)
+dequant4_t_kernel(const Quant4Params p) {
+    __shared__ __align__(16) T tile[Q4_TILE * Q4_TILE_LD];
+    pdl_launch();
+    pdl_wait();
+    const int tiles_c = (p.cols + Q4_TILE - 1) / Q4_TILE;
+    const int r0 = (int)(blockIdx.x / (unsigned)tiles_c) * Q4_TILE, k0 = (int)(blockIdx.x % (unsigned)tiles_c) * Q4_TILE;
+    const int pair = threadIdx.x & 31, kg = threadIdx.x >> 5;
+    const float up = pow2f(p.exp);
+    F8 f[2];
+#pragma unroll
+    for (int i = 0; i < 2; i++) {
+        const int r = r0 + 2 * pair + i, c = k0 + 8 * kg;
+        if (r < p.rows && c < p.cols) f[i] = q4_values8<FMT>(p, r, c, up);
+        else
+#pragma unroll
+            for (int e = 0; e < 8; e++) f[i].v[e] = 0.f;
+    }
+#pragma unroll
+    for (int e = 0; e < 8; e++) {
+        struct alignas(2 * sizeof(T)) Two { T a, b; } two = {from_f32<T>(f[0].v[e]), from_f32<T>(f[1].v[e])};
+        *reinterpret_cast<Two*>(&tile[(8 * kg + e) * Q4_TILE_LD + 2 * pair]) = two;
+    }
+    __syncthreads();
+    for (int i = threadIdx.x; i < Q4_TILE * Q4_TILE / 8; i += 256) {
+        const int k = i / (Q4_TILE / 8), c = (i % (Q4_TILE / 8)) * 8;
+        if (k0 + k >= p.cols || r0 + c >= p.rows) continue;
+        const F8 v = Io<T>::ld8(&tile[k * Q4_TILE_LD + c]);
+        store8(static_cast<T*>(p.y) + (size_t)(k0 + k) * p.ld_x + r0, c, p.rows - r0, p.wide, v);
+    }
+}
+
+}  // namespace kb

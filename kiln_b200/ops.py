@@ -102,6 +102,27 @@ def lib():
         L.kb_selfcheck_workspace_bytes.restype = sz
         L.kb_attn_selfcheck.restype = i
         L.kb_attn_selfcheck.argtypes = [vp, sz, ctypes.POINTER(ctypes.c_float), vp]
+        L.kb_quant4_row_bytes.restype = i
+        L.kb_quant4_row_bytes.argtypes = [i]
+        L.kb_quant4_scale_bytes.restype = sz
+        L.kb_quant4_scale_bytes.argtypes = [i, i, i]
+        L.kb_quant4.restype = i
+        L.kb_quant4.argtypes = [vp, i, vp, vp, i, i, i, i, i, i, vp]
+        L.kb_dequant4.restype = i
+        L.kb_dequant4.argtypes = [vp, i, i, vp, i, vp, i, i, i, i, i, vp]
+        L.kb_linear4.restype = i
+        L.kb_linear4.argtypes = [vp, i, vp, vp, i, vp, vp, i, vp, i, i, i, i, i, f, vp, vp]
+        L.kb_linear4_dx_workspace_bytes.restype = sz
+        L.kb_linear4_dx_workspace_bytes.argtypes = [i, i]
+        L.kb_linear4_dx.restype = i
+        L.kb_linear4_dx.argtypes = [vp, i, i, vp, i, vp, i, vp, i, i, i, i, i, vp, sz, vp]
+        d = ctypes.c_double
+        L.kb_rope_freqs.restype = i
+        L.kb_rope_freqs.argtypes = [ctypes.POINTER(d), i, d, i, d, d, d, d]
+        L.kb_rope.restype = i
+        L.kb_rope.argtypes = [i, pvp, pi, pvp, pi, pi, i, i, i, i, i, vp, i, i, i, vp, vp, f, i, vp]
+        L.kb_dropout.restype = i
+        L.kb_dropout.argtypes = [vp, i, i, vp, i, i, vp, i, i, i, d, vp, vp]
         _lib = L
     return _lib
 
@@ -318,6 +339,154 @@ def cross_kv(k16, v16, ctx, Wk, Wv, kn_w=None, eps=1e-6, workspace=None):
     _check(lib().kb_cross_kv(_ptr(k16), _ptr(v16), _ld(k16), _ptr(ctx), _ld(ctx), _dt(ctx), L, N, K, _ptr(Wk), _ptr(Wv), _ld(Wk), _ptr(kn_w), eps,
                              _ptr(workspace), 0 if workspace is None else workspace.numel(), _stream()), "kb_cross_kv")
     return k16, v16
+
+
+def _here(*tensors):
+    """The calls below run on the current device: a tensor that lies elsewhere is refused before its address gets there."""
+    _stream()
+    dev = _cur_device()
+    for t in tensors:
+        if t is not None and t.get_device() != dev:
+            raise ValueError(f"tensor on {t.device}, but the current device is cuda:{dev}")
+
+
+def padded_empty(rows, cols, dtype, device):
+    """An uninitialised [rows, cols] matrix whose rows start on 16 bytes, as the products' outputs have to."""
+    import torch
+    step = 16 // torch.empty((), dtype=dtype).element_size()
+    return torch.empty(rows, -(-cols // step) * step, dtype=dtype, device=device)[:, :cols]
+
+
+MX4, NV4 = 0, 1
+EPI_GELU4 = 5
+
+
+class Quant4:
+    """A matrix [rows, cols] of 4-bit numbers in blocks (kb_quant4): codes uint8 [rows, >= 16 ceil(cols / 32)], scales uint8, fmt MX4 or NV4, 2^exp for all of it."""
+    __slots__ = ("codes", "scales", "rows", "cols", "fmt", "exp")
+
+    def __init__(self, codes, scales, rows, cols, fmt, exp=0):
+        if codes.element_size() != 1 or scales.element_size() != 1 or codes.dim() != 2 or not scales.is_contiguous():
+            raise ValueError("codes are a [rows, bytes] matrix of bytes, scales contiguous bytes")
+        if codes.shape[0] < rows or (codes.shape[1] > 1 and codes.stride(1) != 1) or codes.shape[1] < lib().kb_quant4_row_bytes(cols):
+            raise ValueError(f"codes {tuple(codes.shape)} do not hold {rows} rows of {cols} columns")
+        if rows and scales.numel() < lib().kb_quant4_scale_bytes(rows, cols, fmt):
+            raise ValueError(f"scales of {scales.numel()} bytes do not hold {rows} rows of {cols} columns")
+        self.codes, self.scales, self.rows, self.cols, self.fmt, self.exp = codes, scales, rows, cols, fmt, exp
+
+
+def quant4_empty(rows, cols, fmt, device, exp=0):
+    """Uninitialised buffers of a 4-bit matrix."""
+    import torch
+    return Quant4(torch.empty(rows, lib().kb_quant4_row_bytes(cols), dtype=torch.uint8, device=device),
+                  torch.empty(lib().kb_quant4_scale_bytes(rows, cols, fmt), dtype=torch.uint8, device=device), rows, cols, fmt, exp)
+
+
+def quant4(x, fmt, exp=0, out=None):
+    """x [rows, cols] fp16 / bf16 / fp32 as 4-bit numbers in blocks along the rows (see kb_quant4 for the two formats and exp)."""
+    rows, cols = x.shape
+    if out is None:
+        out = quant4_empty(rows, cols, fmt, x.device, exp)
+    elif (out.rows, out.cols, out.fmt, out.exp) != (rows, cols, fmt, exp):
+        raise ValueError("out was made for another matrix")
+    _here(x, out.codes, out.scales)
+    _check(lib().kb_quant4(_ptr(out.codes), out.codes.stride(0), _ptr(out.scales), _ptr(x), _ld(x), _dt(x), rows, cols, fmt, exp, _stream()), "kb_quant4")
+    return out
+
+
+def dequant4(y, q, transpose=False):
+    """y [rows, cols], or with transpose [cols, rows], fp16 / bf16 / fp32 = the values that q stands for."""
+    if tuple(y.shape) != ((q.cols, q.rows) if transpose else (q.rows, q.cols)):
+        raise ValueError(f"y {tuple(y.shape)} for a matrix of {q.rows} x {q.cols}")
+    _here(y, q.codes, q.scales)
+    _check(lib().kb_dequant4(_ptr(y), _ld(y), _dt(y), _ptr(q.codes), q.codes.stride(0), _ptr(q.scales), q.rows, q.cols, q.fmt, q.exp, int(transpose), _stream()),
+           "kb_dequant4")
+    return y
+
+
+def linear4(C, A, W, epi, gate=None, alpha=1.0):
+    """C = epilogue(alpha * A @ W.T) for 4-bit A [M, K] and W [N, K] (Quant4 of one format, their powers of two included): EPI_F32 / EPI_RESID into
+    an fp32 C, EPI_F16 / EPI_GELU16 into an fp16 C, EPI_GELU4 into a Quant4 C of the same format with exp 0."""
+    M, N, K = A.rows, W.rows, A.cols
+    if W.cols != K or W.fmt != A.fmt:
+        raise ValueError("A and W have to agree in columns and format")
+    four = isinstance(C, Quant4)
+    if four != (epi == EPI_GELU4) or ((C.rows, C.cols) if four else tuple(C.shape)) != (M, N) or (four and (C.fmt, C.exp) != (A.fmt, 0)):
+        raise ValueError("C does not fit the product or its epilogue")
+    if not four and _dt(C) != (KB_F32 if epi in (EPI_F32, EPI_RESID) else KB_F16):
+        raise ValueError("C has another type than its epilogue")
+    if gate is not None and (_dt(gate) != KB_F32 or gate.numel() < N or not gate.is_contiguous()):
+        raise ValueError("gate is fp32 [N]")
+    out, scales = (C.codes, C.scales) if four else (C, None)
+    _here(out, scales, A.codes, A.scales, W.codes, W.scales, gate)
+    _check(lib().kb_linear4(_ptr(out), out.stride(0) if four else _ld(out), _ptr(scales), _ptr(A.codes), A.codes.stride(0), _ptr(A.scales), _ptr(W.codes),
+                            W.codes.stride(0), _ptr(W.scales), M, N, K, A.fmt, epi, alpha * 2.0 ** (A.exp + W.exp), _ptr(gate), _stream()), "kb_linear4")
+    return C
+
+
+def linear4_dx(dx, dy, W, workspace=None):
+    """dx [M, K] (fp16 or fp32) = dy [M, N] @ W for a 4-bit W [N, K]: the gradient of linear4's input. dy fp16."""
+    import torch
+    M, N = dy.shape
+    if N != W.rows or tuple(dx.shape) != (M, W.cols) or _dt(dy) != KB_F16:
+        raise ValueError("dy is fp16 [M, N], dx [M, K] for a weight of [N, K]")
+    if workspace is None:
+        workspace = torch.empty(lib().kb_linear4_dx_workspace_bytes(N, W.cols), dtype=torch.uint8, device=dy.device)
+    _here(dx, dy, W.codes, W.scales, workspace)
+    wp, wb = _ws(workspace)
+    _check(lib().kb_linear4_dx(_ptr(dx), _ld(dx), _dt(dx), _ptr(dy), _ld(dy), _ptr(W.codes), W.codes.stride(0), _ptr(W.scales), M, N, W.cols, W.fmt, W.exp,
+                               wp, wb, _stream()), "kb_linear4_dx")
+    return dx
+
+
+ROPE_HALF, ROPE_INTERLEAVED = 0, 1
+ROPE_PLAIN, ROPE_LINEAR, ROPE_BASE, ROPE_PARTS = 0, 1, 2, 3
+
+
+def rope_freqs(rot_dim, base=10000.0, scaling=ROPE_PLAIN, factor=1.0, trained_len=0.0, slow_turns=1.0, fast_turns=32.0):
+    """Radians per position of every pair, float64 [rot_dim / 2] on the host; see kb_rope_freqs for the ways to stretch a context."""
+    import numpy as np
+    freq = np.empty(max(rot_dim, 0) // 2, np.float64)
+    _check(lib().kb_rope_freqs(freq.ctypes.data_as(ctypes.POINTER(ctypes.c_double)), rot_dim, base, scaling, factor, trained_len, slow_turns, fast_turns),
+           "kb_rope_freqs")
+    return freq
+
+
+def rope(outs, xs, heads, head_dim, pos, freq, axis=None, layout=ROPE_HALF, amplitude=1.0, inverse=False):
+    """Rotary positions of up to four tensors xs[k] [rows, heads[k] * head_dim] of one type in one launch; outs may be xs. pos: int32 [pos_rows, axes] on the
+    device (row r takes pos[r % pos_rows]); freq (float64) and axis (int32 or None), one entry per pair, numpy arrays on the host. inverse = the gradient."""
+    import numpy as np
+    import torch
+    n = len(xs)
+    if len(outs) != n or len(heads) != n or not n:
+        raise ValueError("one output and one number of heads per tensor")
+    rows = xs[0].shape[0]
+    for o, x, h in zip(outs, xs, heads):
+        if x.shape[0] != rows or x.shape[1] < h * head_dim or o.shape[0] != rows or o.shape[1] < h * head_dim or o.dtype != x.dtype or x.dtype != xs[0].dtype:
+            raise ValueError("tensors are [rows, heads * head_dim] of one type")
+    if pos.dtype != torch.int32 or pos.dim() != 2 or (pos.shape[1] > 1 and pos.stride(1) != 1):
+        raise ValueError("pos is int32 [rows, axes]")
+    if freq.dtype != np.float64 or not freq.flags.c_contiguous or (axis is not None and (axis.dtype != np.int32 or not axis.flags.c_contiguous or axis.size != freq.size)):
+        raise ValueError("freq is float64 and axis int32, one per pair")
+    _here(pos, *outs, *xs)
+    vpn, in_ = ctypes.c_void_p * n, ctypes.c_int * n
+    _check(lib().kb_rope(n, vpn(*[o.data_ptr() for o in outs]), in_(*[_ld(o) for o in outs]), vpn(*[x.data_ptr() for x in xs]), in_(*[_ld(x) for x in xs]),
+                         in_(*heads), _dt(xs[0]), rows, head_dim, 2 * freq.size, layout, _ptr(pos), pos.shape[0], pos.stride(0), pos.shape[1], freq.ctypes.data,
+                         None if axis is None else axis.ctypes.data, amplitude, int(inverse), _stream()), "kb_rope")
+    return outs
+
+
+def dropout(out, x, rng, p, resid=None):
+    """out = dropout(x) (+ resid); rng: int64 [2] on the device, seed and offset. The gradient is dropout(dout) with the same rng (see kb_dropout)."""
+    import torch
+    if tuple(out.shape) != tuple(x.shape) or (resid is not None and (tuple(resid.shape) != tuple(x.shape) or resid.dtype != out.dtype)):
+        raise ValueError("out, x and resid have one shape, out and resid one type")
+    if rng.dtype not in (torch.int64, torch.uint64) or rng.numel() != 2 or not rng.is_contiguous():
+        raise ValueError("rng is int64 [2]: seed and offset")
+    _here(out, x, rng, resid)
+    _check(lib().kb_dropout(_ptr(out), _ld(out), _dt(out), _ptr(x), _ld(x), _dt(x), _ptr(resid), 0 if resid is None else _ld(resid), x.shape[0], x.shape[1], p,
+                            _ptr(rng), _stream()), "kb_dropout")
+    return out
 
 
 def check_status():

@@ -92,8 +92,10 @@ int set_gemm_smem() {
 template <int EPI>
 int set_gemm4_smem() {
     int rc;
-    if ((rc = set_smem(gemm4_kernel<EPI, FMT_MX4>, G4_SMEM))) return rc;
-    return set_smem(gemm4_kernel<EPI, FMT_NV4>, G4_SMEM);
+    if ((rc = set_smem(gemm4_kernel<EPI, FMT_MX4, false>, G4_SMEM)) || (rc = set_smem(gemm4_kernel<EPI, FMT_NV4, false>, G4_SMEM)) ||
+        (rc = set_smem(gemm4_kernel<EPI, FMT_MX4, true>, G4_SMEM)))
+        return rc;
+    return set_smem(gemm4_kernel<EPI, FMT_NV4, true>, G4_SMEM);
 }
 
 int init_device(DeviceState& st, int dev) {
@@ -1059,14 +1061,24 @@ int make_tmap_scales(CUtensorMap* tm, const void* ptr, int rows, int cols, int f
     return r == CUDA_SUCCESS ? KB_OK : KB_ERR_CUDA;
 }
 
-template <int EPI, int FMT>
-int launch_gemm4(DeviceState* st, const Gemm4Maps& maps, Gemm4Params p, cudaStream_t stream) {
-    p.tiles_m = (p.M + 127) / 128;
-    p.tiles_n = (p.N + 127) / 128;
+template <int EPI, int FMT, bool PAIR>
+int launch_gemm4_shape(DeviceState* st, const Gemm4Maps& maps, Gemm4Params p, cudaStream_t stream) {
+    constexpr int TILE = PAIR ? 256 : 128, CTAS = PAIR ? 2 : 1;
+    p.tiles_m = (p.M + TILE - 1) / TILE;
+    p.tiles_n = (p.N + TILE - 1) / TILE;
     const long long n_tiles = (long long)p.tiles_m * p.tiles_n;
     if (n_tiles > 0x3fffffffLL) return KB_ERR_SHAPE;
-    const unsigned grid = (unsigned)(n_tiles < st->sm_count ? n_tiles : st->sm_count);
-    return launch_dependent(gemm4_kernel<EPI, FMT>, dim3(grid), dim3(G_THREADS), G4_SMEM, stream, nullptr, maps, p);
+    const int max_groups = st->sm_count / CTAS, groups = n_tiles < max_groups ? (int)n_tiles : max_groups;
+    cudaLaunchAttribute cluster;
+    cluster.id = cudaLaunchAttributeClusterDimension;
+    cluster.val.clusterDim.x = CTAS; cluster.val.clusterDim.y = 1; cluster.val.clusterDim.z = 1;
+    return launch_dependent(gemm4_kernel<EPI, FMT, PAIR>, dim3((unsigned)(groups * CTAS)), dim3(G_THREADS), G4_SMEM, stream, PAIR ? &cluster : nullptr, maps, p);
+}
+
+template <int EPI, int FMT>
+int launch_gemm4(DeviceState* st, const Gemm4Maps& maps, const Gemm4Params& p, cudaStream_t stream) {
+    if (gemm4_pair(p.M, p.N, (p.K + G4_K - 1) / G4_K, st->sm_count)) return launch_gemm4_shape<EPI, FMT, true>(st, maps, p, stream);
+    return launch_gemm4_shape<EPI, FMT, false>(st, maps, p, stream);
 }
 
 template <int FMT>

@@ -5,6 +5,11 @@
 // The schedule is that of the fp16 product next door (gemm_sm100.cuh): persistent CTAs, one warp loads by TMA, one issues, eight run the epilogue of one
 // tile under the main loop of the next. What differs: a k step in shared memory holds 256 columns (128 bytes) of each operand, plus their scales
 // (2 KB per 128 rows for NV4, 1 KB for MX4), which tcgen05.cp copies to TMEM in front of the step's products, four lanes' quarters at a time.
+//
+// Two shapes. Single: one CTA per 128 x 128 tile. PAIR: two CTAs share a 256 x 256 tile (cta_group::2), each with its 128 rows of A, half of the W rows,
+// the scales of its rows and of ALL 256 columns, and its 128 x 256 half of the accumulator. Two such accumulators fill TMEM and leave no room for
+// scales, so they overlap: the first lies in columns [0, 256), the second in [128, 384), the scales behind them. The epilogue drains the 128 columns that
+// both own first, and then the next tile's products may begin: half of the epilogue still runs under them.
 #pragma once
 #include "gemm_sm100.cuh"   // gelu, elect_one, pack16
 #include "quant4.cuh"
@@ -105,15 +110,15 @@ __device__ __forceinline__ void quant32(const float* v, uint4& codes, uint32_t& 
     codes = make_uint4(words[0], words[1], words[2], words[3]);
 }
 
-template <int EPI, int FMT>
+template <int EPI, int FMT, bool PAIR>
 __global__ void __launch_bounds__(G_THREADS, 1)
 gemm4_kernel(const __grid_constant__ Gemm4Maps maps, const Gemm4Params p) {
-    constexpr bool PAIR = false;
-    constexpr int BN = 128, TILE_M = 128;
-    constexpr int BUF_COLS = 128, ACC_SF = 2 * BUF_COLS;                  // TMEM: two accumulators, then the scales
+    constexpr int BN = PAIR ? 256 : 128, TILE_M = PAIR ? 256 : 128;
+    constexpr int BUF_COLS = 128, ACC_SF = BUF_COLS + BN;                 // TMEM: the second accumulator begins at BUF_COLS, the scales behind it
     constexpr int PIECES = FMT == FMT_MX4 ? 2 : 4;                        // scale pieces of a k step per row block
     constexpr int W_BLOCKS = BN / 128;                                    // row blocks of W whose scales a CTA holds
-    constexpr int SF_COLS = 4 * PIECES * (1 + W_BLOCKS), SF_BUFS = 4;     // TMEM columns of a step's scales; steps of them in flight
+    constexpr int SF_COLS = 4 * PIECES * (1 + W_BLOCKS);                  // TMEM columns of a step's scales
+    constexpr int SF_BUFS = PAIR && FMT == FMT_NV4 ? 2 : 4;               // steps of them in flight
     static_assert(ACC_SF + SF_BUFS * SF_COLS <= (int)TMEM_ALL_COLUMNS, "TMEM");
     constexpr uint32_t STAGE_TX = 32768 + PIECES * 512 * (1 + W_BLOCKS);
     constexpr bool OUT32 = EPI == EPI_F32 || EPI == EPI_RESID;
@@ -131,11 +136,12 @@ gemm4_kernel(const __grid_constant__ Gemm4Maps maps, const Gemm4Params p) {
     auto bar = [&](int i) { return bars + 8u * (uint32_t)i; };
 
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-    const int group = (int)blockIdx.x, n_groups = (int)gridDim.x;
+    const uint32_t rank = PAIR ? cluster_ctarank() : 0u;                  // 0 issues the MMAs
+    const int group = (int)blockIdx.x / (PAIR ? 2 : 1), n_groups = (int)gridDim.x / (PAIR ? 2 : 1);
     const int n_tiles = p.tiles_m * p.tiles_n, ksteps = (p.K + G4_K - 1) / G4_K;
 
     if (tid == 0) {
-        for (int i = 0; i < G4BAR_COUNT; i++) mbar_init(bar(i), i >= G4BAR_ACC_EMPTY ? G_EPI_WARPS : 1u);
+        for (int i = 0; i < G4BAR_COUNT; i++) mbar_init(bar(i), i >= G4BAR_ACC_EMPTY ? (PAIR ? 2u : 1u) * G_EPI_WARPS : 1u);   // acc_empty: one arrival per epilogue warp of the group
         *abort_flag = 0u;
         mbar_fence_init();
         fence_proxy_async_smem();
@@ -147,7 +153,7 @@ gemm4_kernel(const __grid_constant__ Gemm4Maps maps, const Gemm4Params p) {
     }
     pdl_launch();
     tc_fence_before();
-    __syncthreads();
+    if (PAIR) { cluster_arrive(); cluster_wait(); } else __syncthreads();
     tc_fence_after();
     constexpr uint32_t tmem_base = 0u;                                    // see TMEM_ALL_COLUMNS
     pdl_wait();
@@ -163,14 +169,15 @@ gemm4_kernel(const __grid_constant__ Gemm4Maps maps, const Gemm4Params p) {
             const int buf = k & 1;
             int tm, tn;
             gemm4_tile(w, p, tm, tn);
-            const int m0 = tm * TILE_M, n0 = tn * BN;
+            const int m0 = tm * TILE_M + (int)rank * GB_M, n0 = tn * BN;
             const bool ok = __all_sync(0xffffffffu, mbar_wait(bar(G4BAR_ACC_FULL + buf), use[buf] & 1u, abort_flag));
             ++use[buf];
             if (!ok) break;
             tc_fence_after();
             const int row = m0 + quarter * 32 + lane, nrow = p.M - (m0 + quarter * 32);
 #pragma unroll 1
-            for (int ch = half; ch < NCH; ch += 2) {
+            for (int i = 0; i < NCH / 2; i++) {
+                const int ch = half + 2 * (PAIR ? i ^ buf ^ 1 : i);       // PAIR: the columns that both accumulators own first
                 float v[CW];
                 {
                     uint32_t a[CW / 32][32];
@@ -184,10 +191,13 @@ gemm4_kernel(const __grid_constant__ Gemm4Maps maps, const Gemm4Params p) {
                         for (int e = 0; e < 32; e++) v[32 * q + e] = __uint_as_float(a[q][e]) * p.alpha;
                     }
                 }
-                if (ch + 2 >= NCH) {                                      // the last chunk of this warp is in registers
+                if (i == 0) {                                             // single: the only chunk; the next tile's products may come
                     tc_fence_before();
                     __syncwarp();
-                    if (lane == 0) mbar_arrive(bar(G4BAR_ACC_EMPTY + buf));
+                    if (lane == 0) {
+                        if (PAIR && rank != 0) mbar_arrive_cluster(mapa_u32(bar(G4BAR_ACC_EMPTY), 0));
+                        else mbar_arrive(bar(G4BAR_ACC_EMPTY + (PAIR ? 0 : buf)));
+                    }
                 }
                 const int c0 = n0 + ch * CW;
                 if constexpr (EPI == EPI_GELU16 || EPI == EPI_GELU4) {
@@ -275,13 +285,18 @@ gemm4_kernel(const __grid_constant__ Gemm4Maps maps, const Gemm4Params p) {
         if (lane == 0) tma_store_wait_read();
     } else if (warp == G_EPI_WARPS) {
         setmaxnreg_dec<56>();
-        if (elect_one()) {
+        if (rank == 0 && elect_one()) {
             uint32_t ring = 0, use[2] = {0, 0};
             bool good = true;
             int k = 0;
             for (int w = group; w < n_tiles && good; w += n_groups, ++k) {
                 const int buf = k & 1;
-                good = mbar_wait(bar(G4BAR_ACC_EMPTY + buf), (use[buf] & 1u) ^ 1u, abort_flag);   // passes at once for the first two tiles
+                if (PAIR) {
+                    // the tile before this one is out of the shared columns, so the one before that is out of all of its own
+                    if (k > 0) good = mbar_wait(bar(G4BAR_ACC_EMPTY), (uint32_t)(k - 1) & 1u, abort_flag);
+                } else {
+                    good = mbar_wait(bar(G4BAR_ACC_EMPTY + buf), (use[buf] & 1u) ^ 1u, abort_flag);   // passes at once for the first two tiles
+                }
                 ++use[buf];
                 if (!good) break;
                 tc_fence_after();
@@ -308,9 +323,9 @@ gemm4_kernel(const __grid_constant__ Gemm4Maps maps, const Gemm4Params p) {
                         mma_f4<FMT, PAIR>(tmem_base + (uint32_t)(buf * BUF_COLS), adesc + (uint64_t)(kk * 2), wdesc + (uint64_t)(kk * 2),
                                           idesc_f4(FMT == FMT_MX4, TILE_M, BN, byte), sfa + 4 * q, sfb + 4 * q * W_BLOCKS, (ks > 0 || kk > 0) ? 1u : 0u);
                     }
-                    tc_commit(bar(G4BAR_EMPTY + st));
+                    if (PAIR) tc_commit_pair(bar(G4BAR_EMPTY + st), (uint16_t)3); else tc_commit(bar(G4BAR_EMPTY + st));
                 }
-                if (good) tc_commit(bar(G4BAR_ACC_FULL + buf));
+                if (good) { if (PAIR) tc_commit_pair(bar(G4BAR_ACC_FULL + buf), (uint16_t)3); else tc_commit(bar(G4BAR_ACC_FULL + buf)); }
             }
         }
         __syncwarp();
@@ -326,22 +341,40 @@ gemm4_kernel(const __grid_constant__ Gemm4Maps maps, const Gemm4Params p) {
                     const uint32_t st = ring % G4_STAGES;
                     good = mbar_wait(bar(G4BAR_EMPTY + st), ((ring / G4_STAGES) & 1u) ^ 1u, abort_flag);
                     if (!good) break;
-                    const uint32_t a_s = base + st * G4_STAGE_BYTES, fb = bar(G4BAR_FULL + st);
-                    mbar_expect_tx(fb, STAGE_TX);
-                    tma_load_3d(a_s, &maps.a, fb, ks * 128, tm * TILE_M, 0);
-                    tma_load_3d(a_s + 16384, &maps.w, fb, ks * 128, tn * BN, 0);
-                    tma_load_3d(a_s + G4_SF_OFF, &maps.sa, fb, 0, ks * PIECES, tm);
+                    const uint32_t a_s = base + st * G4_STAGE_BYTES, s_s = a_s + G4_SF_OFF;
+                    if (PAIR) {
+                        // both CTAs' bytes complete on the issuing CTA's barrier
+                        if (rank == 0) mbar_expect_tx(bar(G4BAR_FULL + st), 2 * STAGE_TX);
+                        const uint32_t fb = mapa_u32(bar(G4BAR_FULL + st), 0);
+                        tma_load_3d_pair(a_s, &maps.a, fb, ks * 128, tm * TILE_M + (int)rank * 128, 0);
+                        tma_load_3d_pair(a_s + 16384, &maps.w, fb, ks * 128, tn * BN + (int)rank * 128, 0);
+                        tma_load_3d_pair(s_s, &maps.sa, fb, 0, ks * PIECES, tm * 2 + (int)rank);
 #pragma unroll
-                    for (int b = 0; b < W_BLOCKS; b++) tma_load_3d(a_s + G4_SF_OFF + PIECES * 512 * (1 + b), &maps.sw, fb, 0, ks * PIECES, tn * W_BLOCKS + b);
+                        for (int b = 0; b < W_BLOCKS; b++) tma_load_3d_pair(s_s + PIECES * 512 * (1 + b), &maps.sw, fb, 0, ks * PIECES, tn * W_BLOCKS + b);
+                    } else {
+                        const uint32_t fb = bar(G4BAR_FULL + st);
+                        mbar_expect_tx(fb, STAGE_TX);
+                        tma_load_3d(a_s, &maps.a, fb, ks * 128, tm * TILE_M, 0);
+                        tma_load_3d(a_s + 16384, &maps.w, fb, ks * 128, tn * BN, 0);
+                        tma_load_3d(s_s, &maps.sa, fb, 0, ks * PIECES, tm);
+                        tma_load_3d(s_s + PIECES * 512, &maps.sw, fb, 0, ks * PIECES, tn);
+                    }
                 }
             }
-            if (!good || *abort_flag)                                     // let the copies already requested land before the memory goes away
-                for (uint32_t k = ring > (uint32_t)G4_STAGES ? ring - G4_STAGES : 0u; k < ring; ++k) drain_wait(bar(G4BAR_FULL + k % G4_STAGES), (k / G4_STAGES) & 1u);
+            if (!good || *abort_flag) {
+                // let the copies already requested land before the memory goes away, as in gemm16_kernel
+                if (!PAIR || rank == 0) {
+                    for (uint32_t k = ring > (uint32_t)G4_STAGES ? ring - G4_STAGES : 0u; k < ring; ++k) drain_wait(bar(G4BAR_FULL + k % G4_STAGES), (k / G4_STAGES) & 1u);
+                } else {
+                    const uint64_t t0 = globaltimer_ns();
+                    while (globaltimer_ns() - t0 < 20000ull) {}
+                }
+            }
         }
         __syncwarp();
     }
     tc_fence_before();
-    __syncthreads();
+    if (PAIR) { cluster_arrive(); cluster_wait(); } else __syncthreads();
     if (warp == G_EPI_WARPS) {
         if (lane == 0 && *abort_flag) atomicOr(p.status, ST_TIMEOUT);
         tc_fence_after();

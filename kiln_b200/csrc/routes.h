@@ -193,4 +193,14 @@ inline GemmShape gemm_shape(int M, int N, long long ksteps, int n_seg, bool any_
     return g;
 }
 
+#ifndef KB_G4
+#define KB_G4 -1
+#endif
+inline bool gemm4_pair(int M, int N, int ksteps, int sm_count) {
+    if (KB_G4 >= 0) return KB_G4;
+    const long long single = (((long long)(M + 127) / 128) * ((N + 127) / 128) + sm_count - 1) / sm_count;
+    const long long pair = (((long long)(M + 255) / 256) * ((N + 255) / 256) + sm_count / 2 - 1) / (sm_count / 2);
+    return M > 128 && 16 * pair < 10 * single;
+}
+
 }  // namespace kb

@@ -341,24 +341,40 @@ def cross_kv(k16, v16, ctx, Wk, Wv, kn_w=None, eps=1e-6, workspace=None):
     return k16, v16
 
 
-def _here(*tensors):
+def _here(stream_device, *tensors):
     """The calls below run on the current device: a tensor that lies elsewhere is refused before its address gets there."""
-    _stream()
-    dev = _cur_device()
     for t in tensors:
-        if t is not None and t.get_device() != dev:
-            raise ValueError(f"tensor on {t.device}, but the current device is cuda:{dev}")
+        if t is not None and t.get_device() != stream_device:
+            raise ValueError(f"tensor on {t.device}, but the current device is cuda:{stream_device}")
+
+
+def _stream_device():
+    """(raw handle of the current stream, current device)"""
+    handle = _stream()
+    return handle, _cur_device()
 
 
 def padded_empty(rows, cols, dtype, device):
     """An uninitialised [rows, cols] matrix whose rows start on 16 bytes, as the products' outputs have to."""
     import torch
-    step = 16 // torch.empty((), dtype=dtype).element_size()
-    return torch.empty(rows, -(-cols // step) * step, dtype=dtype, device=device)[:, :cols]
+    step = 16 // dtype.itemsize
+    if cols % step == 0:
+        return torch.empty((rows, cols), dtype=dtype, device=device)
+    return torch.empty((rows, (cols // step + 1) * step), dtype=dtype, device=device)[:, :cols]
 
 
 MX4, NV4 = 0, 1
 EPI_GELU4 = 5
+
+
+MAX_Q4_COLS = 1 << 24
+
+
+def _q4_bytes(rows, cols, fmt):
+    """(bytes of a row of codes, bytes of the scales): kb_quant4_row_bytes and kb_quant4_scale_bytes without a call"""
+    if rows < 0 or not 0 < cols <= MAX_Q4_COLS or fmt not in (MX4, NV4):
+        raise ValueError(f"no 4-bit matrix of {rows} x {cols}, format {fmt}")
+    return (cols + 31) // 32 * 16, (rows + 127) // 128 * ((cols + 63) // 64 if fmt else (cols + 127) // 128) * 512
 
 
 class Quant4:
@@ -366,11 +382,13 @@ class Quant4:
     __slots__ = ("codes", "scales", "rows", "cols", "fmt", "exp")
 
     def __init__(self, codes, scales, rows, cols, fmt, exp=0):
-        if codes.element_size() != 1 or scales.element_size() != 1 or codes.dim() != 2 or not scales.is_contiguous():
+        row_bytes, scale_bytes = _q4_bytes(rows, cols, fmt)
+        have, st = codes.shape, codes.stride()
+        if codes.element_size() != 1 or scales.element_size() != 1 or len(have) != 2 or not scales.is_contiguous():
             raise ValueError("codes are a [rows, bytes] matrix of bytes, scales contiguous bytes")
-        if codes.shape[0] < rows or (codes.shape[1] > 1 and codes.stride(1) != 1) or codes.shape[1] < lib().kb_quant4_row_bytes(cols):
-            raise ValueError(f"codes {tuple(codes.shape)} do not hold {rows} rows of {cols} columns")
-        if rows and scales.numel() < lib().kb_quant4_scale_bytes(rows, cols, fmt):
+        if have[0] < rows or have[1] < row_bytes or st[1] != 1:
+            raise ValueError(f"codes {tuple(have)} do not hold {rows} rows of {cols} columns")
+        if scales.numel() < scale_bytes:
             raise ValueError(f"scales of {scales.numel()} bytes do not hold {rows} rows of {cols} columns")
         self.codes, self.scales, self.rows, self.cols, self.fmt, self.exp = codes, scales, rows, cols, fmt, exp
 
@@ -378,8 +396,12 @@ class Quant4:
 def quant4_empty(rows, cols, fmt, device, exp=0):
     """Uninitialised buffers of a 4-bit matrix."""
     import torch
-    return Quant4(torch.empty(rows, lib().kb_quant4_row_bytes(cols), dtype=torch.uint8, device=device),
-                  torch.empty(lib().kb_quant4_scale_bytes(rows, cols, fmt), dtype=torch.uint8, device=device), rows, cols, fmt, exp)
+    row_bytes, scale_bytes = _q4_bytes(rows, cols, fmt)
+    q = Quant4.__new__(Quant4)                     # what is made here needs no checks
+    q.codes = torch.empty((rows, row_bytes), dtype=torch.uint8, device=device)
+    q.scales = torch.empty(scale_bytes, dtype=torch.uint8, device=device)
+    q.rows, q.cols, q.fmt, q.exp = rows, cols, fmt, exp
+    return q
 
 
 def quant4(x, fmt, exp=0, out=None):
@@ -389,8 +411,10 @@ def quant4(x, fmt, exp=0, out=None):
         out = quant4_empty(rows, cols, fmt, x.device, exp)
     elif (out.rows, out.cols, out.fmt, out.exp) != (rows, cols, fmt, exp):
         raise ValueError("out was made for another matrix")
-    _here(x, out.codes, out.scales)
-    _check(lib().kb_quant4(_ptr(out.codes), out.codes.stride(0), _ptr(out.scales), _ptr(x), _ld(x), _dt(x), rows, cols, fmt, exp, _stream()), "kb_quant4")
+    stream, dev = _stream_device()
+    codes, scales = out.codes, out.scales
+    _here(dev, x, codes, scales)
+    _check(lib().kb_quant4(codes.data_ptr(), codes.stride(0), scales.data_ptr(), x.data_ptr(), _ld(x), _dt(x), rows, cols, fmt, exp, stream), "kb_quant4")
     return out
 
 
@@ -398,8 +422,9 @@ def dequant4(y, q, transpose=False):
     """y [rows, cols], or with transpose [cols, rows], fp16 / bf16 / fp32 = the values that q stands for."""
     if tuple(y.shape) != ((q.cols, q.rows) if transpose else (q.rows, q.cols)):
         raise ValueError(f"y {tuple(y.shape)} for a matrix of {q.rows} x {q.cols}")
-    _here(y, q.codes, q.scales)
-    _check(lib().kb_dequant4(_ptr(y), _ld(y), _dt(y), _ptr(q.codes), q.codes.stride(0), _ptr(q.scales), q.rows, q.cols, q.fmt, q.exp, int(transpose), _stream()),
+    stream, dev = _stream_device()
+    _here(dev, y, q.codes, q.scales)
+    _check(lib().kb_dequant4(_ptr(y), _ld(y), _dt(y), _ptr(q.codes), q.codes.stride(0), _ptr(q.scales), q.rows, q.cols, q.fmt, q.exp, int(transpose), stream),
            "kb_dequant4")
     return y
 
@@ -410,17 +435,23 @@ def linear4(C, A, W, epi, gate=None, alpha=1.0):
     M, N, K = A.rows, W.rows, A.cols
     if W.cols != K or W.fmt != A.fmt:
         raise ValueError("A and W have to agree in columns and format")
-    four = isinstance(C, Quant4)
-    if four != (epi == EPI_GELU4) or ((C.rows, C.cols) if four else tuple(C.shape)) != (M, N) or (four and (C.fmt, C.exp) != (A.fmt, 0)):
-        raise ValueError("C does not fit the product or its epilogue")
-    if not four and _dt(C) != (KB_F32 if epi in (EPI_F32, EPI_RESID) else KB_F16):
-        raise ValueError("C has another type than its epilogue")
+    if epi == EPI_GELU4:
+        if not isinstance(C, Quant4) or (C.rows, C.cols, C.fmt, C.exp) != (M, N, A.fmt, 0):
+            raise ValueError("EPI_GELU4 goes into a Quant4 [M, N] of the operands' format with exp 0")
+        out, scales = C.codes, C.scales
+        ldc = out.stride(0)
+    else:
+        out, scales = C, None
+        if isinstance(C, Quant4) or C.shape != (M, N) or _dt(C) != (KB_F32 if epi in (EPI_F32, EPI_RESID) else KB_F16):
+            raise ValueError("C is [M, N] of its epilogue's type")
+        ldc = _ld(C)
     if gate is not None and (_dt(gate) != KB_F32 or gate.numel() < N or not gate.is_contiguous()):
         raise ValueError("gate is fp32 [N]")
-    out, scales = (C.codes, C.scales) if four else (C, None)
-    _here(out, scales, A.codes, A.scales, W.codes, W.scales, gate)
-    _check(lib().kb_linear4(_ptr(out), out.stride(0) if four else _ld(out), _ptr(scales), _ptr(A.codes), A.codes.stride(0), _ptr(A.scales), _ptr(W.codes),
-                            W.codes.stride(0), _ptr(W.scales), M, N, K, A.fmt, epi, alpha * 2.0 ** (A.exp + W.exp), _ptr(gate), _stream()), "kb_linear4")
+    stream, dev = _stream_device()
+    a, sa, w, sw = A.codes, A.scales, W.codes, W.scales
+    _here(dev, out, scales, a, sa, w, sw, gate)
+    _check(lib().kb_linear4(out.data_ptr(), ldc, _ptr(scales), a.data_ptr(), a.stride(0), sa.data_ptr(), w.data_ptr(), w.stride(0), sw.data_ptr(), M, N, K, A.fmt,
+                            epi, alpha * 2.0 ** (A.exp + W.exp), _ptr(gate), stream), "kb_linear4")
     return C
 
 
@@ -432,10 +463,11 @@ def linear4_dx(dx, dy, W, workspace=None):
         raise ValueError("dy is fp16 [M, N], dx [M, K] for a weight of [N, K]")
     if workspace is None:
         workspace = torch.empty(lib().kb_linear4_dx_workspace_bytes(N, W.cols), dtype=torch.uint8, device=dy.device)
-    _here(dx, dy, W.codes, W.scales, workspace)
+    stream, dev = _stream_device()
+    _here(dev, dx, dy, W.codes, W.scales, workspace)
     wp, wb = _ws(workspace)
     _check(lib().kb_linear4_dx(_ptr(dx), _ld(dx), _dt(dx), _ptr(dy), _ld(dy), _ptr(W.codes), W.codes.stride(0), _ptr(W.scales), M, N, W.cols, W.fmt, W.exp,
-                               wp, wb, _stream()), "kb_linear4_dx")
+                               wp, wb, stream), "kb_linear4_dx")
     return dx
 
 
@@ -468,24 +500,26 @@ def rope(outs, xs, heads, head_dim, pos, freq, axis=None, layout=ROPE_HALF, ampl
         raise ValueError("pos is int32 [rows, axes]")
     if freq.dtype != np.float64 or not freq.flags.c_contiguous or (axis is not None and (axis.dtype != np.int32 or not axis.flags.c_contiguous or axis.size != freq.size)):
         raise ValueError("freq is float64 and axis int32, one per pair")
-    _here(pos, *outs, *xs)
+    stream, dev = _stream_device()
+    _here(dev, pos, *outs, *xs)
     vpn, in_ = ctypes.c_void_p * n, ctypes.c_int * n
     _check(lib().kb_rope(n, vpn(*[o.data_ptr() for o in outs]), in_(*[_ld(o) for o in outs]), vpn(*[x.data_ptr() for x in xs]), in_(*[_ld(x) for x in xs]),
-                         in_(*heads), _dt(xs[0]), rows, head_dim, 2 * freq.size, layout, _ptr(pos), pos.shape[0], pos.stride(0), pos.shape[1], freq.ctypes.data,
-                         None if axis is None else axis.ctypes.data, amplitude, int(inverse), _stream()), "kb_rope")
+                         in_(*heads), _dt(xs[0]), rows, head_dim, 2 * freq.size, layout, _ptr(pos), pos.shape[0], pos.stride(0), pos.shape[1], freq.__array_interface__["data"][0],
+                         None if axis is None else axis.__array_interface__["data"][0], amplitude, int(inverse), stream), "kb_rope")
     return outs
 
 
 def dropout(out, x, rng, p, resid=None):
     """out = dropout(x) (+ resid); rng: int64 [2] on the device, seed and offset. The gradient is dropout(dout) with the same rng (see kb_dropout)."""
     import torch
-    if tuple(out.shape) != tuple(x.shape) or (resid is not None and (tuple(resid.shape) != tuple(x.shape) or resid.dtype != out.dtype)):
+    if out.shape != x.shape or (resid is not None and (resid.shape != x.shape or resid.dtype != out.dtype)):
         raise ValueError("out, x and resid have one shape, out and resid one type")
     if rng.dtype not in (torch.int64, torch.uint64) or rng.numel() != 2 or not rng.is_contiguous():
         raise ValueError("rng is int64 [2]: seed and offset")
-    _here(out, x, rng, resid)
+    stream, dev = _stream_device()
+    _here(dev, out, x, rng, resid)
     _check(lib().kb_dropout(_ptr(out), _ld(out), _dt(out), _ptr(x), _ld(x), _dt(x), _ptr(resid), 0 if resid is None else _ld(resid), x.shape[0], x.shape[1], p,
-                            _ptr(rng), _stream()), "kb_dropout")
+                            _ptr(rng), stream), "kb_dropout")
     return out
 
 

@@ -92,10 +92,11 @@ int set_gemm_smem() {
 template <int EPI>
 int set_gemm4_smem() {
     int rc;
-    if ((rc = set_smem(gemm4_kernel<EPI, FMT_MX4, false>, G4_SMEM)) || (rc = set_smem(gemm4_kernel<EPI, FMT_NV4, false>, G4_SMEM)) ||
-        (rc = set_smem(gemm4_kernel<EPI, FMT_MX4, true>, G4_SMEM)))
+    if ((rc = set_smem(gemm4_kernel<EPI, FMT_MX4, 128>, G4_SMEM)) || (rc = set_smem(gemm4_kernel<EPI, FMT_NV4, 128>, G4_SMEM)) ||
+        (rc = set_smem(gemm4_kernel<EPI, FMT_MX4, 192>, G4_SMEM)) || (rc = set_smem(gemm4_kernel<EPI, FMT_NV4, 192>, G4_SMEM)) ||
+        (rc = set_smem(gemm4_kernel<EPI, FMT_MX4, 256>, G4_SMEM)))
         return rc;
-    return set_smem(gemm4_kernel<EPI, FMT_NV4, true>, G4_SMEM);
+    return set_smem(gemm4_kernel<EPI, FMT_NV4, 256>, G4_SMEM);
 }
 
 int init_device(DeviceState& st, int dev) {
@@ -1039,11 +1040,11 @@ int launch_dequant4(Quant4Params& p, int dtype, bool transpose, cudaStream_t str
     return launch_dequant4_t<FMT, float>(p, transpose, stream);
 }
 
-// codes [rows][row bytes]: box 128 bytes x 128 rows
-int make_tmap_codes(CUtensorMap* tm, const void* ptr, int rows, int cols, int ld) {
+// codes [rows][row bytes]: box 128 bytes x box_rows rows
+int make_tmap_codes(CUtensorMap* tm, const void* ptr, int rows, int cols, int ld, int box_rows) {
     const cuuint64_t dims[3] = {(cuuint64_t)q4_row_bytes(cols), (cuuint64_t)rows, 1};
     const cuuint64_t strides[2] = {(cuuint64_t)ld, (cuuint64_t)rows * (cuuint64_t)ld};
-    const cuuint32_t box[3] = {128, 128, 1};
+    const cuuint32_t box[3] = {128, (cuuint32_t)box_rows, 1};
     const cuuint32_t estr[3] = {1, 1, 1};
     CUresult r = g_encode(tm, CU_TENSOR_MAP_DATA_TYPE_UINT8, 3, const_cast<void*>(ptr), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
                           CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
@@ -1061,34 +1062,35 @@ int make_tmap_scales(CUtensorMap* tm, const void* ptr, int rows, int cols, int f
     return r == CUDA_SUCCESS ? KB_OK : KB_ERR_CUDA;
 }
 
-template <int EPI, int FMT, bool PAIR>
+template <int EPI, int FMT, int BN>
 int launch_gemm4_shape(DeviceState* st, const Gemm4Maps& maps, Gemm4Params p, cudaStream_t stream) {
-    constexpr int TILE = PAIR ? 256 : 128, CTAS = PAIR ? 2 : 1;
-    p.tiles_m = (p.M + TILE - 1) / TILE;
-    p.tiles_n = (p.N + TILE - 1) / TILE;
+    constexpr int TILE_M = BN == 128 ? 128 : 256, CTAS = BN == 128 ? 1 : 2;
+    p.tiles_m = (p.M + TILE_M - 1) / TILE_M;
+    p.tiles_n = (p.N + BN - 1) / BN;
     const long long n_tiles = (long long)p.tiles_m * p.tiles_n;
     if (n_tiles > 0x3fffffffLL) return KB_ERR_SHAPE;
     const int max_groups = st->sm_count / CTAS, groups = n_tiles < max_groups ? (int)n_tiles : max_groups;
     cudaLaunchAttribute cluster;
     cluster.id = cudaLaunchAttributeClusterDimension;
     cluster.val.clusterDim.x = CTAS; cluster.val.clusterDim.y = 1; cluster.val.clusterDim.z = 1;
-    return launch_dependent(gemm4_kernel<EPI, FMT, PAIR>, dim3((unsigned)(groups * CTAS)), dim3(G_THREADS), G4_SMEM, stream, PAIR ? &cluster : nullptr, maps, p);
+    return launch_dependent(gemm4_kernel<EPI, FMT, BN>, dim3((unsigned)(groups * CTAS)), dim3(G_THREADS), G4_SMEM, stream, CTAS == 2 ? &cluster : nullptr, maps, p);
 }
 
 template <int EPI, int FMT>
-int launch_gemm4(DeviceState* st, const Gemm4Maps& maps, const Gemm4Params& p, cudaStream_t stream) {
-    if (gemm4_pair(p.M, p.N, (p.K + G4_K - 1) / G4_K, st->sm_count)) return launch_gemm4_shape<EPI, FMT, true>(st, maps, p, stream);
-    return launch_gemm4_shape<EPI, FMT, false>(st, maps, p, stream);
+int launch_gemm4(DeviceState* st, int width, const Gemm4Maps& maps, const Gemm4Params& p, cudaStream_t stream) {
+    if (width == 256) return launch_gemm4_shape<EPI, FMT, 256>(st, maps, p, stream);
+    if (width == 192) return launch_gemm4_shape<EPI, FMT, 192>(st, maps, p, stream);
+    return launch_gemm4_shape<EPI, FMT, 128>(st, maps, p, stream);
 }
 
 template <int FMT>
-int launch_gemm4_epi(DeviceState* st, int epi, const Gemm4Maps& maps, const Gemm4Params& p, cudaStream_t stream) {
+int launch_gemm4_epi(DeviceState* st, int epi, int width, const Gemm4Maps& maps, const Gemm4Params& p, cudaStream_t stream) {
     switch (epi) {
-        case KB_EPI_F32: return launch_gemm4<EPI_F32, FMT>(st, maps, p, stream);
-        case KB_EPI_F16: return launch_gemm4<EPI_F16, FMT>(st, maps, p, stream);
-        case KB_EPI_GELU16: return launch_gemm4<EPI_GELU16, FMT>(st, maps, p, stream);
-        case KB_EPI_RESID: return launch_gemm4<EPI_RESID, FMT>(st, maps, p, stream);
-        default: return launch_gemm4<EPI_GELU4, FMT>(st, maps, p, stream);
+        case KB_EPI_F32: return launch_gemm4<EPI_F32, FMT>(st, width, maps, p, stream);
+        case KB_EPI_F16: return launch_gemm4<EPI_F16, FMT>(st, width, maps, p, stream);
+        case KB_EPI_GELU16: return launch_gemm4<EPI_GELU16, FMT>(st, width, maps, p, stream);
+        case KB_EPI_RESID: return launch_gemm4<EPI_RESID, FMT>(st, width, maps, p, stream);
+        default: return launch_gemm4<EPI_GELU4, FMT>(st, width, maps, p, stream);
     }
 }
 
@@ -1162,15 +1164,16 @@ int kb_linear4(void* C, int ldc, void* C_scales, const void* A, int lda, const v
     if (M == 0) return KB_OK;
     Gemm4Maps maps;
     memset(&maps, 0, sizeof(maps));
-    if ((rc = make_tmap_codes(&maps.a, A, M, K, lda)) || (rc = make_tmap_codes(&maps.w, W, N, K, ldw)) ||
+    const int width = gemm4_width(M, N, (K + G4_K - 1) / G4_K, st->sm_count);
+    if ((rc = make_tmap_codes(&maps.a, A, M, K, lda, 128)) || (rc = make_tmap_codes(&maps.w, W, N, K, ldw, width == 192 ? 96 : 128)) ||
         (rc = make_tmap_scales(&maps.sa, A_scales, M, K, fmt)) || (rc = make_tmap_scales(&maps.sw, W_scales, N, K, fmt)) ||
-        (!out4 && (rc = make_tmap_out(&maps.c, C, M, N, ldc, out32, false, false))))
+        (!out4 && (rc = make_tmap_out(&maps.c, C, M, N, ldc, out32, false, width == 192))))
         return rc;
     Gemm4Params p = {};
     p.M = M; p.N = N; p.K = K; p.alpha = alpha; p.C = C; p.ldc = ldc; p.gate = gate; p.status = st->status;
     if (out4) { p.codes = static_cast<uint8_t*>(C); p.scales = static_cast<uint8_t*>(C_scales); p.ld_codes = ldc; p.pieces = q4_pieces(N, fmt); }
     ProfScope ps(st, KB_PROF_LINEAR, stream);
-    return fmt == KB_MX4 ? launch_gemm4_epi<FMT_MX4>(st, epi, maps, p, stream) : launch_gemm4_epi<FMT_NV4>(st, epi, maps, p, stream);
+    return fmt == KB_MX4 ? launch_gemm4_epi<FMT_MX4>(st, epi, width, maps, p, stream) : launch_gemm4_epi<FMT_NV4>(st, epi, width, maps, p, stream);
 }
 
 size_t kb_linear4_dx_workspace_bytes(int N, int K) { return N > 0 && K > 0 ? (size_t)N * (size_t)K * 2 : 0; }

@@ -6,10 +6,11 @@
 // tile under the main loop of the next. What differs: a k step in shared memory holds 256 columns (128 bytes) of each operand, plus their scales
 // (2 KB per 128 rows for NV4, 1 KB for MX4), which tcgen05.cp copies to TMEM in front of the step's products, four lanes' quarters at a time.
 //
-// Two shapes. Single: one CTA per 128 x 128 tile. PAIR: two CTAs share a 256 x 256 tile (cta_group::2), each with its 128 rows of A, half of the W rows,
-// the scales of its rows and of ALL 256 columns, and its 128 x 256 half of the accumulator. Two such accumulators fill TMEM and leave no room for
-// scales, so they overlap: the first lies in columns [0, 256), the second in [128, 384), the scales behind them. The epilogue drains the 128 columns that
-// both own first, and then the next tile's products may begin: half of the epilogue still runs under them.
+// Three shapes. Single: one CTA per 128 x 128 tile. Pairs of CTAs on 256 x 192 or 256 x 256 tiles (cta_group::2): each loads its 128 rows of A, half of the W
+// rows, the scales of its rows and of ALL columns of the tile, and keeps its half of the accumulator. Two accumulators of 256 columns fill TMEM and leave no
+// room for scales, so they overlap: the first lies in columns [0, 256), the second in [128, 384), the scales behind them. The epilogue drains the 128
+// columns that both own first, and then the next tile's products begin; until then the tensor pipe waits, about 1.5 us per tile. Tiles of 192 columns
+// have two accumulators beside the scales and no such wait, for a third more loads per product.
 #pragma once
 #include "gemm_sm100.cuh"   // gelu, elect_one, pack16
 #include "quant4.cuh"
@@ -86,43 +87,80 @@ __device__ __forceinline__ void gemm4_tile(int w, const Gemm4Params& p, int& tm,
     tn = in_g / gsz;
 }
 
-// Codes and scales of 32 neighbouring columns of a row (two blocks of NV4, one of MX4): 16 bytes, and the scale bytes from bit 0 on
+// gelu() of gemm_sm100.cuh on a packed pair, the same arithmetic to the bit: (v + |v|) / 2 is max(v, 0) that keeps a NaN, and halving commutes with the
+// last rounding
+__device__ __forceinline__ uint64_t gelu2(uint64_t v) {
+    float v0, v1;
+    unpack2(v, v0, v1);
+    const uint64_t a = pack2(fminf(fabsf(v0), 7.f), fminf(fabsf(v1), 7.f));
+    auto both = [](float c) { return pack2(c, c); };
+    uint64_t q = both(2.5095840960887017e-09f);                           // the polynomial with its sign turned
+    q = fma2(q, a, both(-9.659256505756275e-08f));
+    q = fma2(q, a, both(1.6297367437800858e-06f));
+    q = fma2(q, a, both(-1.5769759556860663e-05f));
+    q = fma2(q, a, both(9.427715122001246e-05f));
+    q = fma2(q, a, both(-3.198326739948243e-04f));
+    q = fma2(q, a, both(5.3875570301897824e-05f));
+    q = fma2(q, a, both(6.906468421220779e-03f));
+    q = fma2(q, a, both(-5.242638662457466e-02f));
+    q = fma2(q, a, both(-0.4592227637767792f));
+    q = fma2(q, a, both(-1.151104211807251f));
+    float t0, t1;
+    unpack2(mul2(q, a), t0, t1);
+    return fma2(mul2(a, both(-0.5f)), pack2(ex2(t0), ex2(t1)), pack2(max0_nan(v0), max0_nan(v1)));
+}
+
+// Codes and scales of 32 neighbouring columns of a row (two blocks of NV4, one of MX4), packed pairs: 16 bytes, and the scale bytes from bit 0 on
 template <int FMT>
-__device__ __forceinline__ void quant32(const float* v, uint4& codes, uint32_t& scale_bytes) {
+__device__ __forceinline__ void quant32(const uint64_t* v, uint4& codes, uint32_t& scale_bytes) {
     uint32_t words[4];
     scale_bytes = 0u;
     constexpr int BLK = q4_block(FMT);
 #pragma unroll
     for (int b = 0; b < 32 / BLK; b++) {
-        uint32_t top = 0u;
+        float top = 0.f;
 #pragma unroll
-        for (int e = 0; e < BLK; e++) top = max(top, __float_as_uint(v[b * BLK + e]) & 0x7fffffffu);
-        const BlockScale<FMT> bs(top, 1.f);
+        for (int e = 0; e < BLK / 2; e++) {
+            float x, y;
+            unpack2(v[b * BLK / 2 + e], x, y);
+            top = max3_abs_nan(top, x, y);
+        }
+        const BlockScale<FMT> bs(__float_as_uint(top) & 0x7fffffffu, 1.f);
         scale_bytes |= bs.byte << (8 * b);
+        const uint64_t r = pack2(bs.r, bs.r), ns = pack2(-bs.s, -bs.s);
 #pragma unroll
         for (int i = 0; i < BLK / 8; i++) {
             float q[8];
 #pragma unroll
-            for (int e = 0; e < 8; e++) q[e] = bs(v[b * BLK + 8 * i + e], 1.f);
+            for (int e = 0; e < 4; e++) {
+                const uint64_t y = v[b * BLK / 2 + 4 * i + e];
+                uint64_t z = mul2(y, r);
+                if (FMT == FMT_NV4) z = fma2(fma2(z, ns, y), r, z);
+                unpack2(z, q[2 * e], q[2 * e + 1]);
+            }
             words[b * (BLK / 8) + i] = e2m1_pack8(q);
         }
     }
     codes = make_uint4(words[0], words[1], words[2], words[3]);
 }
 
-template <int EPI, int FMT, bool PAIR>
+template <int EPI, int FMT, int BN>
 __global__ void __launch_bounds__(G_THREADS, 1)
 gemm4_kernel(const __grid_constant__ Gemm4Maps maps, const Gemm4Params p) {
-    constexpr int BN = PAIR ? 256 : 128, TILE_M = PAIR ? 256 : 128;
-    constexpr int BUF_COLS = 128, ACC_SF = BUF_COLS + BN;                 // TMEM: the second accumulator begins at BUF_COLS, the scales behind it
+    static_assert(BN == 128 || BN == 192 || BN == 256, "tile width");
+    constexpr bool PAIR = BN != 128, OVERLAP = BN == 256;                 // OVERLAP: two accumulators share half of their columns
+    constexpr int TILE_M = PAIR ? 256 : 128, W_ROWS = PAIR ? BN / 2 : BN; // W rows that this CTA loads
+    constexpr int BUF_COLS = OVERLAP ? 128 : BN, ACC_SF = BUF_COLS + BN;  // TMEM: the second accumulator begins at BUF_COLS, the scales behind it
     constexpr int PIECES = FMT == FMT_MX4 ? 2 : 4;                        // scale pieces of a k step per row block
-    constexpr int W_BLOCKS = BN / 128;                                    // row blocks of W whose scales a CTA holds
+    constexpr int W_BLOCKS = PAIR ? 2 : 1;                                // row blocks of W whose scales a CTA holds
     constexpr int SF_COLS = 4 * PIECES * (1 + W_BLOCKS);                  // TMEM columns of a step's scales
     constexpr int SF_BUFS = PAIR && FMT == FMT_NV4 ? 2 : 4;               // steps of them in flight
     static_assert(ACC_SF + SF_BUFS * SF_COLS <= (int)TMEM_ALL_COLUMNS, "TMEM");
-    constexpr uint32_t STAGE_TX = 32768 + PIECES * 512 * (1 + W_BLOCKS);
+    constexpr uint32_t STAGE_TX = (GB_M + W_ROWS) * 128 + PIECES * 512 * (1 + W_BLOCKS);
     constexpr bool OUT32 = EPI == EPI_F32 || EPI == EPI_RESID;
-    constexpr int CW = 64, NCH = BN / CW, BOX_COLS = OUT32 ? 32 : 64, BOXES = CW / BOX_COLS;
+    // Columns per chunk of the epilogue, which a warp has NCH / 2 of; a chunk leaves as one or two boxes of 32 rows x 128 bytes, or 64 where 32 16-bit columns are one
+    constexpr int CW = BN == 192 ? 32 : 64, NCH = BN / CW, BOX_COLS = OUT32 ? 32 : CW, BOXES = CW / BOX_COLS, BOX_ROW = BOX_COLS * (OUT32 ? 4 : 2);
+    constexpr int SLOTS = G4_STAGING_WARP / (32 * BOX_ROW);               // boxes on their way out at a time
 
     extern __shared__ uint8_t smem_raw[];
     const uint32_t raw = smem_u32(smem_raw);
@@ -164,7 +202,7 @@ gemm4_kernel(const __grid_constant__ Gemm4Maps maps, const Gemm4Params p) {
         const uint32_t lane_base = (uint32_t)(quarter * 32) << 16;
         uint8_t* const my_stage = stage_out + warp * G4_STAGING_WARP;
         uint32_t use[2] = {0, 0};
-        int k = 0;
+        int k = 0, box_use = 0;
         for (int w = group; w < n_tiles; w += n_groups, ++k) {
             const int buf = k & 1;
             int tm, tn;
@@ -177,65 +215,76 @@ gemm4_kernel(const __grid_constant__ Gemm4Maps maps, const Gemm4Params p) {
             const int row = m0 + quarter * 32 + lane, nrow = p.M - (m0 + quarter * 32);
 #pragma unroll 1
             for (int i = 0; i < NCH / 2; i++) {
-                const int ch = half + 2 * (PAIR ? i ^ buf ^ 1 : i);       // PAIR: the columns that both accumulators own first
-                float v[CW];
+                // OVERLAP: the columns that both accumulators own first; 192 columns: a warp's three chunks side by side
+                const int ch = OVERLAP ? half + 2 * (i ^ buf ^ 1) : half * (NCH / 2) + i;
+                uint64_t v[CW / 2];
                 {
                     uint32_t a[CW / 32][32];
 #pragma unroll
                     for (int q = 0; q < CW / 32; q++) tmem_ld32(tmem_base + lane_base + (uint32_t)(buf * BUF_COLS + ch * CW + 32 * q), a[q]);
                     tmem_wait_ld();
+                    const uint64_t alpha = pack2(p.alpha, p.alpha);
 #pragma unroll
                     for (int q = 0; q < CW / 32; q++) {
                         reg_fence32(a[q]);
 #pragma unroll
-                        for (int e = 0; e < 32; e++) v[32 * q + e] = __uint_as_float(a[q][e]) * p.alpha;
+                        for (int e = 0; e < 16; e++) v[16 * q + e] = mul2(pack2u(a[q][2 * e], a[q][2 * e + 1]), alpha);
                     }
                 }
-                if (i == 0) {                                             // single: the only chunk; the next tile's products may come
+                if (i == (OVERLAP ? 0 : NCH / 2 - 1)) {                   // what the next products overwrite is in registers
                     tc_fence_before();
                     __syncwarp();
                     if (lane == 0) {
-                        if (PAIR && rank != 0) mbar_arrive_cluster(mapa_u32(bar(G4BAR_ACC_EMPTY), 0));
-                        else mbar_arrive(bar(G4BAR_ACC_EMPTY + (PAIR ? 0 : buf)));
+                        const uint32_t b = bar(G4BAR_ACC_EMPTY + (OVERLAP ? 0 : buf));
+                        if (PAIR && rank != 0) mbar_arrive_cluster(mapa_u32(b, 0));
+                        else mbar_arrive(b);
                     }
                 }
                 const int c0 = n0 + ch * CW;
                 if constexpr (EPI == EPI_GELU16 || EPI == EPI_GELU4) {
 #pragma unroll
-                    for (int c = 0; c < CW; c++) v[c] = gelu(v[c]);
+                    for (int c = 0; c < CW / 2; c++) v[c] = gelu2(v[c]);
                 }
                 if constexpr (EPI == EPI_GELU4) {
                     if (c0 + CW > p.N) {                                  // nothing of W's rows behind the last, whose scales may be anything
 #pragma unroll
-                        for (int c = 0; c < CW; c++) v[c] = c0 + c < p.N ? v[c] : 0.f;
+                        for (int c = 0; c < CW / 2; c++) {
+                            float x, y;
+                            unpack2(v[c], x, y);
+                            v[c] = pack2(c0 + 2 * c < p.N ? x : 0.f, c0 + 2 * c + 1 < p.N ? y : 0.f);
+                        }
                     }
-                    // a thread has whole blocks: 32 bytes of codes and the scales of 64 columns, stored as they are
-                    uint4 codes[2];
-                    uint32_t sb[2];
-                    quant32<FMT>(v, codes[0], sb[0]);
-                    quant32<FMT>(v + 32, codes[1], sb[1]);
-                    if (row < p.M && c0 < p.N) {
-                        uint8_t* const dst = p.codes + (size_t)row * p.ld_codes + (c0 >> 1);
-                        *reinterpret_cast<uint4*>(dst) = codes[0];
-                        if (c0 + 32 < p.N) *reinterpret_cast<uint4*>(dst + 16) = codes[1];
-                        // scales of blocks behind the last column are zeros
-                        constexpr int PER = 32 / q4_block(FMT);
-                        uint32_t word = sb[0] | (c0 + 32 < p.N ? sb[1] << (8 * PER) : 0u);
-                        const int blocks = (p.N - c0 + q4_block(FMT) - 1) / q4_block(FMT);
-                        if (blocks < 2 * PER) word &= (1u << (8 * blocks)) - 1u;
-                        if constexpr (FMT == FMT_NV4) {
-                            *reinterpret_cast<uint32_t*>(p.scales + q4_scale_at(row, c0 >> 6, p.pieces)) = word;
-                        } else {                                          // half a piece; behind the last column the other half as well
-                            uint8_t* const s = p.scales + q4_scale_at(row, c0 >> 7, p.pieces);
-                            if ((c0 & 64) == 0 && c0 + 64 >= p.N) *reinterpret_cast<uint32_t*>(s) = word;
-                            else *reinterpret_cast<uint16_t*>(s + ((c0 >> 5) & 2)) = (uint16_t)word;
+                    // A thread has whole blocks: 16 bytes of codes and the scales of 32 columns at a time, stored as they are. The scales of a piece's blocks
+                    // behind the last column are zeros: whoever has the last column writes them.
+                    constexpr int PER = 32 / q4_block(FMT), PIECE = 4 * q4_block(FMT);
+#pragma unroll
+                    for (int q = 0; q < CW / 32; q++) {
+                        const int c = c0 + 32 * q;
+                        uint4 codes;
+                        uint32_t sb;
+                        quant32<FMT>(v + 16 * q, codes, sb);
+                        if (row >= p.M || c >= p.N) continue;
+                        *reinterpret_cast<uint4*>(p.codes + (size_t)row * p.ld_codes + (c >> 1)) = codes;
+                        uint8_t* const s = p.scales + q4_scale_at(row, c / PIECE, p.pieces);
+                        const int b = c % PIECE / q4_block(FMT);          // its first block in the piece
+                        if (c + 32 >= p.N) {
+                            const int blocks = (p.N - c + q4_block(FMT) - 1) / q4_block(FMT);
+                            if (blocks < PER) sb &= 0xffu;
+#pragma unroll
+                            for (int e = 0; e < 4; e++)
+                                if (b + e < 4) s[b + e] = (uint8_t)(sb >> (8 * e));
+                        } else if (PER == 2) {
+                            *reinterpret_cast<uint16_t*>(s + b) = (uint16_t)sb;
+                        } else {
+                            s[b] = (uint8_t)sb;
                         }
                     }
                 } else {
                     if constexpr (EPI == EPI_RESID) {
                         if (p.gate) {
 #pragma unroll
-                            for (int c = 0; c < CW; c++) v[c] *= c0 + c < p.N ? p.gate[c0 + c] : 0.f;
+                            for (int c = 0; c < CW / 2; c++)
+                                v[c] = mul2(v[c], pack2(c0 + 2 * c < p.N ? p.gate[c0 + 2 * c] : 0.f, c0 + 2 * c + 1 < p.N ? p.gate[c0 + 2 * c + 1] : 0.f));
                         }
                     }
                     // 32 rows of the chunk as swizzled boxes in shared memory, which leave by TMA
@@ -248,34 +297,42 @@ gemm4_kernel(const __grid_constant__ Gemm4Maps maps, const Gemm4Params p) {
 #pragma unroll
                                 for (int c = 0; c < BOX_COLS; c++) {
                                     if (x + c >= p.N) continue;
+                                    float lo, hi;
+                                    unpack2(v[(b * BOX_COLS + c) / 2], lo, hi);
+                                    const float u = c & 1 ? hi : lo;
                                     const size_t at = (size_t)row * p.ldc + x + c;
-                                    if constexpr (EPI == EPI_RESID) static_cast<float*>(p.C)[at] += v[b * 32 + c];
-                                    else if constexpr (OUT32) static_cast<float*>(p.C)[at] = v[b * 32 + c];
-                                    else static_cast<__half*>(p.C)[at] = __float2half_rn(v[c]);
+                                    if constexpr (EPI == EPI_RESID) static_cast<float*>(p.C)[at] += u;
+                                    else if constexpr (OUT32) static_cast<float*>(p.C)[at] = u;
+                                    else static_cast<__half*>(p.C)[at] = __float2half_rn(u);
                                 }
                             }
                             continue;
                         }
-                        if (lane == 0) tma_store_wait_read();             // the box that was here has been read
+                        uint8_t* const box = my_stage + (SLOTS == 2 ? (box_use & 1) * 32 * BOX_ROW : 0);
+                        ++box_use;
+                        if (lane == 0) { if (SLOTS == 2) tma_store_wait_read_1(); else tma_store_wait_read(); }   // the box that was here has been read
                         __syncwarp();
 #pragma unroll
-                        for (int c = 0; c < 8; c++) {
+                        for (int c = 0; c < BOX_ROW / 16; c++) {
                             uint4 pk;
                             if constexpr (OUT32) {
-                                const float* const u = v + b * 32 + 4 * c;
-                                pk = make_uint4(__float_as_uint(u[0]), __float_as_uint(u[1]), __float_as_uint(u[2]), __float_as_uint(u[3]));
+                                const uint64_t* const u = v + b * 16 + 2 * c;
+                                pk = make_uint4((uint32_t)u[0], (uint32_t)(u[0] >> 32), (uint32_t)u[1], (uint32_t)(u[1] >> 32));
                             } else {
-                                const float* const u = v + 8 * c;
-                                pk.x = pack16<DT_F16>(u[0], u[1]); pk.y = pack16<DT_F16>(u[2], u[3]);
-                                pk.z = pack16<DT_F16>(u[4], u[5]); pk.w = pack16<DT_F16>(u[6], u[7]);
+                                const uint64_t* const u = v + 4 * c;
+                                auto two = [](uint64_t w) { float lo, hi; unpack2(w, lo, hi); return pack16<DT_F16>(lo, hi); };
+                                pk = make_uint4(two(u[0]), two(u[1]), two(u[2]), two(u[3]));
                             }
-                            *reinterpret_cast<uint4*>(my_stage + lane * 128 + ((c ^ (lane & 7)) << 4)) = pk;
+                            const int piece = BOX_ROW == 128 ? c ^ (lane & 7) : c ^ ((lane >> 1) & 3);
+                            *reinterpret_cast<uint4*>(box + lane * BOX_ROW + (piece << 4)) = pk;
                         }
                         fence_proxy_async_smem();
                         __syncwarp();
-                        if (lane == 0 && nrow > 0 && x < p.N) {
-                            if constexpr (EPI == EPI_RESID) tma_reduce_add_3d(&maps.c, smem_u32(my_stage), x, y, 0);
-                            else tma_store_3d(&maps.c, smem_u32(my_stage), x, y, 0);
+                        if (lane == 0) {                                  // an empty group where nothing is stored, so that groups count boxes
+                            if (nrow > 0 && x < p.N) {
+                                if constexpr (EPI == EPI_RESID) tma_reduce_add_3d(&maps.c, smem_u32(box), x, y, 0);
+                                else tma_store_3d(&maps.c, smem_u32(box), x, y, 0);
+                            }
                             tma_store_commit();
                         }
                     }
@@ -291,7 +348,7 @@ gemm4_kernel(const __grid_constant__ Gemm4Maps maps, const Gemm4Params p) {
             int k = 0;
             for (int w = group; w < n_tiles && good; w += n_groups, ++k) {
                 const int buf = k & 1;
-                if (PAIR) {
+                if (OVERLAP) {
                     // the tile before this one is out of the shared columns, so the one before that is out of all of its own
                     if (k > 0) good = mbar_wait(bar(G4BAR_ACC_EMPTY), (uint32_t)(k - 1) & 1u, abort_flag);
                 } else {
@@ -300,6 +357,10 @@ gemm4_kernel(const __grid_constant__ Gemm4Maps maps, const Gemm4Params p) {
                 ++use[buf];
                 if (!good) break;
                 tc_fence_after();
+                // 192 columns: every other tile begins in the middle of a row block of scales, two TMEM columns further
+                int tm, tn;
+                gemm4_tile(w, p, tm, tn);
+                const uint32_t sfb_skip = BN == 192 ? (uint32_t)(tn & 1) * 2u : 0u;
                 for (int ks = 0; ks < ksteps && good; ++ks, ++ring) {
                     const uint32_t st = ring % G4_STAGES;
                     good = mbar_wait(bar(G4BAR_FULL + st), (ring / G4_STAGES) & 1u, abort_flag);
@@ -321,7 +382,7 @@ gemm4_kernel(const __grid_constant__ Gemm4Maps maps, const Gemm4Params p) {
                     for (int kk = 0; kk < 4; kk++) {
                         const int q = kk * PIECES / 4, byte = FMT == FMT_MX4 ? (kk & 1) * 2 : 0;
                         mma_f4<FMT, PAIR>(tmem_base + (uint32_t)(buf * BUF_COLS), adesc + (uint64_t)(kk * 2), wdesc + (uint64_t)(kk * 2),
-                                          idesc_f4(FMT == FMT_MX4, TILE_M, BN, byte), sfa + 4 * q, sfb + 4 * q * W_BLOCKS, (ks > 0 || kk > 0) ? 1u : 0u);
+                                          idesc_f4(FMT == FMT_MX4, TILE_M, BN, byte), sfa + 4 * q, sfb + sfb_skip + 4 * q * W_BLOCKS, (ks > 0 || kk > 0) ? 1u : 0u);
                     }
                     if (PAIR) tc_commit_pair(bar(G4BAR_EMPTY + st), (uint16_t)3); else tc_commit(bar(G4BAR_EMPTY + st));
                 }
@@ -347,10 +408,10 @@ gemm4_kernel(const __grid_constant__ Gemm4Maps maps, const Gemm4Params p) {
                         if (rank == 0) mbar_expect_tx(bar(G4BAR_FULL + st), 2 * STAGE_TX);
                         const uint32_t fb = mapa_u32(bar(G4BAR_FULL + st), 0);
                         tma_load_3d_pair(a_s, &maps.a, fb, ks * 128, tm * TILE_M + (int)rank * 128, 0);
-                        tma_load_3d_pair(a_s + 16384, &maps.w, fb, ks * 128, tn * BN + (int)rank * 128, 0);
+                        tma_load_3d_pair(a_s + 16384, &maps.w, fb, ks * 128, tn * BN + (int)rank * W_ROWS, 0);
                         tma_load_3d_pair(s_s, &maps.sa, fb, 0, ks * PIECES, tm * 2 + (int)rank);
 #pragma unroll
-                        for (int b = 0; b < W_BLOCKS; b++) tma_load_3d_pair(s_s + PIECES * 512 * (1 + b), &maps.sw, fb, 0, ks * PIECES, tn * W_BLOCKS + b);
+                        for (int b = 0; b < W_BLOCKS; b++) tma_load_3d_pair(s_s + PIECES * 512 * (1 + b), &maps.sw, fb, 0, ks * PIECES, tn * BN / 128 + b);
                     } else {
                         const uint32_t fb = bar(G4BAR_FULL + st);
                         mbar_expect_tx(fb, STAGE_TX);

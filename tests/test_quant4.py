@@ -194,7 +194,7 @@ def _pair(ops, seed, M, N, K, fmt, dtype="f16"):
 
 
 SHAPES = [(1, 1, 1), (1, 8, 32), (1, 2048, 512), (2, 300, 1000), (7, 130, 96), (8, 96, 2048), (9, 520, 64), (77, 256, 1024), (128, 128, 256), (129, 129, 257), (300, 257, 300),
-          (257, 512, 4096), (1000, 64, 160)]
+          (257, 512, 4096), (1000, 64, 160), (513, 577, 1100)]
 
 
 @gpu
@@ -299,6 +299,12 @@ def test_product_shows_bad_blocks(built_lib, fmt, M):
     want[M // 2] = True
     want[:, 11] = True
     assert np.array_equal(np.isnan(out), want)
+    A, W = ops.quant4(x.cuda(), fmt), ops.quant4(w.cuda(), fmt)
+    assert np.array_equal(np.isnan(ops.linear4(ops.padded_empty(M, 40, torch.float16, "cuda"), A, W, ops.EPI_GELU16).float().cpu().numpy()), want)
+    H = held(ops.linear4(ops.quant4_empty(M, 40, fmt, "cuda"), A, W, ops.EPI_GELU4))
+    blocks = np.arange(40) // BLOCK[fmt]
+    want[:, blocks == blocks[11]] = True                                   # in 4 bits the whole block of a NaN
+    assert np.array_equal(np.isnan(H), want)
 
 
 @gpu

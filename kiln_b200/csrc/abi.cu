@@ -92,11 +92,10 @@ int set_gemm_smem() {
 template <int EPI>
 int set_gemm4_smem() {
     int rc;
-    if ((rc = set_smem(gemm4_kernel<EPI, FMT_MX4, 128>, G4_SMEM)) || (rc = set_smem(gemm4_kernel<EPI, FMT_NV4, 128>, G4_SMEM)) ||
-        (rc = set_smem(gemm4_kernel<EPI, FMT_MX4, 192>, G4_SMEM)) || (rc = set_smem(gemm4_kernel<EPI, FMT_NV4, 192>, G4_SMEM)) ||
-        (rc = set_smem(gemm4_kernel<EPI, FMT_MX4, 256>, G4_SMEM)))
+    if ((rc = set_smem(gemm4_kernel<EPI, FMT_MX4, false>, G4_SMEM)) || (rc = set_smem(gemm4_kernel<EPI, FMT_NV4, false>, G4_SMEM)) ||
+        (rc = set_smem(gemm4_kernel<EPI, FMT_MX4, true>, G4_SMEM)))
         return rc;
-    return set_smem(gemm4_kernel<EPI, FMT_NV4, 256>, G4_SMEM);
+    return set_smem(gemm4_kernel<EPI, FMT_NV4, true>, G4_SMEM);
 }
 
 int init_device(DeviceState& st, int dev) {
@@ -1002,35 +1001,29 @@ inline size_t elem_size(int dtype) { return dtype == KB_F32 ? 4 : 2; }
 // whether every row starts on 16 bytes, so that a thread may take eight elements at once
 inline bool wide_rows(const void* p, int ld, int dtype) { return aligned16(p) && (ld * elem_size(dtype)) % 16 == 0; }
 
-int quant4_grid(Quant4Params& p, dim3* grid) {
-    p.segs = (p.cols + Q4_SEGS * 256 - 1) / (Q4_SEGS * 256);
-    const long long blocks = ((long long)p.rows * p.segs + Q4_THREADS / 32 - 1) / (Q4_THREADS / 32);
-    if (blocks > 0x7fffffffLL) return KB_ERR_SHAPE;
-    *grid = dim3((unsigned)blocks);
-    return KB_OK;
+// a warp per row and group of columns
+template <typename T>
+dim3 quant4_grid(const Quant4Params& p) {
+    constexpr int COLS = q4_segs<T>() * 256, WARPS = Q4_THREADS / 32;
+    static_assert(KB_MAX_Q4_COLS / COLS <= 65535, "grid");
+    return dim3((unsigned)(((long long)p.rows + WARPS - 1) / WARPS), (unsigned)((p.cols + COLS - 1) / COLS));
 }
 
 template <int FMT>
 int launch_quant4(Quant4Params& p, int dtype, cudaStream_t stream) {
-    dim3 grid;
-    int rc;
-    if ((rc = quant4_grid(p, &grid))) return rc;
-    if (dtype == KB_F16) return launch_dependent(quant4_kernel<__half, FMT>, grid, dim3(Q4_THREADS), 0, stream, nullptr, p);
-    if (dtype == KB_BF16) return launch_dependent(quant4_kernel<__nv_bfloat16, FMT>, grid, dim3(Q4_THREADS), 0, stream, nullptr, p);
-    return launch_dependent(quant4_kernel<float, FMT>, grid, dim3(Q4_THREADS), 0, stream, nullptr, p);
+    if (dtype == KB_F16) return launch_dependent(quant4_kernel<__half, FMT>, quant4_grid<__half>(p), dim3(Q4_THREADS), 0, stream, nullptr, p);
+    if (dtype == KB_BF16) return launch_dependent(quant4_kernel<__nv_bfloat16, FMT>, quant4_grid<__nv_bfloat16>(p), dim3(Q4_THREADS), 0, stream, nullptr, p);
+    return launch_dependent(quant4_kernel<float, FMT>, quant4_grid<float>(p), dim3(Q4_THREADS), 0, stream, nullptr, p);
 }
 
 template <int FMT, typename T>
 int launch_dequant4_t(Quant4Params& p, bool transpose, cudaStream_t stream) {
-    dim3 grid;
-    int rc;
     if (transpose) {
         const long long blocks = (((long long)p.rows + Q4_TILE - 1) / Q4_TILE) * ((p.cols + Q4_TILE - 1) / Q4_TILE);
         if (blocks > 0x7fffffffLL) return KB_ERR_SHAPE;
         return launch_dependent(dequant4_t_kernel<T, FMT>, dim3((unsigned)blocks), dim3(256), 0, stream, nullptr, p);
     }
-    if ((rc = quant4_grid(p, &grid))) return rc;
-    return launch_dependent(dequant4_kernel<T, FMT>, grid, dim3(Q4_THREADS), 0, stream, nullptr, p);
+    return launch_dependent(dequant4_kernel<T, FMT>, quant4_grid<T>(p), dim3(Q4_THREADS), 0, stream, nullptr, p);
 }
 
 template <int FMT>
@@ -1040,11 +1033,11 @@ int launch_dequant4(Quant4Params& p, int dtype, bool transpose, cudaStream_t str
     return launch_dequant4_t<FMT, float>(p, transpose, stream);
 }
 
-// codes [rows][row bytes]: box 128 bytes x box_rows rows
-int make_tmap_codes(CUtensorMap* tm, const void* ptr, int rows, int cols, int ld, int box_rows) {
+// codes [rows][row bytes]: box 128 bytes x 128 rows
+int make_tmap_codes(CUtensorMap* tm, const void* ptr, int rows, int cols, int ld) {
     const cuuint64_t dims[3] = {(cuuint64_t)q4_row_bytes(cols), (cuuint64_t)rows, 1};
     const cuuint64_t strides[2] = {(cuuint64_t)ld, (cuuint64_t)rows * (cuuint64_t)ld};
-    const cuuint32_t box[3] = {128, (cuuint32_t)box_rows, 1};
+    const cuuint32_t box[3] = {128, 128, 1};
     const cuuint32_t estr[3] = {1, 1, 1};
     CUresult r = g_encode(tm, CU_TENSOR_MAP_DATA_TYPE_UINT8, 3, const_cast<void*>(ptr), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
                           CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
@@ -1062,35 +1055,34 @@ int make_tmap_scales(CUtensorMap* tm, const void* ptr, int rows, int cols, int f
     return r == CUDA_SUCCESS ? KB_OK : KB_ERR_CUDA;
 }
 
-template <int EPI, int FMT, int BN>
+template <int EPI, int FMT, bool PAIR>
 int launch_gemm4_shape(DeviceState* st, const Gemm4Maps& maps, Gemm4Params p, cudaStream_t stream) {
-    constexpr int TILE_M = BN == 128 ? 128 : 256, CTAS = BN == 128 ? 1 : 2;
-    p.tiles_m = (p.M + TILE_M - 1) / TILE_M;
-    p.tiles_n = (p.N + BN - 1) / BN;
+    constexpr int TILE = PAIR ? 256 : 128, CTAS = PAIR ? 2 : 1;
+    p.tiles_m = (p.M + TILE - 1) / TILE;
+    p.tiles_n = (p.N + TILE - 1) / TILE;
     const long long n_tiles = (long long)p.tiles_m * p.tiles_n;
     if (n_tiles > 0x3fffffffLL) return KB_ERR_SHAPE;
     const int max_groups = st->sm_count / CTAS, groups = n_tiles < max_groups ? (int)n_tiles : max_groups;
     cudaLaunchAttribute cluster;
     cluster.id = cudaLaunchAttributeClusterDimension;
     cluster.val.clusterDim.x = CTAS; cluster.val.clusterDim.y = 1; cluster.val.clusterDim.z = 1;
-    return launch_dependent(gemm4_kernel<EPI, FMT, BN>, dim3((unsigned)(groups * CTAS)), dim3(G_THREADS), G4_SMEM, stream, CTAS == 2 ? &cluster : nullptr, maps, p);
+    return launch_dependent(gemm4_kernel<EPI, FMT, PAIR>, dim3((unsigned)(groups * CTAS)), dim3(G_THREADS), G4_SMEM, stream, PAIR ? &cluster : nullptr, maps, p);
 }
 
 template <int EPI, int FMT>
-int launch_gemm4(DeviceState* st, int width, const Gemm4Maps& maps, const Gemm4Params& p, cudaStream_t stream) {
-    if (width == 256) return launch_gemm4_shape<EPI, FMT, 256>(st, maps, p, stream);
-    if (width == 192) return launch_gemm4_shape<EPI, FMT, 192>(st, maps, p, stream);
-    return launch_gemm4_shape<EPI, FMT, 128>(st, maps, p, stream);
+int launch_gemm4(DeviceState* st, const Gemm4Maps& maps, const Gemm4Params& p, cudaStream_t stream) {
+    if (gemm4_pair(p.M, p.N, (p.K + G4_K - 1) / G4_K, EPI, st->sm_count)) return launch_gemm4_shape<EPI, FMT, true>(st, maps, p, stream);
+    return launch_gemm4_shape<EPI, FMT, false>(st, maps, p, stream);
 }
 
 template <int FMT>
-int launch_gemm4_epi(DeviceState* st, int epi, int width, const Gemm4Maps& maps, const Gemm4Params& p, cudaStream_t stream) {
+int launch_gemm4_epi(DeviceState* st, int epi, const Gemm4Maps& maps, const Gemm4Params& p, cudaStream_t stream) {
     switch (epi) {
-        case KB_EPI_F32: return launch_gemm4<EPI_F32, FMT>(st, width, maps, p, stream);
-        case KB_EPI_F16: return launch_gemm4<EPI_F16, FMT>(st, width, maps, p, stream);
-        case KB_EPI_GELU16: return launch_gemm4<EPI_GELU16, FMT>(st, width, maps, p, stream);
-        case KB_EPI_RESID: return launch_gemm4<EPI_RESID, FMT>(st, width, maps, p, stream);
-        default: return launch_gemm4<EPI_GELU4, FMT>(st, width, maps, p, stream);
+        case KB_EPI_F32: return launch_gemm4<EPI_F32, FMT>(st, maps, p, stream);
+        case KB_EPI_F16: return launch_gemm4<EPI_F16, FMT>(st, maps, p, stream);
+        case KB_EPI_GELU16: return launch_gemm4<EPI_GELU16, FMT>(st, maps, p, stream);
+        case KB_EPI_RESID: return launch_gemm4<EPI_RESID, FMT>(st, maps, p, stream);
+        default: return launch_gemm4<EPI_GELU4, FMT>(st, maps, p, stream);
     }
 }
 
@@ -1164,16 +1156,15 @@ int kb_linear4(void* C, int ldc, void* C_scales, const void* A, int lda, const v
     if (M == 0) return KB_OK;
     Gemm4Maps maps;
     memset(&maps, 0, sizeof(maps));
-    const int width = gemm4_width(M, N, (K + G4_K - 1) / G4_K, st->sm_count);
-    if ((rc = make_tmap_codes(&maps.a, A, M, K, lda, 128)) || (rc = make_tmap_codes(&maps.w, W, N, K, ldw, width == 192 ? 96 : 128)) ||
+    if ((rc = make_tmap_codes(&maps.a, A, M, K, lda)) || (rc = make_tmap_codes(&maps.w, W, N, K, ldw)) ||
         (rc = make_tmap_scales(&maps.sa, A_scales, M, K, fmt)) || (rc = make_tmap_scales(&maps.sw, W_scales, N, K, fmt)) ||
-        (!out4 && (rc = make_tmap_out(&maps.c, C, M, N, ldc, out32, false, width == 192))))
+        (!out4 && (rc = make_tmap_out(&maps.c, C, M, N, ldc, out32, false, false))))
         return rc;
     Gemm4Params p = {};
     p.M = M; p.N = N; p.K = K; p.alpha = alpha; p.C = C; p.ldc = ldc; p.gate = gate; p.status = st->status;
     if (out4) { p.codes = static_cast<uint8_t*>(C); p.scales = static_cast<uint8_t*>(C_scales); p.ld_codes = ldc; p.pieces = q4_pieces(N, fmt); }
     ProfScope ps(st, KB_PROF_LINEAR, stream);
-    return fmt == KB_MX4 ? launch_gemm4_epi<FMT_MX4>(st, epi, width, maps, p, stream) : launch_gemm4_epi<FMT_NV4>(st, epi, width, maps, p, stream);
+    return fmt == KB_MX4 ? launch_gemm4_epi<FMT_MX4>(st, epi, maps, p, stream) : launch_gemm4_epi<FMT_NV4>(st, epi, maps, p, stream);
 }
 
 size_t kb_linear4_dx_workspace_bytes(int N, int K) { return N > 0 && K > 0 ? (size_t)N * (size_t)K * 2 : 0; }
@@ -1236,10 +1227,11 @@ int launch_rope_t(const RopeParams& p, bool half, bool vec, unsigned blocks, cud
 }
 
 template <typename InT>
-int launch_dropout_t(const DropoutParams& p, int out_dtype, unsigned blocks, cudaStream_t stream) {
-    if (out_dtype == KB_F16) return launch_dependent(dropout_kernel<InT, __half>, dim3(blocks), dim3(DROP_THREADS), 0, stream, nullptr, p);
-    if (out_dtype == KB_BF16) return launch_dependent(dropout_kernel<InT, __nv_bfloat16>, dim3(blocks), dim3(DROP_THREADS), 0, stream, nullptr, p);
-    return launch_dependent(dropout_kernel<InT, float>, dim3(blocks), dim3(DROP_THREADS), 0, stream, nullptr, p);
+int launch_dropout_t(const DropoutParams& p, int out_dtype, dim3 grid, cudaStream_t stream) {
+    const dim3 block(DROP_THREADS);
+    if (out_dtype == KB_F16) return launch_dependent(dropout_kernel<InT, __half>, grid, block, 0, stream, nullptr, p);
+    if (out_dtype == KB_BF16) return launch_dependent(dropout_kernel<InT, __nv_bfloat16>, grid, block, 0, stream, nullptr, p);
+    return launch_dependent(dropout_kernel<InT, float>, grid, block, 0, stream, nullptr, p);
 }
 
 }  // namespace
@@ -1256,13 +1248,14 @@ int kb_rope(int n, void* const* out, const int* ld_out, const void* const* in, c
     if (head_dim > 2 * ROPE_MAX_PAIRS || rot_dim > head_dim || n_axes > 255 || ld_pos < n_axes) return KB_ERR_SHAPE;
     if (reinterpret_cast<uintptr_t>(pos) % 4) return KB_ERR_ALIGN;
     RopeParams p = {};
-    p.wide = head_dim % 8 == 0;
+    bool wide = head_dim % 8 == 0;
     for (int i = 0; i < n; i++) {
         if (!out[i] || !in[i] || heads[i] <= 0) return KB_ERR_ARG;
         if (heads[i] > MAX_HEADS || ld_in[i] < heads[i] * head_dim || ld_out[i] < heads[i] * head_dim) return KB_ERR_SHAPE;
         if (reinterpret_cast<uintptr_t>(out[i]) % elem_size(dtype) || reinterpret_cast<uintptr_t>(in[i]) % elem_size(dtype)) return KB_ERR_ALIGN;
-        p.t[i].x = in[i]; p.t[i].y = out[i]; p.t[i].heads = heads[i]; p.t[i].ld_x = ld_in[i]; p.t[i].ld_y = ld_out[i];
-        p.wide = p.wide && wide_rows(in[i], ld_in[i], dtype) && wide_rows(out[i], ld_out[i], dtype);
+        p.t[i].x = in[i]; p.t[i].y = out[i]; p.t[i].first = p.heads; p.t[i].ld_x = ld_in[i]; p.t[i].ld_y = ld_out[i];
+        p.heads += heads[i];
+        wide = wide && wide_rows(in[i], ld_in[i], dtype) && wide_rows(out[i], ld_out[i], dtype);
     }
     for (int i = 0; i < rot_dim / 2; i++) {
         const int ax = axis ? axis[i] : 0;
@@ -1277,10 +1270,9 @@ int kb_rope(int n, void* const* out, const int* ld_out, const void* const* in, c
     if (rows == 0) return KB_OK;
     p.pos = pos; p.n = n; p.rows = rows; p.pos_rows = pos_rows; p.ld_pos = ld_pos; p.dim = head_dim; p.rot = rot_dim; p.inverse = inverse != 0;
     p.amplitude = amplitude;
-    const int pairs = rot_dim / 2;
-    p.block_rows = ROPE_SLOTS / pairs < 4 ? ROPE_SLOTS / pairs : 4;
+    const bool half = layout == KB_ROPE_HALF, vec = wide && (!half || rot_dim % 16 == 0);
+    p.block_rows = rope_block_rows(half, vec, head_dim, rot_dim, p.heads);
     const unsigned blocks = (unsigned)(((long long)rows + p.block_rows - 1) / p.block_rows);
-    const bool half = layout == KB_ROPE_HALF, vec = p.wide && (!half || pairs % 8 == 0);
     ProfScope ps(st, KB_PROF_NORM_ROPE, stream);
     if (dtype == KB_F16) return launch_rope_t<__half>(p, half, vec, blocks, stream);
     if (dtype == KB_BF16) return launch_rope_t<__nv_bfloat16>(p, half, vec, blocks, stream);
@@ -1304,16 +1296,20 @@ int kb_dropout(void* out, int ld_out, int out_dtype, const void* in, int ld_in, 
     if (rows == 0) return KB_OK;
     DropoutParams p = {};
     p.x = in; p.resid = resid; p.y = out; p.rng = rng;
-    p.cols = cols; p.groups = (cols + 7) / 8; p.units = (long long)rows * p.groups;
+    p.rows = rows; p.cols = cols;
     p.ld_x = ld_in; p.ld_r = ld_resid; p.ld_y = ld_out;
     p.t = t; p.scale = (float)(65536.0 / (65536.0 - t));
     p.wide = wide_rows(in, ld_in, in_dtype) && wide_rows(out, ld_out, out_dtype) && (!resid || wide_rows(resid, ld_resid, out_dtype));
-    const long long blocks = (p.units + DROP_THREADS - 1) / DROP_THREADS;
-    if (blocks > 0x7fffffffLL) return KB_ERR_SHAPE;
+    // a row of a block's threads as wide as a row of the matrix, up to all of them
+    const long long groups = ((long long)cols + 8 * DROP_GROUPS - 1) / (8 * DROP_GROUPS);
+    while (p.width_log2 < DROP_THREADS_LOG2 && 1LL << p.width_log2 < groups) ++p.width_log2;
+    const long long across = (groups + (1LL << p.width_log2) - 1) >> p.width_log2, block_rows = DROP_THREADS >> p.width_log2;
+    if (across > 65535) return KB_ERR_SHAPE;
+    const dim3 grid((unsigned)(((long long)rows + block_rows - 1) / block_rows), (unsigned)across);
     ProfScope ps(st, KB_PROF_LINEAR, stream);
-    if (in_dtype == KB_F16) return launch_dropout_t<__half>(p, out_dtype, (unsigned)blocks, stream);
-    if (in_dtype == KB_BF16) return launch_dropout_t<__nv_bfloat16>(p, out_dtype, (unsigned)blocks, stream);
-    return launch_dropout_t<float>(p, out_dtype, (unsigned)blocks, stream);
+    if (in_dtype == KB_F16) return launch_dropout_t<__half>(p, out_dtype, grid, stream);
+    if (in_dtype == KB_BF16) return launch_dropout_t<__nv_bfloat16>(p, out_dtype, grid, stream);
+    return launch_dropout_t<float>(p, out_dtype, grid, stream);
 }
 
 int kb_lora_pack(void* dst_f16, int ld, int col0, const void* src_bf16, int rows, int cols, float scale, void* stream) {

@@ -25,38 +25,52 @@ struct DropoutParams {
     const void* resid;                    // of the output's type, or null
     void* y;
     const unsigned long long* rng;        // seed, offset
-    long long units;                      // groups of eight columns, over all rows
-    int cols, groups, ld_x, ld_r, ld_y;   // groups: of a row
+    int rows, cols, ld_x, ld_r, ld_y;
+    int width_log2;                       // threads of a block side by side on a row
     unsigned t;                           // a 16-bit number below t drops its element
     float scale;
     bool wide;                            // every row of every matrix starts on 16 bytes
 };
 
-constexpr int DROP_THREADS = 256;
+// A thread takes DROP_GROUPS groups of eight columns, its loads first.
+constexpr int DROP_THREADS_LOG2 = 8, DROP_THREADS = 1 << DROP_THREADS_LOG2, DROP_GROUPS = 2;
 
 template <typename InT, typename OutT>
 __global__ void __launch_bounds__(DROP_THREADS)
 dropout_kernel(const DropoutParams p) {
     pdl_launch();
     pdl_wait();
-    const long long unit = (long long)blockIdx.x * DROP_THREADS + threadIdx.x;
-    if (unit >= p.units) return;
-    const int row = (int)(unit / p.groups), g = (int)(unit % p.groups), c = g * 8;
+    const int width = 1 << p.width_log2;
+    const unsigned row = blockIdx.x * (unsigned)(DROP_THREADS >> p.width_log2) + (threadIdx.x >> p.width_log2);
+    const int g0 = (int)blockIdx.y * (DROP_GROUPS * width) + (int)(threadIdx.x & (unsigned)(width - 1));
+    if (row >= (unsigned)p.rows) return;
+    const InT* const x = static_cast<const InT*>(p.x) + (size_t)row * p.ld_x;
+    OutT* const y = static_cast<OutT*>(p.y) + (size_t)row * p.ld_y;
     const unsigned long long seed = p.rng[0], offset = p.rng[1];
-    const F8 x = load8(static_cast<const InT*>(p.x) + (size_t)row * p.ld_x, c, p.cols, p.wide);
-    F8 y;
-    if (p.resid) y = load8(static_cast<const OutT*>(p.resid) + (size_t)row * p.ld_r, c, p.cols, p.wide);
-    else
+    F8 in[DROP_GROUPS], out[DROP_GROUPS];
 #pragma unroll
-        for (int i = 0; i < 8; i++) y.v[i] = 0.f;
-    const uint4 w = philox4x32(make_uint4((uint32_t)g, (uint32_t)row, (uint32_t)offset, (uint32_t)(offset >> 32)), (uint32_t)seed, (uint32_t)(seed >> 32));
-    const uint32_t words[4] = {w.x, w.y, w.z, w.w};
+    for (int i = 0; i < DROP_GROUPS; i++) {
+        const int c = (g0 + i * width) * 8;
+        if (c >= p.cols) break;
+        in[i] = load8(x, c, p.cols, p.wide);
+        if (p.resid) out[i] = load8(static_cast<const OutT*>(p.resid) + (size_t)row * p.ld_r, c, p.cols, p.wide);
+        else
 #pragma unroll
-    for (int i = 0; i < 8; i++) {
-        const uint32_t r = (i & 1) ? words[i >> 1] >> 16 : words[i >> 1] & 0xffffu;
-        if (r >= p.t) y.v[i] = __fadd_rn(y.v[i], __fmul_rn(x.v[i], p.scale));   // product and sum rounded apart, with a residual and without
+            for (int e = 0; e < 8; e++) out[i].v[e] = 0.f;
     }
-    store8(static_cast<OutT*>(p.y) + (size_t)row * p.ld_y, c, p.cols, p.wide, y);
+#pragma unroll
+    for (int i = 0; i < DROP_GROUPS; i++) {
+        const int g = g0 + i * width, c = g * 8;
+        if (c >= p.cols) break;
+        const uint4 w = philox4x32(make_uint4((uint32_t)g, row, (uint32_t)offset, (uint32_t)(offset >> 32)), (uint32_t)seed, (uint32_t)(seed >> 32));
+        const uint32_t words[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+        for (int e = 0; e < 8; e++) {
+            const uint32_t r = (e & 1) ? words[e >> 1] >> 16 : words[e >> 1] & 0xffffu;
+            if (r >= p.t) out[i].v[e] = __fadd_rn(out[i].v[e], __fmul_rn(in[i].v[e], p.scale));   // product and sum rounded apart, with a residual and without
+        }
+        store8(y, c, p.cols, p.wide, out[i]);
+    }
 }
 
 }  // namespace kb

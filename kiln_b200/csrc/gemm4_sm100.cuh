@@ -6,11 +6,14 @@
 // tile under the main loop of the next. What differs: a k step in shared memory holds 256 columns (128 bytes) of each operand, plus their scales
 // (2 KB per 128 rows for NV4, 1 KB for MX4), which tcgen05.cp copies to TMEM in front of the step's products, four lanes' quarters at a time.
 //
-// Three shapes. Single: one CTA per 128 x 128 tile. Pairs of CTAs on 256 x 192 or 256 x 256 tiles (cta_group::2): each loads its 128 rows of A, half of the W
-// rows, the scales of its rows and of ALL columns of the tile, and keeps its half of the accumulator. Two accumulators of 256 columns fill TMEM and leave no
+// Two shapes. Single: one CTA per 128 x 128 tile. PAIR: two CTAs on a 256 x 256 tile (cta_group::2): each loads its 128 rows of A, half of the W rows, the
+// scales of its rows and of ALL columns of the tile, and keeps its half of the accumulator. Two accumulators of 256 columns fill TMEM and leave no
 // room for scales, so they overlap: the first lies in columns [0, 256), the second in [128, 384), the scales behind them. The epilogue drains the 128
-// columns that both own first, and then the next tile's products begin; until then the tensor pipe waits, about 1.5 us per tile. Tiles of 192 columns
-// have two accumulators beside the scales and no such wait, for a third more loads per product.
+// columns that both own first, and then the next tile's products begin; until then the tensor pipe waits, about 1.5 us per tile. (Pairs on 192 columns, which
+// have two whole accumulators beside the scales, measured slower nearly everywhere: N 8192, K 2048, M 4096 37.3 us against 36.0, K 8192, N 2048 32.6 against 28.6.)
+//
+// What bounds it: a k step is 38 KB per CTA and comes from L2 at 64 bytes per clock and SM, 608 clocks, against 512 that the products of a 256 x 256 tile
+// take; measured 595. At 4 bits a larger tile, not a faster pipe, is what would help. 8192^3 199 us (5.5 PFLOP/s), M 4096, N 2048, K 8192 28.6 us (4.8).
 #pragma once
 #include "gemm_sm100.cuh"   // gelu, elect_one, pack16
 #include "quant4.cuh"
@@ -144,23 +147,20 @@ __device__ __forceinline__ void quant32(const uint64_t* v, uint4& codes, uint32_
     codes = make_uint4(words[0], words[1], words[2], words[3]);
 }
 
-template <int EPI, int FMT, int BN>
+template <int EPI, int FMT, bool PAIR>
 __global__ void __launch_bounds__(G_THREADS, 1)
 gemm4_kernel(const __grid_constant__ Gemm4Maps maps, const Gemm4Params p) {
-    static_assert(BN == 128 || BN == 192 || BN == 256, "tile width");
-    constexpr bool PAIR = BN != 128, OVERLAP = BN == 256;                 // OVERLAP: two accumulators share half of their columns
-    constexpr int TILE_M = PAIR ? 256 : 128, W_ROWS = PAIR ? BN / 2 : BN; // W rows that this CTA loads
-    constexpr int BUF_COLS = OVERLAP ? 128 : BN, ACC_SF = BUF_COLS + BN;  // TMEM: the second accumulator begins at BUF_COLS, the scales behind it
+    constexpr int BN = PAIR ? 256 : 128, TILE_M = PAIR ? 256 : 128;
+    constexpr int BUF_COLS = 128, ACC_SF = BUF_COLS + BN;                 // TMEM: the second accumulator begins at BUF_COLS, the scales behind it
     constexpr int PIECES = FMT == FMT_MX4 ? 2 : 4;                        // scale pieces of a k step per row block
     constexpr int W_BLOCKS = PAIR ? 2 : 1;                                // row blocks of W whose scales a CTA holds
     constexpr int SF_COLS = 4 * PIECES * (1 + W_BLOCKS);                  // TMEM columns of a step's scales
     constexpr int SF_BUFS = PAIR && FMT == FMT_NV4 ? 2 : 4;               // steps of them in flight
     static_assert(ACC_SF + SF_BUFS * SF_COLS <= (int)TMEM_ALL_COLUMNS, "TMEM");
-    constexpr uint32_t STAGE_TX = (GB_M + W_ROWS) * 128 + PIECES * 512 * (1 + W_BLOCKS);
+    constexpr uint32_t STAGE_TX = 32768 + PIECES * 512 * (1 + W_BLOCKS);
     constexpr bool OUT32 = EPI == EPI_F32 || EPI == EPI_RESID;
-    // Columns per chunk of the epilogue, which a warp has NCH / 2 of; a chunk leaves as one or two boxes of 32 rows x 128 bytes, or 64 where 32 16-bit columns are one
-    constexpr int CW = BN == 192 ? 32 : 64, NCH = BN / CW, BOX_COLS = OUT32 ? 32 : CW, BOXES = CW / BOX_COLS, BOX_ROW = BOX_COLS * (OUT32 ? 4 : 2);
-    constexpr int SLOTS = G4_STAGING_WARP / (32 * BOX_ROW);               // boxes on their way out at a time
+    constexpr int CW = 64, NCH = BN / CW;                                 // columns per chunk of the epilogue, which a warp has NCH / 2 of
+    constexpr int BOX_COLS = OUT32 ? 32 : CW, BOXES = CW / BOX_COLS;      // a chunk leaves as one or two boxes of 32 rows x 128 bytes
 
     extern __shared__ uint8_t smem_raw[];
     const uint32_t raw = smem_u32(smem_raw);
@@ -202,7 +202,7 @@ gemm4_kernel(const __grid_constant__ Gemm4Maps maps, const Gemm4Params p) {
         const uint32_t lane_base = (uint32_t)(quarter * 32) << 16;
         uint8_t* const my_stage = stage_out + warp * G4_STAGING_WARP;
         uint32_t use[2] = {0, 0};
-        int k = 0, box_use = 0;
+        int k = 0;
         for (int w = group; w < n_tiles; w += n_groups, ++k) {
             const int buf = k & 1;
             int tm, tn;
@@ -215,30 +215,29 @@ gemm4_kernel(const __grid_constant__ Gemm4Maps maps, const Gemm4Params p) {
             const int row = m0 + quarter * 32 + lane, nrow = p.M - (m0 + quarter * 32);
 #pragma unroll 1
             for (int i = 0; i < NCH / 2; i++) {
-                // OVERLAP: the columns that both accumulators own first; 192 columns: a warp's three chunks side by side
-                const int ch = OVERLAP ? half + 2 * (i ^ buf ^ 1) : half * (NCH / 2) + i;
+                const int ch = half + 2 * (PAIR ? i ^ buf ^ 1 : i);       // PAIR: the columns that both accumulators own first
                 uint64_t v[CW / 2];
                 {
                     uint32_t a[CW / 32][32];
 #pragma unroll
                     for (int q = 0; q < CW / 32; q++) tmem_ld32(tmem_base + lane_base + (uint32_t)(buf * BUF_COLS + ch * CW + 32 * q), a[q]);
                     tmem_wait_ld();
+#pragma unroll
+                    for (int q = 0; q < CW / 32; q++) reg_fence32(a[q]);
+                    if (i == 0) {                                         // what the next tile's products overwrite is in registers
+                        tc_fence_before();
+                        __syncwarp();
+                        if (lane == 0) {
+                            const uint32_t b = bar(G4BAR_ACC_EMPTY + (PAIR ? 0 : buf));
+                            if (PAIR && rank != 0) mbar_arrive_cluster(mapa_u32(b, 0));
+                            else mbar_arrive(b);
+                        }
+                    }
                     const uint64_t alpha = pack2(p.alpha, p.alpha);
 #pragma unroll
-                    for (int q = 0; q < CW / 32; q++) {
-                        reg_fence32(a[q]);
+                    for (int q = 0; q < CW / 32; q++)
 #pragma unroll
                         for (int e = 0; e < 16; e++) v[16 * q + e] = mul2(pack2u(a[q][2 * e], a[q][2 * e + 1]), alpha);
-                    }
-                }
-                if (i == (OVERLAP ? 0 : NCH / 2 - 1)) {                   // what the next products overwrite is in registers
-                    tc_fence_before();
-                    __syncwarp();
-                    if (lane == 0) {
-                        const uint32_t b = bar(G4BAR_ACC_EMPTY + (OVERLAP ? 0 : buf));
-                        if (PAIR && rank != 0) mbar_arrive_cluster(mapa_u32(b, 0));
-                        else mbar_arrive(b);
-                    }
                 }
                 const int c0 = n0 + ch * CW;
                 if constexpr (EPI == EPI_GELU16 || EPI == EPI_GELU4) {
@@ -308,12 +307,10 @@ gemm4_kernel(const __grid_constant__ Gemm4Maps maps, const Gemm4Params p) {
                             }
                             continue;
                         }
-                        uint8_t* const box = my_stage + (SLOTS == 2 ? (box_use & 1) * 32 * BOX_ROW : 0);
-                        ++box_use;
-                        if (lane == 0) { if (SLOTS == 2) tma_store_wait_read_1(); else tma_store_wait_read(); }   // the box that was here has been read
+                        if (lane == 0) tma_store_wait_read();             // the box that was here has been read
                         __syncwarp();
 #pragma unroll
-                        for (int c = 0; c < BOX_ROW / 16; c++) {
+                        for (int c = 0; c < 8; c++) {
                             uint4 pk;
                             if constexpr (OUT32) {
                                 const uint64_t* const u = v + b * 16 + 2 * c;
@@ -323,16 +320,13 @@ gemm4_kernel(const __grid_constant__ Gemm4Maps maps, const Gemm4Params p) {
                                 auto two = [](uint64_t w) { float lo, hi; unpack2(w, lo, hi); return pack16<DT_F16>(lo, hi); };
                                 pk = make_uint4(two(u[0]), two(u[1]), two(u[2]), two(u[3]));
                             }
-                            const int piece = BOX_ROW == 128 ? c ^ (lane & 7) : c ^ ((lane >> 1) & 3);
-                            *reinterpret_cast<uint4*>(box + lane * BOX_ROW + (piece << 4)) = pk;
+                            *reinterpret_cast<uint4*>(my_stage + lane * 128 + ((c ^ (lane & 7)) << 4)) = pk;
                         }
                         fence_proxy_async_smem();
                         __syncwarp();
-                        if (lane == 0) {                                  // an empty group where nothing is stored, so that groups count boxes
-                            if (nrow > 0 && x < p.N) {
-                                if constexpr (EPI == EPI_RESID) tma_reduce_add_3d(&maps.c, smem_u32(box), x, y, 0);
-                                else tma_store_3d(&maps.c, smem_u32(box), x, y, 0);
-                            }
+                        if (lane == 0 && nrow > 0 && x < p.N) {
+                            if constexpr (EPI == EPI_RESID) tma_reduce_add_3d(&maps.c, smem_u32(my_stage), x, y, 0);
+                            else tma_store_3d(&maps.c, smem_u32(my_stage), x, y, 0);
                             tma_store_commit();
                         }
                     }
@@ -343,12 +337,16 @@ gemm4_kernel(const __grid_constant__ Gemm4Maps maps, const Gemm4Params p) {
     } else if (warp == G_EPI_WARPS) {
         setmaxnreg_dec<56>();
         if (rank == 0 && elect_one()) {
-            uint32_t ring = 0, use[2] = {0, 0};
+            // the products of a step take the pipe 0.3 us, little more than what this thread spends on one: counters instead of remainders
+            uint32_t st = 0, phase = 0;                                   // stage and its parity
+            uint32_t old_st = G4_STAGES - SF_BUFS, old_phase = 1;         // those of the step that had this buffer of scales (passes at once where there was none)
+            uint32_t sf = 0, use[2] = {0, 0};
             bool good = true;
             int k = 0;
             for (int w = group; w < n_tiles && good; w += n_groups, ++k) {
                 const int buf = k & 1;
-                if (OVERLAP) {
+                const uint32_t acc = tmem_base + (uint32_t)(buf * BUF_COLS);
+                if (PAIR) {
                     // the tile before this one is out of the shared columns, so the one before that is out of all of its own
                     if (k > 0) good = mbar_wait(bar(G4BAR_ACC_EMPTY), (uint32_t)(k - 1) & 1u, abort_flag);
                 } else {
@@ -357,19 +355,14 @@ gemm4_kernel(const __grid_constant__ Gemm4Maps maps, const Gemm4Params p) {
                 ++use[buf];
                 if (!good) break;
                 tc_fence_after();
-                // 192 columns: every other tile begins in the middle of a row block of scales, two TMEM columns further
-                int tm, tn;
-                gemm4_tile(w, p, tm, tn);
-                const uint32_t sfb_skip = BN == 192 ? (uint32_t)(tn & 1) * 2u : 0u;
-                for (int ks = 0; ks < ksteps && good; ++ks, ++ring) {
-                    const uint32_t st = ring % G4_STAGES;
-                    good = mbar_wait(bar(G4BAR_FULL + st), (ring / G4_STAGES) & 1u, abort_flag);
+                for (int ks = 0; ks < ksteps; ++ks) {
+                    good = mbar_wait(bar(G4BAR_FULL + st), phase, abort_flag);
                     // the products that read this buffer of scales are done
-                    if (good && ring >= SF_BUFS) good = mbar_wait(bar(G4BAR_EMPTY + (ring - SF_BUFS) % G4_STAGES), ((ring - SF_BUFS) / G4_STAGES) & 1u, abort_flag);
+                    good = good && mbar_wait(bar(G4BAR_EMPTY + old_st), old_phase, abort_flag);
                     if (!good) break;
                     tc_fence_after();
                     const uint32_t a_s = base + st * G4_STAGE_BYTES;
-                    const uint32_t sfa = tmem_base + ACC_SF + (ring % SF_BUFS) * SF_COLS, sfb = sfa + 4 * PIECES;
+                    const uint32_t sfa = tmem_base + ACC_SF + sf * SF_COLS, sfb = sfa + 4 * PIECES;
                     const uint64_t sdesc = smem_desc_scales(a_s + G4_SF_OFF);
 #pragma unroll
                     for (int q = 0; q < PIECES; q++) {
@@ -381,10 +374,13 @@ gemm4_kernel(const __grid_constant__ Gemm4Maps maps, const Gemm4Params p) {
 #pragma unroll
                     for (int kk = 0; kk < 4; kk++) {
                         const int q = kk * PIECES / 4, byte = FMT == FMT_MX4 ? (kk & 1) * 2 : 0;
-                        mma_f4<FMT, PAIR>(tmem_base + (uint32_t)(buf * BUF_COLS), adesc + (uint64_t)(kk * 2), wdesc + (uint64_t)(kk * 2),
-                                          idesc_f4(FMT == FMT_MX4, TILE_M, BN, byte), sfa + 4 * q, sfb + sfb_skip + 4 * q * W_BLOCKS, (ks > 0 || kk > 0) ? 1u : 0u);
+                        mma_f4<FMT, PAIR>(acc, adesc + (uint64_t)(kk * 2), wdesc + (uint64_t)(kk * 2), idesc_f4(FMT == FMT_MX4, TILE_M, BN, byte), sfa + 4 * q,
+                                          sfb + 4 * q * W_BLOCKS, (ks > 0 || kk > 0) ? 1u : 0u);
                     }
                     if (PAIR) tc_commit_pair(bar(G4BAR_EMPTY + st), (uint16_t)3); else tc_commit(bar(G4BAR_EMPTY + st));
+                    if (++st == G4_STAGES) { st = 0; phase ^= 1u; }
+                    if (++old_st == G4_STAGES) { old_st = 0; old_phase ^= 1u; }
+                    if (++sf == SF_BUFS) sf = 0;
                 }
                 if (good) { if (PAIR) tc_commit_pair(bar(G4BAR_ACC_FULL + buf), (uint16_t)3); else tc_commit(bar(G4BAR_ACC_FULL + buf)); }
             }
@@ -408,10 +404,10 @@ gemm4_kernel(const __grid_constant__ Gemm4Maps maps, const Gemm4Params p) {
                         if (rank == 0) mbar_expect_tx(bar(G4BAR_FULL + st), 2 * STAGE_TX);
                         const uint32_t fb = mapa_u32(bar(G4BAR_FULL + st), 0);
                         tma_load_3d_pair(a_s, &maps.a, fb, ks * 128, tm * TILE_M + (int)rank * 128, 0);
-                        tma_load_3d_pair(a_s + 16384, &maps.w, fb, ks * 128, tn * BN + (int)rank * W_ROWS, 0);
+                        tma_load_3d_pair(a_s + 16384, &maps.w, fb, ks * 128, tn * BN + (int)rank * 128, 0);
                         tma_load_3d_pair(s_s, &maps.sa, fb, 0, ks * PIECES, tm * 2 + (int)rank);
 #pragma unroll
-                        for (int b = 0; b < W_BLOCKS; b++) tma_load_3d_pair(s_s + PIECES * 512 * (1 + b), &maps.sw, fb, 0, ks * PIECES, tn * BN / 128 + b);
+                        for (int b = 0; b < W_BLOCKS; b++) tma_load_3d_pair(s_s + PIECES * 512 * (1 + b), &maps.sw, fb, 0, ks * PIECES, tn * W_BLOCKS + b);
                     } else {
                         const uint32_t fb = bar(G4BAR_FULL + st);
                         mbar_expect_tx(fb, STAGE_TX);

@@ -90,7 +90,7 @@ struct BlockScale {
             q = fmaf(fmaf(-q, 6.f, a), sixth, q);
             byte = max(e4m3_byte(q), 1u);
             s = e4m3_value(byte);
-            r = __frcp_rn(s);
+            r = __fdividef(1.f, s);                            // its last bit does not matter: the correction has the rest
         }
         if (abs_bits >= 0x7f800000u) byte = FMT == FMT_MX4 ? 255u : 127u;
     }
@@ -133,36 +133,38 @@ struct Quant4Params {
     uint8_t* codes;
     uint8_t* scales;
     int rows, cols, ld_x, ld;    // ld: bytes of a row of codes
-    int pieces, segs;            // pieces of a row block; groups of Q4_SEGS x 256 columns of a row
+    int pieces;                  // of a row block
     int exp;
     bool wide;
 };
 
-// A lane takes eight columns, so that a block is two (NV4) or four (MX4) lanes, which meet by shuffles; a warp 256 columns side by side, Q4_SEGS
+// A lane takes eight columns, so that a block is two (NV4) or four (MX4) lanes, which meet by shuffles; a warp 256 columns side by side, q4_segs
 // times, its loads first. Bound by memory: 16-bit rows 2 bytes read and 0.56 written per element.
-constexpr int Q4_THREADS = 128, Q4_SEGS = 2;
+constexpr int Q4_THREADS = 128;
+template <typename T> __host__ __device__ constexpr int q4_segs() { return sizeof(T) == 2 ? 4 : 2; }
 
 template <typename T, int FMT>
 __global__ void __launch_bounds__(Q4_THREADS)
 quant4_kernel(const Quant4Params p) {
+    constexpr int SEGS = q4_segs<T>();
     pdl_launch();
     pdl_wait();
-    const long long unit = (long long)blockIdx.x * (Q4_THREADS / 32) + (threadIdx.x >> 5);
-    const long long row64 = unit / p.segs;
-    if (row64 >= p.rows) return;
-    const int row = (int)row64, lane = threadIdx.x & 31;
-    const int c0 = (int)(unit % p.segs) * (Q4_SEGS * 256) + lane * 8;
+    const unsigned row = blockIdx.x * (Q4_THREADS / 32) + (threadIdx.x >> 5);
+    if (row >= (unsigned)p.rows) return;
+    const int lane = threadIdx.x & 31, c0 = (int)blockIdx.y * (SEGS * 256) + lane * 8;
     const T* const src = static_cast<const T*>(p.x) + (size_t)row * p.ld_x;
     const float down = pow2f(-p.exp);
-    F8 f[Q4_SEGS];
+    F8 f[SEGS];
 #pragma unroll
-    for (int i = 0; i < Q4_SEGS; i++) f[i] = load8(src, c0 + i * 256, p.cols, p.wide);
+    for (int i = 0; i < SEGS; i++) f[i] = load8(src, c0 + i * 256, p.cols, p.wide);
 #pragma unroll
-    for (int i = 0; i < Q4_SEGS; i++) {
+    for (int i = 0; i < SEGS; i++) {
         const int c = c0 + i * 256;
-        uint32_t top = 0u;
-#pragma unroll
-        for (int e = 0; e < 8; e++) top = max(top, __float_as_uint(f[i].v[e]) & 0x7fffffffu);
+        if (c - lane * 8 >= p.cols) break;                     // the whole warp is behind the last column (a piece never begins there)
+        float big = max3_abs_nan(f[i].v[0], f[i].v[1], f[i].v[2]);
+        big = max3_abs_nan(big, f[i].v[3], f[i].v[4]);
+        big = max3_abs_nan(big, f[i].v[5], f[i].v[6]);
+        uint32_t top = __float_as_uint(max3_abs_nan(big, f[i].v[7], 0.f)) & 0x7fffffffu;
         top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
         if (FMT == FMT_MX4) top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
         const BlockScale<FMT> bs(top, down);
@@ -200,18 +202,18 @@ __device__ __forceinline__ F8 q4_values8(const Quant4Params& p, int row, int c, 
 template <typename T, int FMT>
 __global__ void __launch_bounds__(Q4_THREADS)
 dequant4_kernel(const Quant4Params p) {
+    constexpr int SEGS = q4_segs<T>();
     pdl_launch();
     pdl_wait();
-    const long long unit = (long long)blockIdx.x * (Q4_THREADS / 32) + (threadIdx.x >> 5);
-    const long long row64 = unit / p.segs;
-    if (row64 >= p.rows) return;
-    const int row = (int)row64, c0 = (int)(unit % p.segs) * (Q4_SEGS * 256) + (threadIdx.x & 31) * 8;
+    const unsigned row = blockIdx.x * (Q4_THREADS / 32) + (threadIdx.x >> 5);
+    if (row >= (unsigned)p.rows) return;
+    const int c0 = (int)blockIdx.y * (SEGS * 256) + (threadIdx.x & 31) * 8;
     T* const dst = static_cast<T*>(p.y) + (size_t)row * p.ld_x;
     const float up = pow2f(p.exp);
 #pragma unroll
-    for (int i = 0; i < Q4_SEGS; i++) {
+    for (int i = 0; i < SEGS; i++) {
         const int c = c0 + i * 256;
-        if (c < p.cols) store8(dst, c, p.cols, p.wide, q4_values8<FMT>(p, row, c, up));
+        if (c < p.cols) store8(dst, c, p.cols, p.wide, q4_values8<FMT>(p, (int)row, c, up));
     }
 }
 

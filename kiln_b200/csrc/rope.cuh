@@ -6,106 +6,154 @@
 // and a position an integer, so their product modulo 2^64 IS the fraction of the turn, exactly, in two integer multiplications: the
 // only rounding is that of the fraction to 32 bits (2^-32 of a turn) and the sine's own.
 //
-// Bound by memory. The sines of a row serve all of its heads: a thread block takes rows, its threads first fill shared memory with one
-// (cos, sin) per row and pair, then turn the heads, eight elements of either side of the pairs at a time.
+// Bound by memory. The sines of a row serve all of its heads of all tensors: a thread block takes a row (several where they are short), fills shared memory
+// with one (cos, sin) per pair, and every thread keeps those of its eight elements while it goes from head to head, its loads in front.
 #pragma once
-#include "quant4.cuh"   // load8, store8
+#include "quant4.cuh"   // to_f32, from_f32
 
 namespace kb {
 
 constexpr int ROPE_MAX_PAIRS = 128, ROPE_MAX_TENSORS = 4, ROPE_THREADS = 128;
-constexpr int ROPE_SLOTS = 512;                        // (row, pair) places in shared memory
+constexpr int ROPE_SLOTS = 1024;                       // (row, pair) places in shared memory
 
 struct RopeTensor {
     const void* x;
     void* y;
-    int heads, ld_x, ld_y;
+    int first, ld_x, ld_y;                             // first: its first head among those of all tensors
 };
 struct RopeParams {
     RopeTensor t[ROPE_MAX_TENSORS];
     unsigned long long freq[ROPE_MAX_PAIRS];           // turns per position, a 64-bit fraction
     unsigned char axis[ROPE_MAX_PAIRS];
     const int* pos;                                    // [pos_rows, ld_pos]; row r takes row r % pos_rows
-    int n, rows, pos_rows, ld_pos, dim, rot, block_rows, inverse;
+    int n, heads, rows, pos_rows, ld_pos, dim, rot, block_rows, inverse;
     float amplitude;
-    bool wide;                                         // rows of all tensors start on 16 bytes
 };
 
-// VEC: pieces of eight elements. HALF needs rot / 2 to be a multiple of 8 for it (the launch decides); else element by element.
+// What a thread takes of a head: eight elements of either side of the pairs (HALF), eight elements, or pieces of the part that does not turn.
+struct RopeUnits {
+    int per_head, turned, slots;                       // units of a head, those that turn, (cos, sin) places of a row
+};
+__host__ __device__ inline RopeUnits rope_units(bool half, int dim, int rot) {
+    const int pairs = rot / 2, each = half ? 8 : 4, turned = (pairs + each - 1) / each;
+    return {half ? turned + (dim - rot) / 8 : dim / 8, turned, turned * each};
+}
+inline int rope_block_rows(bool half, bool vec, int dim, int rot, int heads) {
+    if (!vec) return 1;
+    const RopeUnits u = rope_units(half, dim, rot);
+    const int n = ROPE_THREADS / (u.per_head * heads);
+    return n > 1 ? n : 1;
+}
+
+// VEC: in pieces of eight elements, where every row starts on 16 bytes and a head (HALF: either side of the pairs too) is whole pieces; else a warp takes a head,
+// element by element.
 template <typename T, bool HALF, bool VEC>
 __global__ void __launch_bounds__(ROPE_THREADS)
 rope_kernel(const __grid_constant__ RopeParams p) {
     __shared__ float2 cs[ROPE_SLOTS];
+    constexpr int EACH = HALF ? 8 : 4;
     pdl_launch();
     pdl_wait();
     const int pairs = p.rot >> 1;
-    const long long row0 = (long long)blockIdx.x * p.block_rows;
-    const int rows = (int)min((long long)p.block_rows, (long long)p.rows - row0);
+    const RopeUnits un = rope_units(HALF, p.dim, p.rot);
+    const int stride = VEC ? un.slots : pairs;
+    const unsigned row0 = blockIdx.x * (unsigned)p.block_rows;
+    const int rows = (int)min((unsigned)p.block_rows, (unsigned)p.rows - row0);
     for (int i = threadIdx.x; i < rows * pairs; i += ROPE_THREADS) {
         const int r = i / pairs, f = i - r * pairs;
-        const int pos = p.pos[(size_t)((row0 + r) % p.pos_rows) * p.ld_pos + p.axis[f]];
+        const int pos = p.pos[(size_t)((row0 + (unsigned)r) % (unsigned)p.pos_rows) * p.ld_pos + p.axis[f]];
         const unsigned long long turn = (unsigned long long)(long long)pos * p.freq[f];
         float sn, cn;
         sincospif((float)(int)(turn >> 32) * 0x1p-31f, &sn, &cn);     // in half turns, [-1, 1)
-        cs[i] = make_float2(cn * p.amplitude, (p.inverse ? -sn : sn) * p.amplitude);
+        // VEC: a unit's pairs apart, those of neighbouring units side by side, so that neighbouring lanes read neighbouring words
+        const int at = VEC ? (f % EACH) * un.turned + f / EACH : f;
+        cs[r * stride + at] = make_float2(cn * p.amplitude, (p.inverse ? -sn : sn) * p.amplitude);
     }
     __syncthreads();
-    for (int k = 0; k < p.n; k++) {
-        const RopeTensor& t = p.t[k];
-        if (VEC) {
-            const int pieces = p.dim >> 3, half = pairs >> 3, turned = HALF ? half : 0, rest = HALF ? pieces - 2 * half : pieces;
-            const int per_head = turned + rest, n = rows * t.heads * per_head;     // HALF: `turned` pairs of pieces, then copied pieces
-            for (int i = threadIdx.x; i < n; i += ROPE_THREADS) {
-                const int r = i / (t.heads * per_head), j = i - r * (t.heads * per_head), h = j / per_head, s = j - h * per_head;
-                const T* const src = static_cast<const T*>(t.x) + (size_t)(row0 + r) * t.ld_x + h * p.dim;
-                T* const dst = static_cast<T*>(t.y) + (size_t)(row0 + r) * t.ld_y + h * p.dim;
-                const float2* const row_cs = cs + r * pairs;
-                if (HALF) {
-                    if (s < turned) {
-                        const F8 a = Io<T>::ld8(src + 8 * s), b = Io<T>::ld8(src + pairs + 8 * s);
-                        F8 u, v;
+    auto head = [&](unsigned row, int v, const T*& src, T*& dst) {
+        const RopeTensor* t = &p.t[0];
 #pragma unroll
-                        for (int e = 0; e < 8; e++) {
-                            const float2 z = row_cs[8 * s + e];
-                            u.v[e] = a.v[e] * z.x - b.v[e] * z.y;
-                            v.v[e] = b.v[e] * z.x + a.v[e] * z.y;
-                        }
-                        Io<T>::st8(dst + 8 * s, u);
-                        Io<T>::st8(dst + pairs + 8 * s, v);
-                    } else {
-                        const int c = p.rot + 8 * (s - turned);
-                        Io<T>::st8(dst + c, Io<T>::ld8(src + c));
+        for (int k = 1; k < ROPE_MAX_TENSORS; k++)
+            if (k < p.n && v >= p.t[k].first) t = &p.t[k];
+        src = static_cast<const T*>(t->x) + (size_t)row * t->ld_x + (v - t->first) * p.dim;
+        dst = static_cast<T*>(t->y) + (size_t)row * t->ld_y + (v - t->first) * p.dim;
+    };
+    if constexpr (VEC) {
+        int r = 0, v, s, step;
+        if (p.block_rows == 1) {
+            step = ROPE_THREADS / un.per_head;
+            v = threadIdx.x / un.per_head;
+            s = threadIdx.x - v * un.per_head;
+            if (v >= step) return;
+        } else {                                       // every thread has one unit of one head of one row
+            const int all = un.per_head * p.heads;
+            r = threadIdx.x / all;
+            const int j = threadIdx.x - r * all;
+            v = j / un.per_head;
+            s = j - v * un.per_head;
+            step = p.heads;
+            if (r >= rows) return;
+        }
+        const unsigned row = row0 + (unsigned)r;
+        const bool turns = s < un.turned;
+        float2 z[EACH];
+#pragma unroll
+        for (int e = 0; e < EACH; e++) {
+            const bool in = turns && (HALF || EACH * s + e < pairs);   // interleaved: the last unit that turns may hold pairs that do not
+            z[e] = in ? cs[r * stride + e * un.turned + s] : make_float2(1.f, 0.f);
+        }
+        constexpr int U = sizeof(T) == 2 ? 4 : 2;      // heads whose loads are under way together
+        const int ca = HALF && !turns ? p.rot + 8 * (s - un.turned) : 8 * s, cb = pairs + 8 * s;
+        for (; v < p.heads; v += U * step) {
+            Raw8<T> a[U], b[U];
+            T* dst[U];
+#pragma unroll
+            for (int i = 0; i < U; i++) {
+                if (v + i * step >= p.heads) break;
+                const T* src;
+                head(row, v + i * step, src, dst[i]);
+                a[i] = Io<T>::raw8(src + ca);
+                if (HALF && turns) b[i] = Io<T>::raw8(src + cb);
+            }
+#pragma unroll
+            for (int i = 0; i < U; i++) {
+                if (v + i * step >= p.heads) break;
+                if (!turns) { Io<T>::st8(dst[i] + ca, Io<T>::f8(a[i])); continue; }
+                F8 x = Io<T>::f8(a[i]);
+                if constexpr (HALF) {
+                    F8 y = Io<T>::f8(b[i]);
+#pragma unroll
+                    for (int e = 0; e < 8; e++) {
+                        const float t = x.v[e];
+                        x.v[e] = t * z[e].x - y.v[e] * z[e].y;
+                        y.v[e] = y.v[e] * z[e].x + t * z[e].y;
                     }
+                    Io<T>::st8(dst[i] + cb, y);
                 } else {
-                    F8 a = Io<T>::ld8(src + 8 * s);
 #pragma unroll
                     for (int e = 0; e < 4; e++) {
-                        if (4 * s + e >= pairs) continue;
-                        const float2 z = row_cs[4 * s + e];
-                        const float x = a.v[2 * e], y = a.v[2 * e + 1];
-                        a.v[2 * e] = x * z.x - y * z.y;
-                        a.v[2 * e + 1] = y * z.x + x * z.y;
+                        const float t = x.v[2 * e], u = x.v[2 * e + 1];
+                        x.v[2 * e] = t * z[e].x - u * z[e].y;
+                        x.v[2 * e + 1] = u * z[e].x + t * z[e].y;
                     }
-                    Io<T>::st8(dst + 8 * s, a);
                 }
+                Io<T>::st8(dst[i] + ca, x);
             }
-        } else {
-            const int per_head = pairs + p.dim - p.rot, n = rows * t.heads * per_head;
-            for (int i = threadIdx.x; i < n; i += ROPE_THREADS) {
-                const int r = i / (t.heads * per_head), j = i - r * (t.heads * per_head), h = j / per_head, s = j - h * per_head;
-                const T* const src = static_cast<const T*>(t.x) + (size_t)(row0 + r) * t.ld_x + h * p.dim;
-                T* const dst = static_cast<T*>(t.y) + (size_t)(row0 + r) * t.ld_y + h * p.dim;
-                if (s < pairs) {
-                    const int ia = HALF ? s : 2 * s, ib = HALF ? pairs + s : 2 * s + 1;
-                    const float2 z = cs[r * pairs + s];
-                    const float x = to_f32(src[ia]), y = to_f32(src[ib]);
-                    dst[ia] = from_f32<T>(x * z.x - y * z.y);
-                    dst[ib] = from_f32<T>(y * z.x + x * z.y);
-                } else {
-                    const int c = p.rot + s - pairs;
-                    dst[c] = src[c];
-                }
+        }
+    } else {
+        const int lane = threadIdx.x & 31;
+        for (int v = threadIdx.x >> 5; v < p.heads; v += ROPE_THREADS / 32) {
+            const T* src;
+            T* dst;
+            head(row0, v, src, dst);
+            for (int s = lane; s < pairs; s += 32) {
+                const int ia = HALF ? s : 2 * s, ib = HALF ? pairs + s : 2 * s + 1;
+                const float2 z = cs[s];
+                const float x = to_f32(src[ia]), y = to_f32(src[ib]);
+                dst[ia] = from_f32<T>(x * z.x - y * z.y);
+                dst[ib] = from_f32<T>(y * z.x + x * z.y);
             }
+            for (int c = p.rot + lane; c < p.dim; c += 32) dst[c] = src[c];
         }
     }
 }

@@ -196,11 +196,11 @@ inline GemmShape gemm_shape(int M, int N, long long ksteps, int n_seg, bool any_
 #ifndef KB_G4
 #define KB_G4 0
 #endif
-inline int gemm4_width(int M, int N, int ksteps, int sm_count) {
-    if (KB_G4) return KB_G4;
+inline bool gemm4_pair(int M, int N, int ksteps, int epi, int sm_count) {
+    if (KB_G4) return KB_G4 == 256;
     const long long single = (((long long)(M + 127) / 128) * ((N + 127) / 128) + sm_count - 1) / sm_count;
     const long long pair = (((long long)(M + 255) / 256) * ((N + 255) / 256) + sm_count / 2 - 1) / (sm_count / 2);
-    return M > 128 && 16 * pair < 10 * single ? 256 : 128;
+    return M > 128 && 16 * pair < 10 * single;
 }
 
 }  // namespace kb

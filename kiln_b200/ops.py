@@ -7,6 +7,7 @@ op set (reference: engine/src/gpu.h:149-156): row-major [rows, ld] activations, 
 """
 import ctypes
 import os
+import struct
 
 KB_F16, KB_BF16, KB_F32 = 0, 1, 2
 
@@ -120,7 +121,7 @@ def lib():
         L.kb_rope_freqs.restype = i
         L.kb_rope_freqs.argtypes = [ctypes.POINTER(d), i, d, i, d, d, d, d]
         L.kb_rope.restype = i
-        L.kb_rope.argtypes = [i, pvp, pi, pvp, pi, pi, i, i, i, i, i, vp, i, i, i, vp, vp, f, i, vp]
+        L.kb_rope.argtypes = [i, vp, vp, vp, vp, vp, i, i, i, i, i, vp, i, i, i, vp, vp, f, i, vp]
         L.kb_dropout.restype = i
         L.kb_dropout.argtypes = [vp, i, i, vp, i, i, vp, i, i, i, d, vp, vp]
         _lib = L
@@ -379,7 +380,7 @@ def _q4_bytes(rows, cols, fmt):
 
 class Quant4:
     """A matrix [rows, cols] of 4-bit numbers in blocks (kb_quant4): codes uint8 [rows, >= 16 ceil(cols / 32)], scales uint8, fmt MX4 or NV4, 2^exp for all of it."""
-    __slots__ = ("codes", "scales", "rows", "cols", "fmt", "exp")
+    __slots__ = ("rows", "cols", "fmt", "exp", "device", "ld", "codes_ptr", "scales_ptr", "_codes", "_scales", "_both")
 
     def __init__(self, codes, scales, rows, cols, fmt, exp=0):
         row_bytes, scale_bytes = _q4_bytes(rows, cols, fmt)
@@ -390,7 +391,24 @@ class Quant4:
             raise ValueError(f"codes {tuple(have)} do not hold {rows} rows of {cols} columns")
         if scales.numel() < scale_bytes:
             raise ValueError(f"scales of {scales.numel()} bytes do not hold {rows} rows of {cols} columns")
-        self.codes, self.scales, self.rows, self.cols, self.fmt, self.exp = codes, scales, rows, cols, fmt, exp
+        self.device = codes.get_device()
+        if scales.get_device() != self.device:
+            raise ValueError("codes and scales lie on one device")
+        self.rows, self.cols, self.fmt, self.exp, self._codes, self._scales, self._both = rows, cols, fmt, exp, codes, scales, None
+        self.ld, self.codes_ptr, self.scales_ptr = st[0], codes.data_ptr(), scales.data_ptr()
+
+    # what quant4_empty makes is one buffer: the two views cost more than a launch and are made when they are asked for
+    @property
+    def codes(self):
+        if self._codes is None:
+            self._codes = self._both[:self.rows * self.ld].view(self.rows, self.ld)
+        return self._codes
+
+    @property
+    def scales(self):
+        if self._scales is None:
+            self._scales = self._both[self.rows * self.ld:]
+        return self._scales
 
 
 def quant4_empty(rows, cols, fmt, device, exp=0):
@@ -398,10 +416,16 @@ def quant4_empty(rows, cols, fmt, device, exp=0):
     import torch
     row_bytes, scale_bytes = _q4_bytes(rows, cols, fmt)
     q = Quant4.__new__(Quant4)                     # what is made here needs no checks
-    q.codes = torch.empty((rows, row_bytes), dtype=torch.uint8, device=device)
-    q.scales = torch.empty(scale_bytes, dtype=torch.uint8, device=device)
-    q.rows, q.cols, q.fmt, q.exp = rows, cols, fmt, exp
+    q._both = both = torch.empty((rows * row_bytes + scale_bytes,), dtype=torch.uint8, device=device)
+    q._codes = q._scales = None
+    q.rows, q.cols, q.fmt, q.exp, q.ld, q.device = rows, cols, fmt, exp, row_bytes, both.get_device()
+    q.codes_ptr = p = both.data_ptr()              # a row of codes is a multiple of 16 bytes
+    q.scales_ptr = p + rows * row_bytes
     return q
+
+
+def _elsewhere(device, dev):
+    raise ValueError(f"4-bit matrix on device {device}, but the current device is cuda:{dev}")
 
 
 def quant4(x, fmt, exp=0, out=None):
@@ -412,20 +436,20 @@ def quant4(x, fmt, exp=0, out=None):
     elif (out.rows, out.cols, out.fmt, out.exp) != (rows, cols, fmt, exp):
         raise ValueError("out was made for another matrix")
     stream, dev = _stream_device()
-    codes, scales = out.codes, out.scales
-    _here(dev, x, codes, scales)
-    _check(lib().kb_quant4(codes.data_ptr(), codes.stride(0), scales.data_ptr(), x.data_ptr(), _ld(x), _dt(x), rows, cols, fmt, exp, stream), "kb_quant4")
+    if x.get_device() != dev or out.device != dev:
+        _elsewhere(x.device, dev)
+    _check(lib().kb_quant4(out.codes_ptr, out.ld, out.scales_ptr, x.data_ptr(), _ld(x), _dt(x), rows, cols, fmt, exp, stream), "kb_quant4")
     return out
 
 
 def dequant4(y, q, transpose=False):
     """y [rows, cols], or with transpose [cols, rows], fp16 / bf16 / fp32 = the values that q stands for."""
-    if tuple(y.shape) != ((q.cols, q.rows) if transpose else (q.rows, q.cols)):
+    if y.shape != ((q.cols, q.rows) if transpose else (q.rows, q.cols)):
         raise ValueError(f"y {tuple(y.shape)} for a matrix of {q.rows} x {q.cols}")
     stream, dev = _stream_device()
-    _here(dev, y, q.codes, q.scales)
-    _check(lib().kb_dequant4(_ptr(y), _ld(y), _dt(y), _ptr(q.codes), q.codes.stride(0), _ptr(q.scales), q.rows, q.cols, q.fmt, q.exp, int(transpose), stream),
-           "kb_dequant4")
+    if y.get_device() != dev or q.device != dev:
+        _elsewhere(y.device, dev)
+    _check(lib().kb_dequant4(y.data_ptr(), _ld(y), _dt(y), q.codes_ptr, q.ld, q.scales_ptr, q.rows, q.cols, q.fmt, q.exp, transpose, stream), "kb_dequant4")
     return y
 
 
@@ -438,39 +462,41 @@ def linear4(C, A, W, epi, gate=None, alpha=1.0):
     if epi == EPI_GELU4:
         if not isinstance(C, Quant4) or (C.rows, C.cols, C.fmt, C.exp) != (M, N, A.fmt, 0):
             raise ValueError("EPI_GELU4 goes into a Quant4 [M, N] of the operands' format with exp 0")
-        out, scales = C.codes, C.scales
-        ldc = out.stride(0)
+        out, ldc, scales, there = C.codes_ptr, C.ld, C.scales_ptr, C.device
     else:
-        out, scales = C, None
         if isinstance(C, Quant4) or C.shape != (M, N) or _dt(C) != (KB_F32 if epi in (EPI_F32, EPI_RESID) else KB_F16):
             raise ValueError("C is [M, N] of its epilogue's type")
-        ldc = _ld(C)
-    if gate is not None and (_dt(gate) != KB_F32 or gate.numel() < N or not gate.is_contiguous()):
-        raise ValueError("gate is fp32 [N]")
+        out, ldc, scales, there = C.data_ptr(), _ld(C), None, C.get_device()
+    if gate is not None:
+        if _dt(gate) != KB_F32 or gate.numel() < N or not gate.is_contiguous() or gate.get_device() != there:
+            raise ValueError("gate is fp32 [N], where C is")
+        gate = gate.data_ptr()
     stream, dev = _stream_device()
-    a, sa, w, sw = A.codes, A.scales, W.codes, W.scales
-    _here(dev, out, scales, a, sa, w, sw, gate)
-    _check(lib().kb_linear4(out.data_ptr(), ldc, _ptr(scales), a.data_ptr(), a.stride(0), sa.data_ptr(), w.data_ptr(), w.stride(0), sw.data_ptr(), M, N, K, A.fmt,
-                            epi, alpha * 2.0 ** (A.exp + W.exp), _ptr(gate), stream), "kb_linear4")
+    if not there == A.device == W.device == dev:
+        _elsewhere((there, A.device, W.device), dev)
+    _check(lib().kb_linear4(out, ldc, scales, A.codes_ptr, A.ld, A.scales_ptr, W.codes_ptr, W.ld, W.scales_ptr, M, N, K, A.fmt, epi,
+                            alpha * 2.0 ** (A.exp + W.exp), gate, stream), "kb_linear4")
     return C
 
 
 def linear4_dx(dx, dy, W, workspace=None):
     """dx [M, K] (fp16 or fp32) = dy [M, N] @ W for a 4-bit W [N, K]: the gradient of linear4's input. dy fp16."""
-    import torch
     M, N = dy.shape
-    if N != W.rows or tuple(dx.shape) != (M, W.cols) or _dt(dy) != KB_F16:
+    if N != W.rows or dx.shape != (M, W.cols) or _dt(dy) != KB_F16:
         raise ValueError("dy is fp16 [M, N], dx [M, K] for a weight of [N, K]")
     if workspace is None:
-        workspace = torch.empty(lib().kb_linear4_dx_workspace_bytes(N, W.cols), dtype=torch.uint8, device=dy.device)
+        import torch
+        workspace = torch.empty((2 * N * W.cols,), dtype=torch.uint8, device=dy.device)      # kb_linear4_dx_workspace_bytes
     stream, dev = _stream_device()
-    _here(dev, dx, dy, W.codes, W.scales, workspace)
+    if not W.device == dy.get_device() == dx.get_device() == workspace.get_device() == dev:
+        _elsewhere((W.device, dy.device, dx.device, workspace.device), dev)
     wp, wb = _ws(workspace)
-    _check(lib().kb_linear4_dx(_ptr(dx), _ld(dx), _dt(dx), _ptr(dy), _ld(dy), _ptr(W.codes), W.codes.stride(0), _ptr(W.scales), M, N, W.cols, W.fmt, W.exp,
-                               wp, wb, stream), "kb_linear4_dx")
+    _check(lib().kb_linear4_dx(dx.data_ptr(), _ld(dx), _dt(dx), dy.data_ptr(), _ld(dy), W.codes_ptr, W.ld, W.scales_ptr, M, N, W.cols, W.fmt, W.exp, wp, wb, stream),
+           "kb_linear4_dx")
     return dx
 
 
+_F64 = _I32 = _INT32 = None    # types, filled when first needed
 ROPE_HALF, ROPE_INTERLEAVED = 0, 1
 ROPE_PLAIN, ROPE_LINEAR, ROPE_BASE, ROPE_PARTS = 0, 1, 2, 3
 
@@ -484,42 +510,54 @@ def rope_freqs(rot_dim, base=10000.0, scaling=ROPE_PLAIN, factor=1.0, trained_le
     return freq
 
 
+_PTRS = [struct.Struct("Q" * n) for n in range(5)]     # host arrays of pointers and sizes as bytes: a quarter of a ctypes array's time
+_INTS = [struct.Struct("i" * n) for n in range(5)]
+
+
 def rope(outs, xs, heads, head_dim, pos, freq, axis=None, layout=ROPE_HALF, amplitude=1.0, inverse=False):
     """Rotary positions of up to four tensors xs[k] [rows, heads[k] * head_dim] of one type in one launch; outs may be xs. pos: int32 [pos_rows, axes] on the
     device (row r takes pos[r % pos_rows]); freq (float64) and axis (int32 or None), one entry per pair, numpy arrays on the host. inverse = the gradient."""
-    import numpy as np
-    import torch
+    global _F64, _I32, _INT32
+    if _F64 is None:
+        import numpy as np
+        import torch
+        _F64, _I32, _INT32 = np.dtype(np.float64), np.dtype(np.int32), torch.int32
     n = len(xs)
-    if len(outs) != n or len(heads) != n or not n:
-        raise ValueError("one output and one number of heads per tensor")
-    rows = xs[0].shape[0]
+    if not 1 <= n <= 4 or len(outs) != n or len(heads) != n:
+        raise ValueError("one to four tensors, an output and a number of heads each")
+    rows, dt = xs[0].shape[0], xs[0].dtype
+    px, po, lx, lo = [], [], [], []
     for o, x, h in zip(outs, xs, heads):
-        if x.shape[0] != rows or x.shape[1] < h * head_dim or o.shape[0] != rows or o.shape[1] < h * head_dim or o.dtype != x.dtype or x.dtype != xs[0].dtype:
+        if x.shape[0] != rows or x.shape[1] < h * head_dim or o.shape[0] != rows or o.shape[1] < h * head_dim or o.dtype != dt or x.dtype != dt:
             raise ValueError("tensors are [rows, heads * head_dim] of one type")
-    if pos.dtype != torch.int32 or pos.dim() != 2 or (pos.shape[1] > 1 and pos.stride(1) != 1):
+        px.append(x.data_ptr())
+        po.append(o.data_ptr())
+        lx.append(_ld(x))
+        lo.append(_ld(o))
+    if pos.dtype != _INT32 or pos.dim() != 2 or (pos.shape[1] > 1 and pos.stride(1) != 1):
         raise ValueError("pos is int32 [rows, axes]")
-    if freq.dtype != np.float64 or not freq.flags.c_contiguous or (axis is not None and (axis.dtype != np.int32 or not axis.flags.c_contiguous or axis.size != freq.size)):
+    if freq.dtype != _F64 or freq.ndim != 1 or (axis is not None and (axis.dtype != _I32 or axis.shape != freq.shape)):
         raise ValueError("freq is float64 and axis int32, one per pair")
     stream, dev = _stream_device()
-    _here(dev, pos, *outs, *xs)
-    vpn, in_ = ctypes.c_void_p * n, ctypes.c_int * n
-    _check(lib().kb_rope(n, vpn(*[o.data_ptr() for o in outs]), in_(*[_ld(o) for o in outs]), vpn(*[x.data_ptr() for x in xs]), in_(*[_ld(x) for x in xs]),
-                         in_(*heads), _dt(xs[0]), rows, head_dim, 2 * freq.size, layout, _ptr(pos), pos.shape[0], pos.stride(0), pos.shape[1], freq.__array_interface__["data"][0],
-                         None if axis is None else axis.__array_interface__["data"][0], amplitude, int(inverse), stream), "kb_rope")
+    _here(dev, pos, *xs, *outs)
+    ptrs, ints = _PTRS[n].pack, _INTS[n].pack
+    _check(lib().kb_rope(n, ptrs(*po), ints(*lo), ptrs(*px), ints(*lx), ints(*heads), _dt(xs[0]), rows, head_dim, 2 * freq.size, layout, pos.data_ptr(),
+                         pos.shape[0], pos.stride(0), pos.shape[1], freq.tobytes(), None if axis is None else axis.tobytes(), amplitude, inverse, stream),
+           "kb_rope")
     return outs
 
 
 def dropout(out, x, rng, p, resid=None):
     """out = dropout(x) (+ resid); rng: int64 [2] on the device, seed and offset. The gradient is dropout(dout) with the same rng (see kb_dropout)."""
-    import torch
+    rows, cols = x.shape
     if out.shape != x.shape or (resid is not None and (resid.shape != x.shape or resid.dtype != out.dtype)):
         raise ValueError("out, x and resid have one shape, out and resid one type")
-    if rng.dtype not in (torch.int64, torch.uint64) or rng.numel() != 2 or not rng.is_contiguous():
+    if rng.element_size() != 8 or rng.is_floating_point() or rng.numel() != 2 or not rng.is_contiguous():
         raise ValueError("rng is int64 [2]: seed and offset")
     stream, dev = _stream_device()
     _here(dev, out, x, rng, resid)
-    _check(lib().kb_dropout(_ptr(out), _ld(out), _dt(out), _ptr(x), _ld(x), _dt(x), _ptr(resid), 0 if resid is None else _ld(resid), x.shape[0], x.shape[1], p,
-                            _ptr(rng), stream), "kb_dropout")
+    _check(lib().kb_dropout(out.data_ptr(), _ld(out), _dt(out), x.data_ptr(), _ld(x), _dt(x), _ptr(resid), 0 if resid is None else _ld(resid), rows, cols, p,
+                            rng.data_ptr(), stream), "kb_dropout")
     return out
 
 

@@ -324,10 +324,10 @@ def test_product_outputs_in_wider_rows(built_lib):
 def test_product_of_no_rows(built_lib):
     from kiln_b200 import ops
     A, W = ops.quant4_empty(0, 64, NV4, "cuda"), ops.quant4(_x(1, 16, 64).cuda(), NV4)
-    A.codes, A.scales = torch.empty(1, 32, dtype=torch.uint8, device="cuda"), torch.empty(512, dtype=torch.uint8, device="cuda")
-    out = torch.empty(1, 16, device="cuda")[:0]
-    assert ops.lib().kb_linear4(W.scales.data_ptr(), 16, None, A.codes.data_ptr(), 32, A.scales.data_ptr(), W.codes.data_ptr(), 32, W.scales.data_ptr(), 0, 16, 64, NV4, 0,
-                                1.0, None, None) == 0 and out.numel() == 0
+    some = W.scales_ptr                                                    # an address, as an empty tensor has none
+    assert ops.lib().kb_linear4(some, 16, None, some, 32, some, W.codes_ptr, 32, W.scales_ptr, 0, 16, 64, NV4, 0, 1.0, None, None) == 0 and A.rows == 0
+    assert ops.lib().kb_quant4(some, 32, some, some, 64, 0, 0, 64, NV4, 0, None) == 0
+    assert ops.lib().kb_linear4_dx(some, 64, 0, some, 64, W.codes_ptr, 32, W.scales_ptr, 0, 64, 64, NV4, 0, None, 0, None) == 0
 
 
 @gpu

@@ -38,7 +38,8 @@ def test_refusals(built_lib):
     buf = (ctypes.c_char * 4096)()
     a = (ctypes.addressof(buf) + 255) & ~255
     f = (ctypes.c_double * 128)(*([0.5] * 128))
-    vp1, i1 = ctypes.c_void_p * 1, ctypes.c_int * 1
+    import struct
+    vp1, i1 = (lambda v: struct.pack('Q', v or 0)), (lambda v: struct.pack('i', v))
 
     def r(n=1, out=a, ldo=256, x=a, ldx=256, heads=2, dt=0, rows=4, dim=128, rot=128, layout=0, pos=a, prows=4, ldp=1, axes=1, freq=f, axis=None):
         return L.kb_rope(n, vp1(out), i1(ldo), vp1(x), i1(ldx), i1(heads), dt, rows, dim, rot, layout, pos, prows, ldp, axes, freq, axis, 1.0, 0, None)
@@ -170,6 +171,7 @@ def test_no_rows(built_lib):
     x = torch.empty(4, 128, device="cuda")[:0]
     base = torch.empty(1, 128, device="cuda")
     pos, f = torch.zeros(1, 1, dtype=torch.int32, device="cuda"), ops.rope_freqs(128)
-    vp1, i1 = ctypes.c_void_p * 1, ctypes.c_int * 1
+    import struct
+    vp1, i1 = (lambda v: struct.pack('Q', v)), (lambda v: struct.pack('i', v))
     assert x.numel() == 0 and ops.lib().kb_rope(1, vp1(base.data_ptr()), i1(128), vp1(base.data_ptr()), i1(128), i1(1), 2, 0, 128, 128, 0, pos.data_ptr(), 1, 1, 1, f.ctypes.data,
                                                 None, 1.0, 0, None) == 0

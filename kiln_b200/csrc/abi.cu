@@ -1002,18 +1002,17 @@ inline size_t elem_size(int dtype) { return dtype == KB_F32 ? 4 : 2; }
 inline bool wide_rows(const void* p, int ld, int dtype) { return aligned16(p) && (ld * elem_size(dtype)) % 16 == 0; }
 
 // a warp per row and group of columns
-template <typename T>
 dim3 quant4_grid(const Quant4Params& p) {
-    constexpr int COLS = q4_segs<T>() * 256, WARPS = Q4_THREADS / 32;
+    constexpr int COLS = Q4_SEGS * 256, WARPS = Q4_THREADS / 32;
     static_assert(KB_MAX_Q4_COLS / COLS <= 65535, "grid");
     return dim3((unsigned)(((long long)p.rows + WARPS - 1) / WARPS), (unsigned)((p.cols + COLS - 1) / COLS));
 }
 
 template <int FMT>
 int launch_quant4(Quant4Params& p, int dtype, cudaStream_t stream) {
-    if (dtype == KB_F16) return launch_dependent(quant4_kernel<__half, FMT>, quant4_grid<__half>(p), dim3(Q4_THREADS), 0, stream, nullptr, p);
-    if (dtype == KB_BF16) return launch_dependent(quant4_kernel<__nv_bfloat16, FMT>, quant4_grid<__nv_bfloat16>(p), dim3(Q4_THREADS), 0, stream, nullptr, p);
-    return launch_dependent(quant4_kernel<float, FMT>, quant4_grid<float>(p), dim3(Q4_THREADS), 0, stream, nullptr, p);
+    if (dtype == KB_F16) return launch_dependent(quant4_kernel<__half, FMT>, quant4_grid(p), dim3(Q4_THREADS), 0, stream, nullptr, p);
+    if (dtype == KB_BF16) return launch_dependent(quant4_kernel<__nv_bfloat16, FMT>, quant4_grid(p), dim3(Q4_THREADS), 0, stream, nullptr, p);
+    return launch_dependent(quant4_kernel<float, FMT>, quant4_grid(p), dim3(Q4_THREADS), 0, stream, nullptr, p);
 }
 
 template <int FMT, typename T>
@@ -1023,7 +1022,7 @@ int launch_dequant4_t(Quant4Params& p, bool transpose, cudaStream_t stream) {
         if (blocks > 0x7fffffffLL) return KB_ERR_SHAPE;
         return launch_dependent(dequant4_t_kernel<T, FMT>, dim3((unsigned)blocks), dim3(256), 0, stream, nullptr, p);
     }
-    return launch_dependent(dequant4_kernel<T, FMT>, quant4_grid<T>(p), dim3(Q4_THREADS), 0, stream, nullptr, p);
+    return launch_dependent(dequant4_kernel<T, FMT>, quant4_grid(p), dim3(Q4_THREADS), 0, stream, nullptr, p);
 }
 
 template <int FMT>

@@ -33,7 +33,7 @@ struct DropoutParams {
 };
 
 // A thread takes DROP_GROUPS groups of eight columns, its loads first.
-constexpr int DROP_THREADS_LOG2 = 8, DROP_THREADS = 1 << DROP_THREADS_LOG2, DROP_GROUPS = 2;
+constexpr int DROP_THREADS_LOG2 = 8, DROP_THREADS = 1 << DROP_THREADS_LOG2, DROP_GROUPS = 1;
 
 template <typename InT, typename OutT>
 __global__ void __launch_bounds__(DROP_THREADS)
@@ -47,6 +47,7 @@ dropout_kernel(const DropoutParams p) {
     const InT* const x = static_cast<const InT*>(p.x) + (size_t)row * p.ld_x;
     OutT* const y = static_cast<OutT*>(p.y) + (size_t)row * p.ld_y;
     const unsigned long long seed = p.rng[0], offset = p.rng[1];
+    const uint32_t t = p.t << 16;
     F8 in[DROP_GROUPS], out[DROP_GROUPS];
 #pragma unroll
     for (int i = 0; i < DROP_GROUPS; i++) {
@@ -66,8 +67,9 @@ dropout_kernel(const DropoutParams p) {
         const uint32_t words[4] = {w.x, w.y, w.z, w.w};
 #pragma unroll
         for (int e = 0; e < 8; e++) {
-            const uint32_t r = (e & 1) ? words[e >> 1] >> 16 : words[e >> 1] & 0xffffu;
-            if (r >= p.t) out[i].v[e] = __fadd_rn(out[i].v[e], __fmul_rn(in[i].v[e], p.scale));   // product and sum rounded apart, with a residual and without
+            // a half word against t is the word, with that half on top, against 2^16 t
+            const uint32_t r = (e & 1) ? words[e >> 1] : words[e >> 1] << 16;
+            if (r >= t) out[i].v[e] = __fadd_rn(out[i].v[e], __fmul_rn(in[i].v[e], p.scale));   // product and sum rounded apart, with a residual and without
         }
         store8(y, c, p.cols, p.wide, out[i]);
     }

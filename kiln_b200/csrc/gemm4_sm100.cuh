@@ -128,21 +128,10 @@ __device__ __forceinline__ void quant32(const uint64_t* v, uint4& codes, uint32_
             unpack2(v[b * BLK / 2 + e], x, y);
             top = max3_abs_nan(top, x, y);
         }
-        const BlockScale<FMT> bs(__float_as_uint(top) & 0x7fffffffu, 1.f);
+        const BlockScale<FMT> bs(__float_as_uint(top) & 0x7fffffffu, 1.f, 1.f);
         scale_bytes |= bs.byte << (8 * b);
-        const uint64_t r = pack2(bs.r, bs.r), ns = pack2(-bs.s, -bs.s);
 #pragma unroll
-        for (int i = 0; i < BLK / 8; i++) {
-            float q[8];
-#pragma unroll
-            for (int e = 0; e < 4; e++) {
-                const uint64_t y = v[b * BLK / 2 + 4 * i + e];
-                uint64_t z = mul2(y, r);
-                if (FMT == FMT_NV4) z = fma2(fma2(z, ns, y), r, z);
-                unpack2(z, q[2 * e], q[2 * e + 1]);
-            }
-            words[b * (BLK / 8) + i] = e2m1_pack8(q);
-        }
+        for (int i = 0; i < BLK / 8; i++) words[b * (BLK / 8) + i] = bs.codes(v + b * BLK / 2 + 4 * i);
     }
     codes = make_uint4(words[0], words[1], words[2], words[3]);
 }

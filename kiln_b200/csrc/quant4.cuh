@@ -72,13 +72,13 @@ __device__ __forceinline__ float q4_scale_value(uint32_t byte) {
     return byte == 0u ? __uint_as_float(0x00400000u) : byte == 255u ? __uint_as_float(0x7fffffffu) : __uint_as_float(byte << 23);
 }
 
-// The scale of a block whose largest |x| has these bits: its byte, and what elements are divided by (s) and multiplied with (r = 1 / s).
+// The scale of a block whose largest |x| has these bits: its byte, and with 2^exp what elements are divided by (s) and multiplied with (r ~ 1 / s).
 template <int FMT>
 struct BlockScale {
     uint32_t byte;
     float s, r;
-    // down = 2^-exp of the matrix (NV4)
-    __device__ __forceinline__ BlockScale(uint32_t abs_bits, float down) {
+    // down, up = 2^-exp, 2^exp of the matrix (NV4)
+    __device__ __forceinline__ BlockScale(uint32_t abs_bits, float down, float up) {
         if (FMT == FMT_MX4) {
             const uint32_t e = abs_bits >> 23;
             byte = e > 2u ? e - 2u : 0u;                       // floor(log2 a) + 127 - 2
@@ -89,15 +89,22 @@ struct BlockScale {
             float q = a * sixth;
             q = fmaf(fmaf(-q, 6.f, a), sixth, q);
             byte = max(e4m3_byte(q), 1u);
-            s = e4m3_value(byte);
+            s = e4m3_value(byte) * up;
             r = __fdividef(1.f, s);                            // its last bit does not matter: the correction has the rest
         }
         if (abs_bits >= 0x7f800000u) byte = FMT == FMT_MX4 ? 255u : 127u;
     }
-    __device__ __forceinline__ float operator()(float x, float down) const {
-        if (FMT == FMT_MX4) return x * r;
-        const float y = x * down, q = y * r;
-        return fmaf(fmaf(-q, s, y), r, q);
+    // eight elements, as packed pairs, to eight codes
+    __device__ __forceinline__ uint32_t codes(const uint64_t* v) const {
+        const uint64_t r2 = pack2(r, r), ns2 = pack2(-s, -s);
+        float q[8];
+#pragma unroll
+        for (int e = 0; e < 4; e++) {
+            uint64_t z = mul2(v[e], r2);
+            if (FMT == FMT_NV4) z = fma2(fma2(z, ns2, v[e]), r2, z);
+            unpack2(z, q[2 * e], q[2 * e + 1]);
+        }
+        return e2m1_pack8(q);
     }
 };
 
@@ -120,6 +127,14 @@ __device__ __forceinline__ F8 load8(const T* row, int c, int cols, bool wide) {
     return f;
 }
 template <typename T>
+__device__ __forceinline__ Raw8<T> load8_raw(const T* row, int c, int cols, bool wide) {
+    if (wide && c + 8 <= cols) return Io<T>::raw8(row + c);
+    Raw8<T> r;
+#pragma unroll
+    for (int i = 0; i < 8; i++) reinterpret_cast<T*>(r.u)[i] = c + i < cols ? row[c + i] : from_f32<T>(0.f);
+    return r;
+}
+template <typename T>
 __device__ __forceinline__ void store8(T* row, int c, int cols, bool wide, const F8& f) {
     if (wide && c + 8 <= cols) { Io<T>::st8(row + c, f); return; }
 #pragma unroll
@@ -138,40 +153,39 @@ struct Quant4Params {
     bool wide;
 };
 
-// A lane takes eight columns, so that a block is two (NV4) or four (MX4) lanes, which meet by shuffles; a warp 256 columns side by side, q4_segs
+// A lane takes eight columns, so that a block is two (NV4) or four (MX4) lanes, which meet by shuffles; a warp 256 columns side by side, Q4_SEGS
 // times, its loads first. Bound by memory: 16-bit rows 2 bytes read and 0.56 written per element.
-constexpr int Q4_THREADS = 128;
-template <typename T> __host__ __device__ constexpr int q4_segs() { return sizeof(T) == 2 ? 4 : 2; }
+constexpr int Q4_THREADS = 128, Q4_SEGS = 2;
 
 template <typename T, int FMT>
-__global__ void __launch_bounds__(Q4_THREADS)
+__global__ void __launch_bounds__(Q4_THREADS, 12)
 quant4_kernel(const Quant4Params p) {
-    constexpr int SEGS = q4_segs<T>();
     pdl_launch();
     pdl_wait();
     const unsigned row = blockIdx.x * (Q4_THREADS / 32) + (threadIdx.x >> 5);
     if (row >= (unsigned)p.rows) return;
-    const int lane = threadIdx.x & 31, c0 = (int)blockIdx.y * (SEGS * 256) + lane * 8;
+    const int lane = threadIdx.x & 31, c0 = (int)blockIdx.y * (Q4_SEGS * 256) + lane * 8;
     const T* const src = static_cast<const T*>(p.x) + (size_t)row * p.ld_x;
-    const float down = pow2f(-p.exp);
-    F8 f[SEGS];
+    const float down = pow2f(-p.exp), up = pow2f(p.exp);
+    Raw8<T> raw[Q4_SEGS];
 #pragma unroll
-    for (int i = 0; i < SEGS; i++) f[i] = load8(src, c0 + i * 256, p.cols, p.wide);
+    for (int i = 0; i < Q4_SEGS; i++) raw[i] = load8_raw(src, c0 + i * 256, p.cols, p.wide);
 #pragma unroll
-    for (int i = 0; i < SEGS; i++) {
+    for (int i = 0; i < Q4_SEGS; i++) {
         const int c = c0 + i * 256;
         if (c - lane * 8 >= p.cols) break;                     // the whole warp is behind the last column (a piece never begins there)
-        float big = max3_abs_nan(f[i].v[0], f[i].v[1], f[i].v[2]);
-        big = max3_abs_nan(big, f[i].v[3], f[i].v[4]);
-        big = max3_abs_nan(big, f[i].v[5], f[i].v[6]);
-        uint32_t top = __float_as_uint(max3_abs_nan(big, f[i].v[7], 0.f)) & 0x7fffffffu;
+        const F8 f = Io<T>::f8(raw[i]);
+        float big = max3_abs_nan(f.v[0], f.v[1], f.v[2]);
+        big = max3_abs_nan(big, f.v[3], f.v[4]);
+        big = max3_abs_nan(big, f.v[5], f.v[6]);
+        uint32_t top = __float_as_uint(max3_abs_nan(big, f.v[7], 0.f)) & 0x7fffffffu;
         top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
         if (FMT == FMT_MX4) top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
-        const BlockScale<FMT> bs(top, down);
-        float v[8];
+        const BlockScale<FMT> bs(top, down, up);
+        uint64_t v[4];
 #pragma unroll
-        for (int e = 0; e < 8; e++) v[e] = bs(f[i].v[e], down);
-        if (c < q4_row_bytes(p.cols) * 2) *reinterpret_cast<uint32_t*>(p.codes + (size_t)row * p.ld + (c >> 1)) = e2m1_pack8(v);
+        for (int e = 0; e < 4; e++) v[e] = pack2(f.v[2 * e], f.v[2 * e + 1]);
+        if (c < q4_row_bytes(p.cols) * 2) *reinterpret_cast<uint32_t*>(p.codes + (size_t)row * p.ld + (c >> 1)) = bs.codes(v);
         // the four scales of a piece, 8 (NV4) or 16 lanes, meet in its first lane
         constexpr int STEP = q4_block(FMT) / 8;
         uint32_t word = c < p.cols ? bs.byte << (8 * ((lane / STEP) & 3)) : 0u;
@@ -182,13 +196,33 @@ quant4_kernel(const Quant4Params p) {
     }
 }
 
-// eight values from column c (a multiple of 8) of a row, up = 2^exp
+// eight codes from column c (a multiple of 8) of a row, and their scale's byte
+struct Q4Raw { uint32_t codes, scale; };
 template <int FMT>
-__device__ __forceinline__ F8 q4_values8(const Quant4Params& p, int row, int c, float up) {
-    uint32_t h[4];
-    e2m1_unpack8(*reinterpret_cast<const uint32_t*>(p.codes + (size_t)row * p.ld + (c >> 1)), h);
+__device__ __forceinline__ Q4Raw q4_load8(const Quant4Params& p, int row, int c) {
     const int b = c / q4_block(FMT);
-    const float s = q4_scale_value<FMT>(p.scales[q4_scale_at(row, b >> 2, p.pieces) + (b & 3)]) * up;
+    return {*reinterpret_cast<const uint32_t*>(p.codes + (size_t)row * p.ld + (c >> 1)), p.scales[q4_scale_at(row, b >> 2, p.pieces) + (b & 3)]};
+}
+// The values in T, as they lie in memory; up = 2^exp. In fp16 the product is taken in fp16 where the scale is one of its numbers: the same single rounding.
+template <typename T, int FMT>
+__device__ __forceinline__ Raw8<T> q4_values8(const Q4Raw& q, float up) {
+    uint32_t h[4];
+    e2m1_unpack8(q.codes, h);
+    const float s = q4_scale_value<FMT>(q.scale) * up;
+    Raw8<T> out;
+    if constexpr (std::is_same<T, __half>::value) {
+        const __half sh = __float2half_rn(s);
+        if (__half2float(sh) == s) {
+            const __half2 s2 = __half2half2(sh);
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+                const __half2 v = __hmul2(*reinterpret_cast<const __half2*>(&h[i]), s2);
+                h[i] = *reinterpret_cast<const uint32_t*>(&v);
+            }
+            out.u[0] = make_uint4(h[0], h[1], h[2], h[3]);
+            return out;
+        }
+    }
     F8 f;
 #pragma unroll
     for (int i = 0; i < 4; i++) {
@@ -196,24 +230,40 @@ __device__ __forceinline__ F8 q4_values8(const Quant4Params& p, int row, int c, 
         f.v[2 * i] = v.x * s;
         f.v[2 * i + 1] = v.y * s;
     }
-    return f;
+    Io<T>::st8(reinterpret_cast<T*>(out.u), f);
+    return out;
 }
+// an element of eight that lie in registers
+template <typename T>
+__device__ __forceinline__ T q4_pick(const Raw8<T>& r, int e) { return reinterpret_cast<const T*>(r.u)[e]; }
 
 template <typename T, int FMT>
 __global__ void __launch_bounds__(Q4_THREADS)
 dequant4_kernel(const Quant4Params p) {
-    constexpr int SEGS = q4_segs<T>();
     pdl_launch();
     pdl_wait();
     const unsigned row = blockIdx.x * (Q4_THREADS / 32) + (threadIdx.x >> 5);
     if (row >= (unsigned)p.rows) return;
-    const int c0 = (int)blockIdx.y * (SEGS * 256) + (threadIdx.x & 31) * 8;
+    const int c0 = (int)blockIdx.y * (Q4_SEGS * 256) + (threadIdx.x & 31) * 8;
     T* const dst = static_cast<T*>(p.y) + (size_t)row * p.ld_x;
     const float up = pow2f(p.exp);
+    Q4Raw q[Q4_SEGS];
 #pragma unroll
-    for (int i = 0; i < SEGS; i++) {
+    for (int i = 0; i < Q4_SEGS; i++)
+        if (c0 + i * 256 < p.cols) q[i] = q4_load8<FMT>(p, (int)row, c0 + i * 256);
+#pragma unroll
+    for (int i = 0; i < Q4_SEGS; i++) {
         const int c = c0 + i * 256;
-        if (c < p.cols) store8(dst, c, p.cols, p.wide, q4_values8<FMT>(p, (int)row, c, up));
+        if (c >= p.cols) break;
+        const Raw8<T> v = q4_values8<T, FMT>(q[i], up);
+        if (p.wide && c + 8 <= p.cols) {
+#pragma unroll
+            for (int u = 0; u < (int)sizeof(T) / 2; u++) reinterpret_cast<uint4*>(dst + c)[u] = v.u[u];
+        } else {
+#pragma unroll
+            for (int e = 0; e < 8; e++)
+                if (c + e < p.cols) dst[c + e] = q4_pick(v, e);
+        }
     }
 }
 
@@ -230,26 +280,28 @@ dequant4_t_kernel(const Quant4Params p) {
     const int r0 = (int)(blockIdx.x / (unsigned)tiles_c) * Q4_TILE, k0 = (int)(blockIdx.x % (unsigned)tiles_c) * Q4_TILE;
     const int pair = threadIdx.x & 31, kg = threadIdx.x >> 5;
     const float up = pow2f(p.exp);
-    F8 f[2];
+    Q4Raw q[2] = {{0u, 0u}, {0u, 0u}};
 #pragma unroll
-    for (int i = 0; i < 2; i++) {
-        const int r = r0 + 2 * pair + i, c = k0 + 8 * kg;
-        if (r < p.rows && c < p.cols) f[i] = q4_values8<FMT>(p, r, c, up);
-        else
-#pragma unroll
-            for (int e = 0; e < 8; e++) f[i].v[e] = 0.f;
-    }
+    for (int i = 0; i < 2; i++)
+        if (r0 + 2 * pair + i < p.rows && k0 + 8 * kg < p.cols) q[i] = q4_load8<FMT>(p, r0 + 2 * pair + i, k0 + 8 * kg);
+    const Raw8<T> v0 = q4_values8<T, FMT>(q[0], up), v1 = q4_values8<T, FMT>(q[1], up);
 #pragma unroll
     for (int e = 0; e < 8; e++) {
-        struct alignas(2 * sizeof(T)) Two { T a, b; } two = {from_f32<T>(f[0].v[e]), from_f32<T>(f[1].v[e])};
+        struct alignas(2 * sizeof(T)) Two { T a, b; } two = {q4_pick(v0, e), q4_pick(v1, e)};
         *reinterpret_cast<Two*>(&tile[(8 * kg + e) * Q4_TILE_LD + 2 * pair]) = two;
     }
     __syncthreads();
-    for (int i = threadIdx.x; i < Q4_TILE * Q4_TILE / 8; i += 256) {
-        const int k = i / (Q4_TILE / 8), c = (i % (Q4_TILE / 8)) * 8;
-        if (k0 + k >= p.cols || r0 + c >= p.rows) continue;
-        const F8 v = Io<T>::ld8(&tile[k * Q4_TILE_LD + c]);
-        store8(static_cast<T*>(p.y) + (size_t)(k0 + k) * p.ld_x + r0, c, p.rows - r0, p.wide, v);
+    constexpr int EACH = 16 / sizeof(T), ACROSS = Q4_TILE / EACH;      // elements of 16 bytes
+    for (int i = threadIdx.x; i < Q4_TILE * ACROSS; i += 256) {
+        const int k = i / ACROSS, c = (i % ACROSS) * EACH, left = p.rows - r0 - c;
+        if (k0 + k >= p.cols || left <= 0) continue;
+        T* const dst = static_cast<T*>(p.y) + (size_t)(k0 + k) * p.ld_x + r0 + c;
+        const uint4 v = *reinterpret_cast<const uint4*>(&tile[k * Q4_TILE_LD + c]);
+        if (p.wide && left >= EACH) *reinterpret_cast<uint4*>(dst) = v;
+        else
+#pragma unroll
+            for (int e = 0; e < EACH; e++)
+                if (e < left) dst[e] = reinterpret_cast<const T*>(&v)[e];
     }
 }
 

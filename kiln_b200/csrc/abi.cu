@@ -1004,6 +1004,7 @@ inline bool wide_rows(const void* p, int ld, int dtype) { return aligned16(p) &&
 // a warp per row and group of columns
 dim3 quant4_grid(const Quant4Params& p) {
     constexpr int COLS = Q4_SEGS * 256, WARPS = Q4_THREADS / 32;
+    static_assert(COLS == DEQ_COLS, "one grid for both directions");
     static_assert(KB_MAX_Q4_COLS / COLS <= 65535, "grid");
     return dim3((unsigned)(((long long)p.rows + WARPS - 1) / WARPS), (unsigned)((p.cols + COLS - 1) / COLS));
 }
@@ -1225,12 +1226,17 @@ int launch_rope_t(const RopeParams& p, bool half, bool vec, unsigned blocks, cud
     return launch_dependent(rope_kernel<T, false, false>, grid, block, 0, stream, nullptr, p);
 }
 
+template <typename InT, typename OutT>
+int launch_dropout_t(const DropoutParams& p, dim3 grid, cudaStream_t stream) {
+    if (p.resid) return launch_dependent(dropout_kernel<InT, OutT, true>, grid, dim3(DROP_THREADS), 0, stream, nullptr, p);
+    return launch_dependent(dropout_kernel<InT, OutT, false>, grid, dim3(DROP_THREADS), 0, stream, nullptr, p);
+}
+
 template <typename InT>
-int launch_dropout_t(const DropoutParams& p, int out_dtype, dim3 grid, cudaStream_t stream) {
-    const dim3 block(DROP_THREADS);
-    if (out_dtype == KB_F16) return launch_dependent(dropout_kernel<InT, __half>, grid, block, 0, stream, nullptr, p);
-    if (out_dtype == KB_BF16) return launch_dependent(dropout_kernel<InT, __nv_bfloat16>, grid, block, 0, stream, nullptr, p);
-    return launch_dependent(dropout_kernel<InT, float>, grid, block, 0, stream, nullptr, p);
+int launch_dropout(const DropoutParams& p, int out_dtype, dim3 grid, cudaStream_t stream) {
+    if (out_dtype == KB_F16) return launch_dropout_t<InT, __half>(p, grid, stream);
+    if (out_dtype == KB_BF16) return launch_dropout_t<InT, __nv_bfloat16>(p, grid, stream);
+    return launch_dropout_t<InT, float>(p, grid, stream);
 }
 
 }  // namespace
@@ -1300,15 +1306,18 @@ int kb_dropout(void* out, int ld_out, int out_dtype, const void* in, int ld_in, 
     p.t = t; p.scale = (float)(65536.0 / (65536.0 - t));
     p.wide = wide_rows(in, ld_in, in_dtype) && wide_rows(out, ld_out, out_dtype) && (!resid || wide_rows(resid, ld_resid, out_dtype));
     // a row of a block's threads as wide as a row of the matrix, up to all of them
-    const long long groups = ((long long)cols + 8 * DROP_GROUPS - 1) / (8 * DROP_GROUPS);
+    const long long groups = ((long long)cols + 7) / 8;
     while (p.width_log2 < DROP_THREADS_LOG2 && 1LL << p.width_log2 < groups) ++p.width_log2;
     const long long across = (groups + (1LL << p.width_log2) - 1) >> p.width_log2, block_rows = DROP_THREADS >> p.width_log2;
     if (across > 65535) return KB_ERR_SHAPE;
-    const dim3 grid((unsigned)(((long long)rows + block_rows - 1) / block_rows), (unsigned)across);
+    // 16-bit: one round of thread blocks, each on its share of the rows; fp32: a thread block per rows that it holds at once (see the kernel)
+    const long long down = ((long long)rows + block_rows - 1) / block_rows, room = (long long)DROP_BLOCKS_PER_SM * st->sm_count / across;
+    const bool one_round = in_dtype != KB_F32 && out_dtype != KB_F32 && down > room;
+    const dim3 grid((unsigned)(one_round ? (room > 1 ? room : 1) : down), (unsigned)across);
     ProfScope ps(st, KB_PROF_LINEAR, stream);
-    if (in_dtype == KB_F16) return launch_dropout_t<__half>(p, out_dtype, grid, stream);
-    if (in_dtype == KB_BF16) return launch_dropout_t<__nv_bfloat16>(p, out_dtype, grid, stream);
-    return launch_dropout_t<float>(p, out_dtype, grid, stream);
+    if (in_dtype == KB_F16) return launch_dropout<__half>(p, out_dtype, grid, stream);
+    if (in_dtype == KB_BF16) return launch_dropout<__nv_bfloat16>(p, out_dtype, grid, stream);
+    return launch_dropout<float>(p, out_dtype, grid, stream);
 }
 
 int kb_lora_pack(void* dst_f16, int ld, int col0, const void* src_bf16, int rows, int cols, float scale, void* stream) {

@@ -235,35 +235,48 @@ __device__ __forceinline__ Raw8<T> q4_values8(const Q4Raw& q, float up) {
 }
 // an element of eight that lie in registers
 template <typename T>
-__device__ __forceinline__ T q4_pick(const Raw8<T>& r, int e) { return reinterpret_cast<const T*>(r.u)[e]; }
+__device__ __forceinline__ T q4_pick(const Raw8<T>& r, int e) {
+    T v = reinterpret_cast<const T*>(r.u)[0];
+#pragma unroll
+    for (int i = 1; i < 8; i++) v = e == i ? reinterpret_cast<const T*>(r.u)[i] : v;
+    return v;
+}
 
+// A lane takes 16 bytes of output where rows start on 16 bytes (fp32: half of eight codes), so that every store of a warp is 512 bytes in a row; else a
+// column, DEQ_COLS / 32 times.
+constexpr int DEQ_COLS = 512;                   // columns of a warp
 template <typename T, int FMT>
 __global__ void __launch_bounds__(Q4_THREADS)
 dequant4_kernel(const Quant4Params p) {
+    constexpr int EACH = 16 / sizeof(T), N = DEQ_COLS / (32 * EACH);
     pdl_launch();
     pdl_wait();
     const unsigned row = blockIdx.x * (Q4_THREADS / 32) + (threadIdx.x >> 5);
     if (row >= (unsigned)p.rows) return;
-    const int c0 = (int)blockIdx.y * (Q4_SEGS * 256) + (threadIdx.x & 31) * 8;
+    const int first = (int)blockIdx.y * DEQ_COLS, lane = threadIdx.x & 31;
     T* const dst = static_cast<T*>(p.y) + (size_t)row * p.ld_x;
     const float up = pow2f(p.exp);
-    Q4Raw q[Q4_SEGS];
+    if (!p.wide) {
+        for (int c = first + lane; c < min(first + DEQ_COLS, p.cols); c += 32) dst[c] = q4_pick(q4_values8<T, FMT>(q4_load8<FMT>(p, (int)row, c & ~7), up), c & 7);
+        return;
+    }
+    Q4Raw q[N];
 #pragma unroll
-    for (int i = 0; i < Q4_SEGS; i++)
-        if (c0 + i * 256 < p.cols) q[i] = q4_load8<FMT>(p, (int)row, c0 + i * 256);
+    for (int i = 0; i < N; i++) {
+        const int c = first + (i * 32 + lane) * EACH;
+        if (c < p.cols) q[i] = q4_load8<FMT>(p, (int)row, c & ~7);
+    }
 #pragma unroll
-    for (int i = 0; i < Q4_SEGS; i++) {
-        const int c = c0 + i * 256;
+    for (int i = 0; i < N; i++) {
+        const int c = first + (i * 32 + lane) * EACH;
         if (c >= p.cols) break;
         const Raw8<T> v = q4_values8<T, FMT>(q[i], up);
-        if (p.wide && c + 8 <= p.cols) {
+        const uint4 out = EACH == 8 ? v.u[0] : (c & 4) ? v.u[sizeof(T) / 2 - 1] : v.u[0];
+        if (c + EACH <= p.cols) *reinterpret_cast<uint4*>(dst + c) = out;
+        else
 #pragma unroll
-            for (int u = 0; u < (int)sizeof(T) / 2; u++) reinterpret_cast<uint4*>(dst + c)[u] = v.u[u];
-        } else {
-#pragma unroll
-            for (int e = 0; e < 8; e++)
-                if (c + e < p.cols) dst[c + e] = q4_pick(v, e);
-        }
+            for (int e = 0; e < EACH; e++)
+                if (c + e < p.cols) dst[c + e] = reinterpret_cast<const T*>(&out)[e];
     }
 }
 

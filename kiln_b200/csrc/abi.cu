@@ -18,6 +18,7 @@
 #include "attn_bwd_sm100.cuh"
 #include "quant4.cuh"
 #include "gemm4_sm100.cuh"
+#include "gemv4.cuh"
 #include "rope.cuh"
 #include "dropout.cuh"
 #include "routes.h"
@@ -1086,6 +1087,12 @@ int launch_gemm4_epi(DeviceState* st, int epi, const Gemm4Maps& maps, const Gemm
     }
 }
 
+template <int FMT>
+int launch_gemv4(const Gemv4Params& p, cudaStream_t stream) {
+    const dim3 grid((unsigned)(((p.N + 127) / 128 * 32 + GV4_WARPS - 1) / GV4_WARPS)), block(32 * GV4_WARPS);
+    return launch_dependent(gemv4_kernel<FMT>, grid, block, 0, stream, nullptr, p);
+}
+
 }  // namespace
 
 extern "C" {
@@ -1154,6 +1161,12 @@ int kb_linear4(void* C, int ldc, void* C_scales, const void* A, int lda, const v
     DeviceState* st;
     if ((rc = get_state(&st))) return rc;
     if (M == 0) return KB_OK;
+    ProfScope ps(st, KB_PROF_LINEAR, stream);
+    if (M == 1 && !out4) {                                        // a block of 4-bit output is 32 columns side by side, which lie in several warps there
+        Gemv4Params g = {static_cast<const uint8_t*>(A), static_cast<const uint8_t*>(A_scales), static_cast<const uint8_t*>(W), static_cast<const uint8_t*>(W_scales),
+                         C, gate, N, K, ldw, q4_pieces(K, fmt), alpha, epi};
+        return fmt == KB_MX4 ? launch_gemv4<FMT_MX4>(g, stream) : launch_gemv4<FMT_NV4>(g, stream);
+    }
     Gemm4Maps maps;
     memset(&maps, 0, sizeof(maps));
     if ((rc = make_tmap_codes(&maps.a, A, M, K, lda)) || (rc = make_tmap_codes(&maps.w, W, N, K, ldw)) ||
@@ -1163,7 +1176,6 @@ int kb_linear4(void* C, int ldc, void* C_scales, const void* A, int lda, const v
     Gemm4Params p = {};
     p.M = M; p.N = N; p.K = K; p.alpha = alpha; p.C = C; p.ldc = ldc; p.gate = gate; p.status = st->status;
     if (out4) { p.codes = static_cast<uint8_t*>(C); p.scales = static_cast<uint8_t*>(C_scales); p.ld_codes = ldc; p.pieces = q4_pieces(N, fmt); }
-    ProfScope ps(st, KB_PROF_LINEAR, stream);
     return fmt == KB_MX4 ? launch_gemm4_epi<FMT_MX4>(st, epi, maps, p, stream) : launch_gemm4_epi<FMT_NV4>(st, epi, maps, p, stream);
 }
 

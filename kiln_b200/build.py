@@ -1,4 +1,4 @@
-"""Builds the CUDA library in-tree for sm_100a: kiln_b200/lib/libkiln_b200.so.
+"""Builds the CUDA library in-tree for sm_100a: kiln_b200/lib/libkiln_b200.so, and what binds it: the C++ op-set shim and the torch binding.
 
     python -m kiln_b200.build [--force] [--verbose]
 
@@ -7,6 +7,7 @@ one driver entry point it needs (cuTensorMapEncodeTiled) at run time, so it load
 without a driver; every launch entry point then fails with KB_ERR_DEVICE.
 """
 import os
+import shutil
 import subprocess
 import sys
 
@@ -15,6 +16,7 @@ CSRC = os.path.join(PKG, "csrc")
 LIB_DIR = os.path.join(PKG, "lib")
 LIB = os.path.join(LIB_DIR, "libkiln_b200.so")
 HOST_LIB = os.path.join(LIB_DIR, "libkiln_engine_ops.so")
+BINDING = os.path.join(LIB_DIR, "_kiln_torch.so")
 INCLUDE = os.path.join(os.path.dirname(PKG), "include")
 
 NVCC_FLAGS = ["-O3", "-std=c++17", "-gencode", "arch=compute_100a,code=sm_100a", "-lineinfo",
@@ -41,6 +43,8 @@ def build(force=False, verbose=False, defines=(), out=None):
     out = out or LIB
     os.makedirs(os.path.dirname(out), exist_ok=True)
     deps = _sources([CSRC, INCLUDE], (".cu", ".cuh", ".h"))
+    if out == LIB:
+        build_binding()                            # ops.py binds some of the library's calls with it
     if not force and not _stale(out, deps):
         return out
     cmd = ["nvcc"] + NVCC_FLAGS + (["-Xptxas", "-v"] if verbose else []) + ["-D" + d for d in defines] + \
@@ -67,7 +71,29 @@ def build_host(force=False):
     return HOST_LIB
 
 
+def build_binding(force=False):
+    """Compile the binding of the 4-bit, rotary and dropout calls for torch tensors (a CPython module, no device code); returns its path."""
+    import importlib.util
+    import sysconfig
+    src = os.path.join(PKG, "host", "torch_binding.cpp")
+    if not force and not _stale(BINDING, [src, os.path.join(INCLUDE, "kiln_b200.h")]):
+        return BINDING
+    os.makedirs(LIB_DIR, exist_ok=True)
+    torch_dir = os.path.dirname(importlib.util.find_spec("torch").origin)
+    inc = os.path.join(torch_dir, "include")
+    cuda = os.path.dirname(os.path.dirname(shutil.which("nvcc") or "/usr/local/cuda/bin/nvcc"))
+    cmd = ["g++", "-O2", "-std=c++17", "-fPIC", "-shared", "-w", "-I" + inc, "-I" + os.path.join(inc, "torch", "csrc", "api", "include"),
+           "-I" + os.path.join(cuda, "include"), "-I" + sysconfig.get_paths()["include"], "-o", BINDING + ".new", src, "-L" + os.path.join(torch_dir, "lib"),
+           "-lc10", "-lc10_cuda", "-ltorch_cpu", "-ltorch_python"]
+    r = subprocess.run(cmd, capture_output=True, text=True)
+    if r.returncode != 0:
+        raise RuntimeError("torch binding build failed:\n" + r.stderr[-6000:])
+    os.replace(BINDING + ".new", BINDING)
+    return BINDING
+
+
 if __name__ == "__main__":
     print(build(force="--force" in sys.argv, verbose="--verbose" in sys.argv))
     if os.path.exists(os.path.join(PKG, "host", "gpu_ops.cpp")):
         print(build_host(force="--force" in sys.argv))
+    print(build_binding(force="--force" in sys.argv))

@@ -7,7 +7,6 @@ op set (reference: engine/src/gpu.h:149-156): row-major [rows, ld] activations, 
 """
 import ctypes
 import os
-import struct
 
 KB_F16, KB_BF16, KB_F32 = 0, 1, 2
 
@@ -342,161 +341,72 @@ def cross_kv(k16, v16, ctx, Wk, Wv, kn_w=None, eps=1e-6, workspace=None):
     return k16, v16
 
 
-def _here(stream_device, *tensors):
-    """The calls below run on the current device: a tensor that lies elsewhere is refused before its address gets there."""
-    for t in tensors:
-        if t is not None and t.get_device() != stream_device:
-            raise ValueError(f"tensor on {t.device}, but the current device is cuda:{stream_device}")
+# The calls below go through a compiled binding (host/torch_binding.cpp): they are short enough for what Python and ctypes do per call to be most of their
+# time. A projection of one token, quantisation and product, 22 us of host time so, 9.5 us through it.
+_BINDING_PATH = os.path.join(_PKG, "lib", "_kiln_torch.so")
+_binding = None
 
 
-def _stream_device():
-    """(raw handle of the current stream, current device)"""
-    handle = _stream()
-    return handle, _cur_device()
+def _b():
+    """The compiled binding over the library that lib() has loaded; fails loudly when it has not been built."""
+    global _binding
+    if _binding is None:
+        import importlib.machinery
+        import importlib.util
+        import torch                                   # noqa: F401  (its libraries, which the module links against)
+        L = lib()
+        if not os.path.exists(_BINDING_PATH):
+            raise FileNotFoundError(f"{_BINDING_PATH} is missing: run `python -m kiln_b200.build`")
+        loader = importlib.machinery.ExtensionFileLoader("_kiln_torch", _BINDING_PATH)
+        m = importlib.util.module_from_spec(importlib.util.spec_from_loader("_kiln_torch", loader))
+        loader.exec_module(m)
+        m.bind(KilnError, *[ctypes.cast(f, ctypes.c_void_p).value for f in (L.kb_quant4, L.kb_dequant4, L.kb_linear4, L.kb_linear4_dx, L.kb_rope, L.kb_dropout)])
+        _binding = m
+    return _binding
+
+
+def __getattr__(name):
+    if name == "Quant4":                               # the type of a 4-bit matrix lives in the binding
+        globals()["Quant4"] = _b().Quant4
+        return Quant4                                  # noqa: F821
+    raise AttributeError(f"module {__name__!r} has no attribute {name!r}")
 
 
 def padded_empty(rows, cols, dtype, device):
     """An uninitialised [rows, cols] matrix whose rows start on 16 bytes, as the products' outputs have to."""
-    import torch
-    step = 16 // dtype.itemsize
-    if cols % step == 0:
-        return torch.empty((rows, cols), dtype=dtype, device=device)
-    return torch.empty((rows, (cols // step + 1) * step), dtype=dtype, device=device)[:, :cols]
+    return (_binding or _b()).padded_empty(rows, cols, dtype, device)
 
 
 MX4, NV4 = 0, 1
 EPI_GELU4 = 5
 
 
-MAX_Q4_COLS = 1 << 24
-
-
-def _q4_bytes(rows, cols, fmt):
-    """(bytes of a row of codes, bytes of the scales): kb_quant4_row_bytes and kb_quant4_scale_bytes without a call"""
-    if rows < 0 or not 0 < cols <= MAX_Q4_COLS or fmt not in (MX4, NV4):
-        raise ValueError(f"no 4-bit matrix of {rows} x {cols}, format {fmt}")
-    return (cols + 31) // 32 * 16, (rows + 127) // 128 * ((cols + 63) // 64 if fmt else (cols + 127) // 128) * 512
-
-
-class Quant4:
-    """A matrix [rows, cols] of 4-bit numbers in blocks (kb_quant4): codes uint8 [rows, >= 16 ceil(cols / 32)], scales uint8, fmt MX4 or NV4, 2^exp for all of it."""
-    __slots__ = ("rows", "cols", "fmt", "exp", "device", "ld", "codes_ptr", "scales_ptr", "_codes", "_scales", "_both")
-
-    def __init__(self, codes, scales, rows, cols, fmt, exp=0):
-        row_bytes, scale_bytes = _q4_bytes(rows, cols, fmt)
-        have, st = codes.shape, codes.stride()
-        if codes.element_size() != 1 or scales.element_size() != 1 or len(have) != 2 or not scales.is_contiguous():
-            raise ValueError("codes are a [rows, bytes] matrix of bytes, scales contiguous bytes")
-        if have[0] < rows or have[1] < row_bytes or st[1] != 1:
-            raise ValueError(f"codes {tuple(have)} do not hold {rows} rows of {cols} columns")
-        if scales.numel() < scale_bytes:
-            raise ValueError(f"scales of {scales.numel()} bytes do not hold {rows} rows of {cols} columns")
-        self.device = codes.get_device()
-        if scales.get_device() != self.device:
-            raise ValueError("codes and scales lie on one device")
-        self.rows, self.cols, self.fmt, self.exp, self._codes, self._scales, self._both = rows, cols, fmt, exp, codes, scales, None
-        self.ld, self.codes_ptr, self.scales_ptr = st[0], codes.data_ptr(), scales.data_ptr()
-
-    # what quant4_empty makes is one buffer: the two views cost more than a launch and are made when they are asked for
-    @property
-    def codes(self):
-        if self._codes is None:
-            self._codes = self._both[:self.rows * self.ld].view(self.rows, self.ld)
-        return self._codes
-
-    @property
-    def scales(self):
-        if self._scales is None:
-            self._scales = self._both[self.rows * self.ld:]
-        return self._scales
-
-
 def quant4_empty(rows, cols, fmt, device, exp=0):
-    """Uninitialised buffers of a 4-bit matrix."""
-    import torch
-    row_bytes, scale_bytes = _q4_bytes(rows, cols, fmt)
-    q = Quant4.__new__(Quant4)                     # what is made here needs no checks
-    q._both = both = torch.empty((rows * row_bytes + scale_bytes,), dtype=torch.uint8, device=device)
-    q._codes = q._scales = None
-    q.rows, q.cols, q.fmt, q.exp, q.ld, q.device = rows, cols, fmt, exp, row_bytes, both.get_device()
-    q.codes_ptr = p = both.data_ptr()              # a row of codes is a multiple of 16 bytes
-    q.scales_ptr = p + rows * row_bytes
-    return q
-
-
-def _elsewhere(device, dev):
-    raise ValueError(f"4-bit matrix on device {device}, but the current device is cuda:{dev}")
+    """A Quant4 with uninitialised buffers."""
+    return (_binding or _b()).quant4_empty(rows, cols, fmt, device, exp)
 
 
 def quant4(x, fmt, exp=0, out=None):
-    """x [rows, cols] fp16 / bf16 / fp32 as 4-bit numbers in blocks along the rows (see kb_quant4 for the two formats and exp)."""
-    rows, cols = x.shape
-    if out is None:
-        out = quant4_empty(rows, cols, fmt, x.device, exp)
-    elif (out.rows, out.cols, out.fmt, out.exp) != (rows, cols, fmt, exp):
-        raise ValueError("out was made for another matrix")
-    stream, dev = _stream_device()
-    if x.get_device() != dev or out.device != dev:
-        _elsewhere(x.device, dev)
-    _check(lib().kb_quant4(out.codes_ptr, out.ld, out.scales_ptr, x.data_ptr(), _ld(x), _dt(x), rows, cols, fmt, exp, stream), "kb_quant4")
-    return out
+    """x [rows, cols] fp16 / bf16 / fp32 as a Quant4: 4-bit numbers in blocks along the rows (see kb_quant4 for the two formats and exp)."""
+    return (_binding or _b()).quant4(x, fmt, exp, out)
 
 
 def dequant4(y, q, transpose=False):
     """y [rows, cols], or with transpose [cols, rows], fp16 / bf16 / fp32 = the values that q stands for."""
-    if y.shape != ((q.cols, q.rows) if transpose else (q.rows, q.cols)):
-        raise ValueError(f"y {tuple(y.shape)} for a matrix of {q.rows} x {q.cols}")
-    stream, dev = _stream_device()
-    if y.get_device() != dev or q.device != dev:
-        _elsewhere(y.device, dev)
-    _check(lib().kb_dequant4(y.data_ptr(), _ld(y), _dt(y), q.codes_ptr, q.ld, q.scales_ptr, q.rows, q.cols, q.fmt, q.exp, transpose, stream), "kb_dequant4")
-    return y
+    return (_binding or _b()).dequant4(y, q, transpose)
 
 
 def linear4(C, A, W, epi, gate=None, alpha=1.0):
     """C = epilogue(alpha * A @ W.T) for 4-bit A [M, K] and W [N, K] (Quant4 of one format, their powers of two included): EPI_F32 / EPI_RESID into
     an fp32 C, EPI_F16 / EPI_GELU16 into an fp16 C, EPI_GELU4 into a Quant4 C of the same format with exp 0."""
-    M, N, K = A.rows, W.rows, A.cols
-    if W.cols != K or W.fmt != A.fmt:
-        raise ValueError("A and W have to agree in columns and format")
-    if epi == EPI_GELU4:
-        if not isinstance(C, Quant4) or (C.rows, C.cols, C.fmt, C.exp) != (M, N, A.fmt, 0):
-            raise ValueError("EPI_GELU4 goes into a Quant4 [M, N] of the operands' format with exp 0")
-        out, ldc, scales, there = C.codes_ptr, C.ld, C.scales_ptr, C.device
-    else:
-        if isinstance(C, Quant4) or C.shape != (M, N) or _dt(C) != (KB_F32 if epi in (EPI_F32, EPI_RESID) else KB_F16):
-            raise ValueError("C is [M, N] of its epilogue's type")
-        out, ldc, scales, there = C.data_ptr(), _ld(C), None, C.get_device()
-    if gate is not None:
-        if _dt(gate) != KB_F32 or gate.numel() < N or not gate.is_contiguous() or gate.get_device() != there:
-            raise ValueError("gate is fp32 [N], where C is")
-        gate = gate.data_ptr()
-    stream, dev = _stream_device()
-    if not there == A.device == W.device == dev:
-        _elsewhere((there, A.device, W.device), dev)
-    _check(lib().kb_linear4(out, ldc, scales, A.codes_ptr, A.ld, A.scales_ptr, W.codes_ptr, W.ld, W.scales_ptr, M, N, K, A.fmt, epi,
-                            alpha * 2.0 ** (A.exp + W.exp), gate, stream), "kb_linear4")
-    return C
+    return (_binding or _b()).linear4(C, A, W, epi, gate, alpha)
 
 
 def linear4_dx(dx, dy, W, workspace=None):
-    """dx [M, K] (fp16 or fp32) = dy [M, N] @ W for a 4-bit W [N, K]: the gradient of linear4's input. dy fp16."""
-    M, N = dy.shape
-    if N != W.rows or dx.shape != (M, W.cols) or _dt(dy) != KB_F16:
-        raise ValueError("dy is fp16 [M, N], dx [M, K] for a weight of [N, K]")
-    if workspace is None:
-        import torch
-        workspace = torch.empty((2 * N * W.cols,), dtype=torch.uint8, device=dy.device)      # kb_linear4_dx_workspace_bytes
-    stream, dev = _stream_device()
-    if not W.device == dy.get_device() == dx.get_device() == workspace.get_device() == dev:
-        _elsewhere((W.device, dy.device, dx.device, workspace.device), dev)
-    wp, wb = _ws(workspace)
-    _check(lib().kb_linear4_dx(dx.data_ptr(), _ld(dx), _dt(dx), dy.data_ptr(), _ld(dy), W.codes_ptr, W.ld, W.scales_ptr, M, N, W.cols, W.fmt, W.exp, wp, wb, stream),
-           "kb_linear4_dx")
-    return dx
+    """dx [M, K] (fp16 or fp32) = dy [M, N] @ W for a 4-bit W [N, K]: the gradient of linear4's input. dy fp16. workspace: 2 N K bytes, made here if None."""
+    return (_binding or _b()).linear4_dx(dx, dy, W, workspace)
 
 
-_F64 = _I32 = _INT32 = None    # types, filled when first needed
 ROPE_HALF, ROPE_INTERLEAVED = 0, 1
 ROPE_PLAIN, ROPE_LINEAR, ROPE_BASE, ROPE_PARTS = 0, 1, 2, 3
 
@@ -510,55 +420,15 @@ def rope_freqs(rot_dim, base=10000.0, scaling=ROPE_PLAIN, factor=1.0, trained_le
     return freq
 
 
-_PTRS = [struct.Struct("Q" * n) for n in range(5)]     # host arrays of pointers and sizes as bytes: a quarter of a ctypes array's time
-_INTS = [struct.Struct("i" * n) for n in range(5)]
-
-
 def rope(outs, xs, heads, head_dim, pos, freq, axis=None, layout=ROPE_HALF, amplitude=1.0, inverse=False):
     """Rotary positions of up to four tensors xs[k] [rows, heads[k] * head_dim] of one type in one launch; outs may be xs. pos: int32 [pos_rows, axes] on the
     device (row r takes pos[r % pos_rows]); freq (float64) and axis (int32 or None), one entry per pair, numpy arrays on the host. inverse = the gradient."""
-    global _F64, _I32, _INT32
-    if _F64 is None:
-        import numpy as np
-        import torch
-        _F64, _I32, _INT32 = np.dtype(np.float64), np.dtype(np.int32), torch.int32
-    n = len(xs)
-    if not 1 <= n <= 4 or len(outs) != n or len(heads) != n:
-        raise ValueError("one to four tensors, an output and a number of heads each")
-    rows, dt = xs[0].shape[0], xs[0].dtype
-    px, po, lx, lo = [], [], [], []
-    for o, x, h in zip(outs, xs, heads):
-        if x.shape[0] != rows or x.shape[1] < h * head_dim or o.shape[0] != rows or o.shape[1] < h * head_dim or o.dtype != dt or x.dtype != dt:
-            raise ValueError("tensors are [rows, heads * head_dim] of one type")
-        px.append(x.data_ptr())
-        po.append(o.data_ptr())
-        lx.append(_ld(x))
-        lo.append(_ld(o))
-    if pos.dtype != _INT32 or pos.dim() != 2 or (pos.shape[1] > 1 and pos.stride(1) != 1):
-        raise ValueError("pos is int32 [rows, axes]")
-    if freq.dtype != _F64 or freq.ndim != 1 or (axis is not None and (axis.dtype != _I32 or axis.shape != freq.shape)):
-        raise ValueError("freq is float64 and axis int32, one per pair")
-    stream, dev = _stream_device()
-    _here(dev, pos, *xs, *outs)
-    ptrs, ints = _PTRS[n].pack, _INTS[n].pack
-    _check(lib().kb_rope(n, ptrs(*po), ints(*lo), ptrs(*px), ints(*lx), ints(*heads), _dt(xs[0]), rows, head_dim, 2 * freq.size, layout, pos.data_ptr(),
-                         pos.shape[0], pos.stride(0), pos.shape[1], freq.tobytes(), None if axis is None else axis.tobytes(), amplitude, inverse, stream),
-           "kb_rope")
-    return outs
+    return (_binding or _b()).rope(outs, xs, heads, head_dim, pos, freq, axis, layout, amplitude, inverse) and outs
 
 
 def dropout(out, x, rng, p, resid=None):
     """out = dropout(x) (+ resid); rng: int64 [2] on the device, seed and offset. The gradient is dropout(dout) with the same rng (see kb_dropout)."""
-    rows, cols = x.shape
-    if out.shape != x.shape or (resid is not None and (resid.shape != x.shape or resid.dtype != out.dtype)):
-        raise ValueError("out, x and resid have one shape, out and resid one type")
-    if rng.element_size() != 8 or rng.is_floating_point() or rng.numel() != 2 or not rng.is_contiguous():
-        raise ValueError("rng is int64 [2]: seed and offset")
-    stream, dev = _stream_device()
-    _here(dev, out, x, rng, resid)
-    _check(lib().kb_dropout(out.data_ptr(), _ld(out), _dt(out), x.data_ptr(), _ld(x), _dt(x), _ptr(resid), 0 if resid is None else _ld(resid), rows, cols, p,
-                            rng.data_ptr(), stream), "kb_dropout")
-    return out
+    return (_binding or _b()).dropout(out, x, rng, p, resid)
 
 
 def check_status():

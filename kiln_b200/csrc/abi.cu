@@ -1020,7 +1020,7 @@ int launch_quant4(Quant4Params& p, int dtype, cudaStream_t stream) {
 template <int FMT, typename T>
 int launch_dequant4_t(Quant4Params& p, bool transpose, cudaStream_t stream) {
     if (transpose) {
-        const long long blocks = (((long long)p.rows + Q4_TILE - 1) / Q4_TILE) * ((p.cols + Q4_TILE - 1) / Q4_TILE);
+        const long long blocks = (((long long)p.rows + Q4_TILE_R - 1) / Q4_TILE_R) * ((p.cols + Q4_TILE_C - 1) / Q4_TILE_C);
         if (blocks > 0x7fffffffLL) return KB_ERR_SHAPE;
         return launch_dependent(dequant4_t_kernel<T, FMT>, dim3((unsigned)blocks), dim3(256), 0, stream, nullptr, p);
     }

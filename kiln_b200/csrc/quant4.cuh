@@ -280,36 +280,45 @@ dequant4_kernel(const Quant4Params p) {
     }
 }
 
-// The transpose [cols, ld_x], through shared memory in tiles of 64 x 64: a thread decodes eight columns of two rows side by side, which become
-// eight pairs along a row of the transpose. What the gradient of a projection's input multiplies with.
-constexpr int Q4_TILE = 64, Q4_TILE_LD = 72;      // elements of a tile row in shared memory: a row starts on 16 bytes, four banks further
+// The transpose [cols, ld_x], through shared memory in tiles of 128 rows x 64 columns: a thread decodes sixteen columns (one scale) of two rows side by side, which
+// become sixteen pairs along rows of the transpose. What the gradient of a projection's input multiplies with.
+constexpr int Q4_TILE_R = 128, Q4_TILE_C = 64, Q4_TILE_LD = Q4_TILE_R + 8;      // a tile row in shared memory starts on 16 bytes, four banks further
 template <typename T, int FMT>
 __global__ void __launch_bounds__(256)
 dequant4_t_kernel(const Quant4Params p) {
-    __shared__ __align__(16) T tile[Q4_TILE * Q4_TILE_LD];
+    __shared__ __align__(16) T tile[Q4_TILE_C * Q4_TILE_LD];
     pdl_launch();
     pdl_wait();
-    const int tiles_c = (p.cols + Q4_TILE - 1) / Q4_TILE;
-    const int r0 = (int)(blockIdx.x / (unsigned)tiles_c) * Q4_TILE, k0 = (int)(blockIdx.x % (unsigned)tiles_c) * Q4_TILE;
-    const int pair = threadIdx.x & 31, kg = threadIdx.x >> 5;
+    const int tiles_c = (p.cols + Q4_TILE_C - 1) / Q4_TILE_C;
+    const int r0 = (int)(blockIdx.x / (unsigned)tiles_c) * Q4_TILE_R, k0 = (int)(blockIdx.x % (unsigned)tiles_c) * Q4_TILE_C;
+    const int pair = threadIdx.x & 63, kg = threadIdx.x >> 6, c = k0 + 16 * kg;
     const float up = pow2f(p.exp);
-    Q4Raw q[2] = {{0u, 0u}, {0u, 0u}};
+    uint2 codes[2];
+    uint32_t scale[2];
 #pragma unroll
-    for (int i = 0; i < 2; i++)
-        if (r0 + 2 * pair + i < p.rows && k0 + 8 * kg < p.cols) q[i] = q4_load8<FMT>(p, r0 + 2 * pair + i, k0 + 8 * kg);
-    const Raw8<T> v0 = q4_values8<T, FMT>(q[0], up), v1 = q4_values8<T, FMT>(q[1], up);
+    for (int i = 0; i < 2; i++) {
+        const int r = r0 + 2 * pair + i, b = c / q4_block(FMT);
+        const bool in = r < p.rows && c < p.cols;
+        codes[i] = in ? *reinterpret_cast<const uint2*>(p.codes + (size_t)r * p.ld + (c >> 1)) : make_uint2(0u, 0u);
+        scale[i] = in ? p.scales[q4_scale_at(r, b >> 2, p.pieces) + (b & 3)] : 0u;
+    }
 #pragma unroll
-    for (int e = 0; e < 8; e++) {
-        struct alignas(2 * sizeof(T)) Two { T a, b; } two = {q4_pick(v0, e), q4_pick(v1, e)};
-        *reinterpret_cast<Two*>(&tile[(8 * kg + e) * Q4_TILE_LD + 2 * pair]) = two;
+    for (int h = 0; h < 2; h++) {
+        const Raw8<T> v0 = q4_values8<T, FMT>({h ? codes[0].y : codes[0].x, scale[0]}, up), v1 = q4_values8<T, FMT>({h ? codes[1].y : codes[1].x, scale[1]}, up);
+#pragma unroll
+        for (int e = 0; e < 8; e++) {
+            struct alignas(2 * sizeof(T)) Two { T a, b; } two = {reinterpret_cast<const T*>(v0.u)[e], reinterpret_cast<const T*>(v1.u)[e]};
+            *reinterpret_cast<Two*>(&tile[(16 * kg + 8 * h + e) * Q4_TILE_LD + 2 * pair]) = two;
+        }
     }
     __syncthreads();
-    constexpr int EACH = 16 / sizeof(T), ACROSS = Q4_TILE / EACH;      // elements of 16 bytes
-    for (int i = threadIdx.x; i < Q4_TILE * ACROSS; i += 256) {
-        const int k = i / ACROSS, c = (i % ACROSS) * EACH, left = p.rows - r0 - c;
+    constexpr int EACH = 16 / sizeof(T), ACROSS = Q4_TILE_R / EACH;    // elements of 16 bytes
+#pragma unroll
+    for (int i = threadIdx.x; i < Q4_TILE_C * ACROSS; i += 256) {
+        const int k = i / ACROSS, n = (i % ACROSS) * EACH, left = p.rows - r0 - n;
         if (k0 + k >= p.cols || left <= 0) continue;
-        T* const dst = static_cast<T*>(p.y) + (size_t)(k0 + k) * p.ld_x + r0 + c;
-        const uint4 v = *reinterpret_cast<const uint4*>(&tile[k * Q4_TILE_LD + c]);
+        T* const dst = static_cast<T*>(p.y) + (size_t)(k0 + k) * p.ld_x + r0 + n;
+        const uint4 v = *reinterpret_cast<const uint4*>(&tile[k * Q4_TILE_LD + n]);
         if (p.wide && left >= EACH) *reinterpret_cast<uint4*>(dst) = v;
         else
 #pragma unroll

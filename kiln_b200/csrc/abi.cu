@@ -1003,18 +1003,25 @@ inline size_t elem_size(int dtype) { return dtype == KB_F32 ? 4 : 2; }
 inline bool wide_rows(const void* p, int ld, int dtype) { return aligned16(p) && (ld * elem_size(dtype)) % 16 == 0; }
 
 // a warp per row and group of columns
+template <int COLS>
 dim3 quant4_grid(const Quant4Params& p) {
-    constexpr int COLS = Q4_SEGS * 256, WARPS = Q4_THREADS / 32;
-    static_assert(COLS == DEQ_COLS, "one grid for both directions");
+    constexpr int WARPS = Q4_THREADS / 32;
     static_assert(KB_MAX_Q4_COLS / COLS <= 65535, "grid");
     return dim3((unsigned)(((long long)p.rows + WARPS - 1) / WARPS), (unsigned)((p.cols + COLS - 1) / COLS));
 }
 
+template <typename T, int FMT>
+int launch_quant4_t(const Quant4Params& p, cudaStream_t stream) {
+    if constexpr (sizeof(T) == 2)
+        if ((long long)p.rows * p.cols >= Q4_LARGE) return launch_dependent(quant4_kernel<T, FMT, 4>, quant4_grid<1024>(p), dim3(Q4_THREADS), 0, stream, nullptr, p);
+    return launch_dependent(quant4_kernel<T, FMT, 2>, quant4_grid<512>(p), dim3(Q4_THREADS), 0, stream, nullptr, p);
+}
+
 template <int FMT>
-int launch_quant4(Quant4Params& p, int dtype, cudaStream_t stream) {
-    if (dtype == KB_F16) return launch_dependent(quant4_kernel<__half, FMT>, quant4_grid(p), dim3(Q4_THREADS), 0, stream, nullptr, p);
-    if (dtype == KB_BF16) return launch_dependent(quant4_kernel<__nv_bfloat16, FMT>, quant4_grid(p), dim3(Q4_THREADS), 0, stream, nullptr, p);
-    return launch_dependent(quant4_kernel<float, FMT>, quant4_grid(p), dim3(Q4_THREADS), 0, stream, nullptr, p);
+int launch_quant4(const Quant4Params& p, int dtype, cudaStream_t stream) {
+    if (dtype == KB_F16) return launch_quant4_t<__half, FMT>(p, stream);
+    if (dtype == KB_BF16) return launch_quant4_t<__nv_bfloat16, FMT>(p, stream);
+    return launch_quant4_t<float, FMT>(p, stream);
 }
 
 template <int FMT, typename T>
@@ -1024,7 +1031,7 @@ int launch_dequant4_t(Quant4Params& p, bool transpose, cudaStream_t stream) {
         if (blocks > 0x7fffffffLL) return KB_ERR_SHAPE;
         return launch_dependent(dequant4_t_kernel<T, FMT>, dim3((unsigned)blocks), dim3(256), 0, stream, nullptr, p);
     }
-    return launch_dependent(dequant4_kernel<T, FMT>, quant4_grid(p), dim3(Q4_THREADS), 0, stream, nullptr, p);
+    return launch_dependent(dequant4_kernel<T, FMT>, quant4_grid<deq_cols<T>()>(p), dim3(Q4_THREADS), 0, stream, nullptr, p);
 }
 
 template <int FMT>

@@ -153,25 +153,28 @@ struct Quant4Params {
     bool wide;
 };
 
-// A lane takes eight columns, so that a block is two (NV4) or four (MX4) lanes, which meet by shuffles; a warp 256 columns side by side, Q4_SEGS
-// times, its loads first. Bound by memory: 16-bit rows 2 bytes read and 0.56 written per element.
-constexpr int Q4_THREADS = 128, Q4_SEGS = 2;
+// A lane takes eight columns, so that a block is two (NV4) or four (MX4) lanes, which meet by shuffles; a warp 256 columns side by side, SEGS times, its loads
+// first. Bound by memory: 16-bit rows 2 bytes read and 0.56 written per element. SEGS is 4 for 16-bit matrices of at least Q4_LARGE elements, where thread blocks of
+// 2 come and go too fast, and else 2. Measured on B200, 2 -> 4, NV4 and MX4: 4096 x 8192 fp16 20.1 -> 18.3 us, 18.9 -> 15.7; 4096 x 2048 6.6 -> 6.7, 6.3 -> 6.0;
+// 1536 x 2048 3.2 -> 4.2, 3.2 -> 3.7. 8192 x 2048 fp32 13.4 and 13.1 us (5.7 TB/s) either way.
+constexpr int Q4_THREADS = 128;
+constexpr long long Q4_LARGE = 12LL << 20;
 
-template <typename T, int FMT>
-__global__ void __launch_bounds__(Q4_THREADS, 12)
+template <typename T, int FMT, int SEGS>
+__global__ void __launch_bounds__(Q4_THREADS, SEGS == 2 ? 12 : 10)
 quant4_kernel(const Quant4Params p) {
     pdl_launch();
     pdl_wait();
     const unsigned row = blockIdx.x * (Q4_THREADS / 32) + (threadIdx.x >> 5);
     if (row >= (unsigned)p.rows) return;
-    const int lane = threadIdx.x & 31, c0 = (int)blockIdx.y * (Q4_SEGS * 256) + lane * 8;
+    const int lane = threadIdx.x & 31, c0 = (int)blockIdx.y * (SEGS * 256) + lane * 8;
     const T* const src = static_cast<const T*>(p.x) + (size_t)row * p.ld_x;
     const float down = pow2f(-p.exp), up = pow2f(p.exp);
-    Raw8<T> raw[Q4_SEGS];
+    Raw8<T> raw[SEGS];
 #pragma unroll
-    for (int i = 0; i < Q4_SEGS; i++) raw[i] = load8_raw(src, c0 + i * 256, p.cols, p.wide);
+    for (int i = 0; i < SEGS; i++) raw[i] = load8_raw(src, c0 + i * 256, p.cols, p.wide);
 #pragma unroll
-    for (int i = 0; i < Q4_SEGS; i++) {
+    for (int i = 0; i < SEGS; i++) {
         const int c = c0 + i * 256;
         if (c - lane * 8 >= p.cols) break;                     // the whole warp is behind the last column (a piece never begins there)
         const F8 f = Io<T>::f8(raw[i]);
@@ -243,21 +246,22 @@ __device__ __forceinline__ T q4_pick(const Raw8<T>& r, int e) {
 }
 
 // A lane takes 16 bytes of output where rows start on 16 bytes (fp32: half of eight codes), so that every store of a warp is 512 bytes in a row; else a
-// column, DEQ_COLS / 32 times.
-constexpr int DEQ_COLS = 512;                   // columns of a warp
+// column at a time. Measured on B200, fp16, 512 columns of a warp -> 1024: 4096 x 8192 18.5 -> 15.8 us, 8192 x 2048 10.0 -> 8.6, 1536 x 2048 3.0 -> 3.0; fp32 the
+// other way: 1536 x 2048 4.6 -> 5.0, 8192 x 2048 14.2 -> 14.8.
+template <typename T> __host__ __device__ constexpr int deq_cols() { return sizeof(T) == 2 ? 1024 : 512; }   // columns of a warp
 template <typename T, int FMT>
 __global__ void __launch_bounds__(Q4_THREADS)
 dequant4_kernel(const Quant4Params p) {
-    constexpr int EACH = 16 / sizeof(T), N = DEQ_COLS / (32 * EACH);
+    constexpr int EACH = 16 / sizeof(T), COLS = deq_cols<T>(), N = COLS / (32 * EACH);
     pdl_launch();
     pdl_wait();
     const unsigned row = blockIdx.x * (Q4_THREADS / 32) + (threadIdx.x >> 5);
     if (row >= (unsigned)p.rows) return;
-    const int first = (int)blockIdx.y * DEQ_COLS, lane = threadIdx.x & 31;
+    const int first = (int)blockIdx.y * COLS, lane = threadIdx.x & 31;
     T* const dst = static_cast<T*>(p.y) + (size_t)row * p.ld_x;
     const float up = pow2f(p.exp);
     if (!p.wide) {
-        for (int c = first + lane; c < min(first + DEQ_COLS, p.cols); c += 32) dst[c] = q4_pick(q4_values8<T, FMT>(q4_load8<FMT>(p, (int)row, c & ~7), up), c & 7);
+        for (int c = first + lane; c < min(first + COLS, p.cols); c += 32) dst[c] = q4_pick(q4_values8<T, FMT>(q4_load8<FMT>(p, (int)row, c & ~7), up), c & 7);
         return;
     }
     Q4Raw q[N];

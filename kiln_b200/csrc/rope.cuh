@@ -7,7 +7,7 @@
 // only rounding is that of the fraction to 32 bits (2^-32 of a turn) and the sine's own.
 //
 // Bound by memory. The sines of a row serve all of its heads of all tensors: a thread block takes a row (several where they are short), fills shared memory
-// with one (cos, sin) per pair, and every thread keeps those of its eight elements while it goes from head to head, its loads in front.
+// with one (cos, sin) per pair while its first loads are under way, and every thread keeps those of its eight elements as it goes from head to head.
 #pragma once
 #include "quant4.cuh"   // to_f32, from_f32
 
@@ -59,17 +59,24 @@ rope_kernel(const __grid_constant__ RopeParams p) {
     const int stride = VEC ? un.slots : pairs;
     const unsigned row0 = blockIdx.x * (unsigned)p.block_rows;
     const int rows = (int)min((unsigned)p.block_rows, (unsigned)p.rows - row0);
-    for (int i = threadIdx.x; i < rows * pairs; i += ROPE_THREADS) {
-        const int r = i / pairs, f = i - r * pairs;
-        const int pos = p.pos[(size_t)((row0 + (unsigned)r) % (unsigned)p.pos_rows) * p.ld_pos + p.axis[f]];
-        const unsigned long long turn = (unsigned long long)(long long)pos * p.freq[f];
-        float sn, cn;
-        sincospif((float)(int)(turn >> 32) * 0x1p-31f, &sn, &cn);     // in half turns, [-1, 1)
-        // VEC: a unit's pairs apart, those of neighbouring units side by side, so that neighbouring lanes read neighbouring words
-        const int at = VEC ? (f % EACH) * un.turned + f / EACH : f;
-        cs[r * stride + at] = make_float2(cn * p.amplitude, (p.inverse ? -sn : sn) * p.amplitude);
-    }
-    __syncthreads();
+    // (cos, sin) of the block's rows; a thread keeps its pair, so that it fetches one frequency
+    auto fill = [&]() {
+        const int per = ROPE_THREADS / pairs, f = threadIdx.x % pairs;
+        int r = threadIdx.x / pairs;
+        if (r < per) {
+            const unsigned long long freq = p.freq[f];
+            const int axis = p.axis[f];
+            // VEC: a unit's pairs apart, those of neighbouring units side by side, so that neighbouring lanes read neighbouring words
+            float2* const at = cs + (VEC ? (f % EACH) * un.turned + f / EACH : f);
+            for (; r < rows; r += per) {
+                const int pos = p.pos[(size_t)((row0 + (unsigned)r) % (unsigned)p.pos_rows) * p.ld_pos + axis];
+                const unsigned long long turn = (unsigned long long)(long long)pos * freq;
+                float sn, cn;
+                sincospif((float)(int)(turn >> 32) * 0x1p-31f, &sn, &cn);     // in half turns, [-1, 1)
+                at[r * stride] = make_float2(cn * p.amplitude, (p.inverse ? -sn : sn) * p.amplitude);
+            }
+        }
+    };
     auto head = [&](unsigned row, int v, const T*& src, T*& dst) {
         const RopeTensor* t = &p.t[0];
 #pragma unroll
@@ -80,11 +87,12 @@ rope_kernel(const __grid_constant__ RopeParams p) {
     };
     if constexpr (VEC) {
         int r = 0, v, s, step;
+        bool busy;
         if (p.block_rows == 1) {
             step = ROPE_THREADS / un.per_head;
             v = threadIdx.x / un.per_head;
             s = threadIdx.x - v * un.per_head;
-            if (v >= step) return;
+            busy = v < step && v < p.heads;
         } else {                                       // every thread has one unit of one head of one row
             const int all = un.per_head * p.heads;
             r = threadIdx.x / all;
@@ -92,21 +100,15 @@ rope_kernel(const __grid_constant__ RopeParams p) {
             v = j / un.per_head;
             s = j - v * un.per_head;
             step = p.heads;
-            if (r >= rows) return;
+            busy = r < rows;
         }
         const unsigned row = row0 + (unsigned)r;
         const bool turns = s < un.turned;
-        float2 z[EACH];
-#pragma unroll
-        for (int e = 0; e < EACH; e++) {
-            const bool in = turns && (HALF || EACH * s + e < pairs);   // interleaved: the last unit that turns may hold pairs that do not
-            z[e] = in ? cs[r * stride + e * un.turned + s] : make_float2(1.f, 0.f);
-        }
         constexpr int U = sizeof(T) == 2 ? 4 : 2;      // heads whose loads are under way together
         const int ca = HALF && !turns ? p.rot + 8 * (s - un.turned) : 8 * s, cb = pairs + 8 * s;
-        for (; v < p.heads; v += U * step) {
-            Raw8<T> a[U], b[U];
-            T* dst[U];
+        Raw8<T> a[U], b[U];
+        T* dst[U];
+        auto load = [&]() {
 #pragma unroll
             for (int i = 0; i < U; i++) {
                 if (v + i * step >= p.heads) break;
@@ -115,6 +117,18 @@ rope_kernel(const __grid_constant__ RopeParams p) {
                 a[i] = Io<T>::raw8(src + ca);
                 if (HALF && turns) b[i] = Io<T>::raw8(src + cb);
             }
+        };
+        if (busy) load();                              // under the sines
+        fill();
+        __syncthreads();
+        if (!busy) return;
+        float2 z[EACH];
+#pragma unroll
+        for (int e = 0; e < EACH; e++) {
+            const bool in = turns && (HALF || EACH * s + e < pairs);   // interleaved: the last unit that turns may hold pairs that do not
+            z[e] = in ? cs[r * stride + e * un.turned + s] : make_float2(1.f, 0.f);
+        }
+        while (true) {
 #pragma unroll
             for (int i = 0; i < U; i++) {
                 if (v + i * step >= p.heads) break;
@@ -139,8 +153,13 @@ rope_kernel(const __grid_constant__ RopeParams p) {
                 }
                 Io<T>::st8(dst[i] + ca, x);
             }
+            v += U * step;
+            if (v >= p.heads) break;
+            load();
         }
     } else {
+        fill();
+        __syncthreads();
         const int lane = threadIdx.x & 31;
         for (int v = threadIdx.x >> 5; v < p.heads; v += ROPE_THREADS / 32) {
             const T* src;

@@ -1245,17 +1245,27 @@ int launch_rope_t(const RopeParams& p, bool half, bool vec, unsigned blocks, cud
     return launch_dependent(rope_kernel<T, false, false>, grid, block, 0, stream, nullptr, p);
 }
 
+template <typename InT, typename OutT, bool RESID>
+int launch_dropout_r(DeviceState* st, const DropoutParams& p, unsigned across, cudaStream_t stream) {
+    const long long block_rows = DROP_THREADS >> p.width_log2, down = ((long long)p.rows + block_rows - 1) / block_rows;
+    long long grid = down;
+    if (drop_one_round<InT, OutT>()) {                    // each thread block on its share of the rows (see the kernel)
+        const long long room = (long long)drop_blocks_per_sm<InT, OutT, RESID>() * st->sm_count / across;
+        grid = down <= room ? down : room > 1 ? room : 1;
+    }
+    return launch_dependent(dropout_kernel<InT, OutT, RESID>, dim3((unsigned)grid, across), dim3(DROP_THREADS), 0, stream, nullptr, p);
+}
+
 template <typename InT, typename OutT>
-int launch_dropout_t(const DropoutParams& p, dim3 grid, cudaStream_t stream) {
-    if (p.resid) return launch_dependent(dropout_kernel<InT, OutT, true>, grid, dim3(DROP_THREADS), 0, stream, nullptr, p);
-    return launch_dependent(dropout_kernel<InT, OutT, false>, grid, dim3(DROP_THREADS), 0, stream, nullptr, p);
+int launch_dropout_t(DeviceState* st, const DropoutParams& p, unsigned across, cudaStream_t stream) {
+    return p.resid ? launch_dropout_r<InT, OutT, true>(st, p, across, stream) : launch_dropout_r<InT, OutT, false>(st, p, across, stream);
 }
 
 template <typename InT>
-int launch_dropout(const DropoutParams& p, int out_dtype, dim3 grid, cudaStream_t stream) {
-    if (out_dtype == KB_F16) return launch_dropout_t<InT, __half>(p, grid, stream);
-    if (out_dtype == KB_BF16) return launch_dropout_t<InT, __nv_bfloat16>(p, grid, stream);
-    return launch_dropout_t<InT, float>(p, grid, stream);
+int launch_dropout(DeviceState* st, const DropoutParams& p, int out_dtype, unsigned across, cudaStream_t stream) {
+    if (out_dtype == KB_F16) return launch_dropout_t<InT, __half>(st, p, across, stream);
+    if (out_dtype == KB_BF16) return launch_dropout_t<InT, __nv_bfloat16>(st, p, across, stream);
+    return launch_dropout_t<InT, float>(st, p, across, stream);
 }
 
 }  // namespace
@@ -1327,16 +1337,12 @@ int kb_dropout(void* out, int ld_out, int out_dtype, const void* in, int ld_in, 
     // a row of a block's threads as wide as a row of the matrix, up to all of them
     const long long groups = ((long long)cols + 7) / 8;
     while (p.width_log2 < DROP_THREADS_LOG2 && 1LL << p.width_log2 < groups) ++p.width_log2;
-    const long long across = (groups + (1LL << p.width_log2) - 1) >> p.width_log2, block_rows = DROP_THREADS >> p.width_log2;
+    const long long across = (groups + (1LL << p.width_log2) - 1) >> p.width_log2;
     if (across > 65535) return KB_ERR_SHAPE;
-    // 16-bit: one round of thread blocks, each on its share of the rows; fp32: a thread block per rows that it holds at once (see the kernel)
-    const long long down = ((long long)rows + block_rows - 1) / block_rows, room = (long long)DROP_BLOCKS_PER_SM * st->sm_count / across;
-    const bool one_round = in_dtype != KB_F32 && out_dtype != KB_F32 && down > room;
-    const dim3 grid((unsigned)(one_round ? (room > 1 ? room : 1) : down), (unsigned)across);
     ProfScope ps(st, KB_PROF_LINEAR, stream);
-    if (in_dtype == KB_F16) return launch_dropout<__half>(p, out_dtype, grid, stream);
-    if (in_dtype == KB_BF16) return launch_dropout<__nv_bfloat16>(p, out_dtype, grid, stream);
-    return launch_dropout<float>(p, out_dtype, grid, stream);
+    if (in_dtype == KB_F16) return launch_dropout<__half>(st, p, out_dtype, (unsigned)across, stream);
+    if (in_dtype == KB_BF16) return launch_dropout<__nv_bfloat16>(st, p, out_dtype, (unsigned)across, stream);
+    return launch_dropout<float>(st, p, out_dtype, (unsigned)across, stream);
 }
 
 int kb_lora_pack(void* dst_f16, int ld, int col0, const void* src_bf16, int rows, int cols, float scale, void* stream) {

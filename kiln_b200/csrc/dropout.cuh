@@ -9,13 +9,24 @@
 
 namespace kb {
 
-__device__ __forceinline__ uint4 philox4x32(uint4 c, uint32_t k0, uint32_t k1) {
+// the keys of the ten rounds
+struct PhiloxKeys {
+    uint32_t a[10], b[10];
+    __device__ __forceinline__ explicit PhiloxKeys(unsigned long long seed) {
+#pragma unroll
+        for (int i = 0; i < 10; i++) { a[i] = (uint32_t)seed + i * 0x9E3779B9u; b[i] = (uint32_t)(seed >> 32) + i * 0xBB67AE85u; }
+    }
+    // in registers from here on, not summed up again for every counter: a sixth of the instructions
+    __device__ __forceinline__ void keep() {
+#pragma unroll
+        for (int i = 0; i < 10; i++) asm volatile("" : "+r"(a[i]), "+r"(b[i]));
+    }
+};
+__device__ __forceinline__ uint4 philox4x32(uint4 c, const PhiloxKeys& k) {
 #pragma unroll
     for (int i = 0; i < 10; i++) {
         const uint64_t p0 = (uint64_t)0xD2511F53u * c.x, p1 = (uint64_t)0xCD9E8D57u * c.z;
-        c = make_uint4((uint32_t)(p1 >> 32) ^ c.y ^ k0, (uint32_t)p1, (uint32_t)(p0 >> 32) ^ c.w ^ k1, (uint32_t)p0);
-        k0 += 0x9E3779B9u;
-        k1 += 0xBB67AE85u;
+        c = make_uint4((uint32_t)(p1 >> 32) ^ c.y ^ k.a[i], (uint32_t)p1, (uint32_t)(p0 >> 32) ^ c.w ^ k.b[i], (uint32_t)p0);
     }
     return c;
 }
@@ -35,10 +46,14 @@ struct DropoutParams {
 // A thread keeps its eight columns and goes down the rows, the next row's load under the ten rounds of this one's. Of 16-bit numbers the integer work bounds
 // it, and one round of thread blocks is best; of fp32 numbers the memory, and many short thread blocks keep more loads under way. Measured on B200, 4096 x 8192,
 // a thread block per row -> one round: bf16 34.9 -> 31.7 us, with a residual 45.1 -> 36.3; fp32 41.5 -> 57.8 (so not taken there).
-constexpr int DROP_THREADS_LOG2 = 8, DROP_THREADS = 1 << DROP_THREADS_LOG2, DROP_BLOCKS_PER_SM = 6;
+constexpr int DROP_THREADS_LOG2 = 8, DROP_THREADS = 1 << DROP_THREADS_LOG2;
+template <typename InT, typename OutT> __host__ __device__ constexpr bool drop_one_round() { return sizeof(InT) == 2 && sizeof(OutT) == 2; }
+template <typename InT, typename OutT, bool RESID> __host__ __device__ constexpr int drop_blocks_per_sm() {   // as many as hold without spills
+    return drop_one_round<InT, OutT>() ? (RESID ? 4 : 5) : (RESID ? 4 : 6);
+}
 
 template <typename InT, typename OutT, bool RESID>
-__global__ void __launch_bounds__(DROP_THREADS, DROP_BLOCKS_PER_SM)
+__global__ void __launch_bounds__(DROP_THREADS, drop_blocks_per_sm<InT, OutT, RESID>())
 dropout_kernel(const DropoutParams p) {
     pdl_launch();
     pdl_wait();
@@ -55,6 +70,8 @@ dropout_kernel(const DropoutParams p) {
     if (RESID) add = load8_raw(res, c, p.cols, p.wide);
     const unsigned long long seed = p.rng[0], offset = p.rng[1];
     const uint32_t t = p.t << 16;
+    PhiloxKeys keys(seed);
+    if (drop_one_round<InT, OutT>()) keys.keep();
     while (true) {
         const F8 v = Io<InT>::f8(in);
         F8 out;
@@ -66,7 +83,7 @@ dropout_kernel(const DropoutParams p) {
             in = load8_raw(x, c, p.cols, p.wide);
             if (RESID) { res += dr; add = load8_raw(res, c, p.cols, p.wide); }
         }
-        const uint4 w = philox4x32(make_uint4((uint32_t)g, row, (uint32_t)offset, (uint32_t)(offset >> 32)), (uint32_t)seed, (uint32_t)(seed >> 32));
+        const uint4 w = philox4x32(make_uint4((uint32_t)g, row, (uint32_t)offset, (uint32_t)(offset >> 32)), keys);
         const uint32_t words[4] = {w.x, w.y, w.z, w.w};
 #pragma unroll
         for (int e = 0; e < 8; e++) {

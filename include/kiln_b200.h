@@ -291,9 +291,11 @@ int kb_cross_kv(void* k16, void* v16, int ld_out, const void* ctx, int ld_ctx, i
  * elements per byte, the even column in the low half, zeros up to a multiple of 32 columns. scales: kb_quant4_scale_bytes(rows, cols, fmt) bytes, in pieces of
  * 512 for 128 rows x 4 blocks: row r, block b at ((r / 128) P + b / 4) 512 + (r % 32) 16 + (r / 32 % 4) 4 + b % 4, P = ceil(blocks / 4); zeros for the blocks
  * behind the last one of a row, nothing is written for rows behind the last. Rows from a multiple of 128 on are a matrix of their own at the
- * same ld_codes (scales 512 P bytes per 128 rows further). Both buffers 16-byte aligned. cols up to KB_MAX_Q4_COLS. */
+ * same ld_codes (scales 512 P bytes per 128 rows further). Both buffers 16-byte aligned. cols up to KB_MAX_Q4_COLS,
+ * rows up to KB_MAX_Q4_ROWS. */
 enum { KB_MX4 = 0, KB_NV4 = 1 };
 #define KB_MAX_Q4_COLS (1 << 24)
+#define KB_MAX_Q4_ROWS (1 << 30)
 int kb_quant4_row_bytes(int cols);                              /* 0: cols out of range */
 size_t kb_quant4_scale_bytes(int rows, int cols, int fmt);      /* 0: bad argument */
 
@@ -308,7 +310,7 @@ int kb_dequant4(void* y, int ld_y, int out_dtype, const void* codes, int ld_code
  * 2^(exp_A + exp_W) (1 for KB_MX4). Epilogues KB_EPI_F32, KB_EPI_F16, KB_EPI_GELU16, KB_EPI_RESID (C += gate[c] * alpha * acc, gate NULL = 1) as there, and
  *   KB_EPI_GELU4   C = gelu_erf(alpha * acc) in 4 bits of the same format (exp 0): C its codes, ldc their row bytes, C_scales its scales, which no other
  *                  epilogue takes. What the next kb_linear4 reads: the hidden activations of an MLP never exist in 16 bits.
- * M, N, K free (K up to KB_MAX_Q4_COLS). C 16-byte aligned, ldc a multiple of 8 (fp16) / 4 (fp32) / 16 (bytes of codes). Repeats are bit-identical. */
+ * M, N, K free (N and K up to KB_MAX_Q4_COLS). C 16-byte aligned, ldc a multiple of 8 (fp16) / 4 (fp32) / 16 (bytes of codes). Repeats are bit-identical. */
 enum { KB_EPI_GELU4 = 5 };
 int kb_linear4(void* C, int ldc, void* C_scales, const void* A, int lda, const void* A_scales, const void* W, int ldw, const void* W_scales, int M, int N,
                int K, int fmt, int epi, float alpha, const float* gate, void* stream);

@@ -1107,14 +1107,14 @@ extern "C" {
 int kb_quant4_row_bytes(int cols) { return cols > 0 && cols <= KB_MAX_Q4_COLS ? q4_row_bytes(cols) : 0; }
 
 size_t kb_quant4_scale_bytes(int rows, int cols, int fmt) {
-    if (rows <= 0 || cols <= 0 || cols > KB_MAX_Q4_COLS || (fmt != KB_MX4 && fmt != KB_NV4)) return 0;
+    if (rows <= 0 || rows > KB_MAX_Q4_ROWS || cols <= 0 || cols > KB_MAX_Q4_COLS || (fmt != KB_MX4 && fmt != KB_NV4)) return 0;
     return (((size_t)rows + 127) / 128) * q4_pieces(cols, fmt) * 512;
 }
 
 int kb_quant4(void* codes, int ld_codes, void* scales, const void* x, int ld_x, int dtype, int rows, int cols, int fmt, int exp, void* stream_) {
     cudaStream_t stream = static_cast<cudaStream_t>(stream_);
     if (!x || rows < 0 || cols <= 0 || !valid_in_dtype(dtype) || !valid_q4(fmt, exp)) return KB_ERR_ARG;
-    if (cols > KB_MAX_Q4_COLS || ld_x < cols) return KB_ERR_SHAPE;
+    if (cols > KB_MAX_Q4_COLS || rows > KB_MAX_Q4_ROWS || ld_x < cols) return KB_ERR_SHAPE;
     if (reinterpret_cast<uintptr_t>(x) % elem_size(dtype)) return KB_ERR_ALIGN;
     int rc;
     if ((rc = check_q4(codes, ld_codes, scales, cols))) return rc;
@@ -1133,7 +1133,7 @@ int kb_dequant4(void* y, int ld_y, int out_dtype, const void* codes, int ld_code
                 int transpose, void* stream_) {
     cudaStream_t stream = static_cast<cudaStream_t>(stream_);
     if (!y || rows < 0 || cols <= 0 || !valid_in_dtype(out_dtype) || !valid_q4(fmt, exp)) return KB_ERR_ARG;
-    if (cols > KB_MAX_Q4_COLS || ld_y < (transpose ? rows : cols)) return KB_ERR_SHAPE;
+    if (cols > KB_MAX_Q4_COLS || rows > KB_MAX_Q4_ROWS || ld_y < (transpose ? rows : cols)) return KB_ERR_SHAPE;
     if (reinterpret_cast<uintptr_t>(y) % elem_size(out_dtype)) return KB_ERR_ALIGN;
     int rc;
     if ((rc = check_q4(codes, ld_codes, scales, cols))) return rc;
@@ -1155,7 +1155,7 @@ int kb_linear4(void* C, int ldc, void* C_scales, const void* A, int lda, const v
     const bool out4 = epi == KB_EPI_GELU4, out32 = epi == KB_EPI_F32 || epi == KB_EPI_RESID;
     if (!out4 && !out32 && epi != KB_EPI_F16 && epi != KB_EPI_GELU16) return KB_ERR_ARG;
     if ((gate && epi != KB_EPI_RESID) || (C_scales && !out4)) return KB_ERR_ARG;
-    if (K > KB_MAX_Q4_COLS || N > KB_MAX_Q4_COLS) return KB_ERR_SHAPE;
+    if (K > KB_MAX_Q4_COLS || N > KB_MAX_Q4_COLS || M > KB_MAX_Q4_ROWS) return KB_ERR_SHAPE;
     int rc;
     if ((rc = check_q4(A, lda, A_scales, K)) || (rc = check_q4(W, ldw, W_scales, K))) return rc;
     if (out4) {
@@ -1193,7 +1193,7 @@ int kb_linear4_dx(void* dx, int ld_dx, int out_dtype, const void* dy_f16, int ld
     cudaStream_t stream = static_cast<cudaStream_t>(stream_);
     if (!dx || !dy_f16 || M < 0 || N <= 0 || K <= 0 || !valid_q4(fmt, exp) || (out_dtype != KB_F16 && out_dtype != KB_F32)) return KB_ERR_ARG;
     if (!aligned16(dx) || !aligned16(dy_f16) || (ld_dy & 7) || (ld_dx & (out_dtype == KB_F32 ? 3 : 7))) return KB_ERR_ALIGN;
-    if ((N % GB_K) || (K % 8) || K > KB_MAX_Q4_COLS || ld_dy < N || ld_dx < K) return KB_ERR_SHAPE;
+    if ((N % GB_K) || (K % 8) || K > KB_MAX_Q4_COLS || N > KB_MAX_Q4_ROWS || M > KB_MAX_Q4_ROWS || ld_dy < N || ld_dx < K) return KB_ERR_SHAPE;
     int rc;
     if ((rc = check_q4(W, ldw, W_scales, K))) return rc;
     if (M == 0) return KB_OK;

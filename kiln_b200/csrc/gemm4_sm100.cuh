@@ -10,10 +10,11 @@
 // scales of its rows and of ALL columns of the tile, and keeps its half of the accumulator. Two accumulators of 256 columns fill TMEM and leave no
 // room for scales, so they overlap: the first lies in columns [0, 256), the second in [128, 384), the scales behind them. The epilogue drains the 128
 // columns that both own first, and then the next tile's products begin; until then the tensor pipe waits, about 1.5 us per tile. (Pairs on 192 columns, which
-// have two whole accumulators beside the scales, measured slower nearly everywhere: N 8192, K 2048, M 4096 37.3 us against 36.0, K 8192, N 2048 32.6 against 28.6.)
+// have two whole accumulators beside the scales, wait for their loads instead: N 8192, K 2048, M 4096 37.3 us against 36.0, K 8192, N 2048 32.6 against 28.6.)
 //
-// What bounds it: a k step is 38 KB per CTA and comes from L2 at 64 bytes per clock and SM, 608 clocks, against 512 that the products of a 256 x 256 tile
-// take; measured 595. At 4 bits a larger tile, not a faster pipe, is what would help. 8192^3 199 us (5.5 PFLOP/s), M 4096, N 2048, K 8192 28.6 us (4.8).
+// What bounds it: a step of a pair takes the products' 512 clocks (490-510 from one to the next by the clock counter), so a long k range runs at the pipe's rate
+// for the clock that the power cap leaves: 8192^3 back to back 229 us at 1.36 GHz and 990 W (4.8 PFLOP/s; 199 us, 5.5, before the clock falls), M 4096, N 2048,
+// K 8192 28.6 us. Short ranges add the waits between tiles: M 4096, N 8192, K 2048 35.5 us, of which the products take 24 at 1.65 GHz.
 #pragma once
 #include "gemm_sm100.cuh"   // gelu, elect_one, pack16
 #include "quant4.cuh"

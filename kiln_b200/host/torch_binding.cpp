@@ -134,7 +134,7 @@ int64_t scale_bytes(int rows, int cols, int fmt) {
     return ((int64_t)rows + 127) / 128 * ((cols + piece - 1) / piece) * 512;
 }
 void check_size(int rows, int cols, int fmt) {
-    if (rows < 0 || cols <= 0 || cols > KB_MAX_Q4_COLS || (fmt != KB_MX4 && fmt != KB_NV4)) refuse("no 4-bit matrix of %d x %d, format %d", rows, cols, fmt);
+    if (rows < 0 || rows > KB_MAX_Q4_ROWS || cols <= 0 || cols > KB_MAX_Q4_COLS || (fmt != KB_MX4 && fmt != KB_NV4)) refuse("no 4-bit matrix of %d x %d, format %d", rows, cols, fmt);
 }
 
 Quant4* new_quant4() {

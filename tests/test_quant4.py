@@ -123,6 +123,21 @@ def test_quantise(built_lib, fmt, dtype, rows, cols):
 
 @gpu
 @pytest.mark.parametrize("fmt", FMTS)
+@pytest.mark.parametrize("dtype", ["f16", "bf16"])
+def test_quantise_large(built_lib, fmt, dtype):
+    """A matrix of more than 12 Mi elements, whose 16-bit form goes another way; sampled rows."""
+    from kiln_b200 import ops
+    rows, cols = 3001, 4265
+    x = torch.randn(rows, cols, generator=torch.Generator(device="cuda").manual_seed(5), device="cuda").to(TYPES[dtype])
+    q = ops.quant4(x, fmt)
+    y = ops.dequant4(torch.empty(rows, cols, device="cuda"), q)
+    pick = np.unique(np.r_[0:5, 126:131, 2990:3001, np.random.RandomState(0).randint(0, rows, 60)])
+    want = quantise(x[torch.from_numpy(pick).cuda()].double().cpu().numpy(), fmt)[2]
+    assert np.array_equal(y.double().cpu().numpy()[pick], want) and np.array_equal(held(q)[pick], want)
+
+
+@gpu
+@pytest.mark.parametrize("fmt", FMTS)
 def test_quantise_borders(built_lib, fmt):
     from kiln_b200 import ops
     x = _borders(fmt)

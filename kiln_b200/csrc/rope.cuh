@@ -104,7 +104,9 @@ rope_kernel(const __grid_constant__ RopeParams p) {
         }
         const unsigned row = row0 + (unsigned)r;
         const bool turns = s < un.turned;
-        constexpr int U = sizeof(T) == 2 ? 4 : 2;      // heads whose loads are under way together
+        // Heads whose loads are under way together. Measured on B200, 16-bit, 2 and 4: 4096 x (16 + 16) heads of 128 half 12.5, 13.6 us, interleaved 14.1, 12.8; fp32 half, 1 and 2:
+        // 1536 rows 10.6, 10.3 us
+        constexpr int U = sizeof(T) == 2 && !HALF ? 4 : 2;
         const int ca = HALF && !turns ? p.rot + 8 * (s - un.turned) : 8 * s, cb = pairs + 8 * s;
         Raw8<T> a[U], b[U];
         T* dst[U];

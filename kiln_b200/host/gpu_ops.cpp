@@ -2,6 +2,7 @@
 #include "gpu_ops.h"
 
 #include <chrono>
+#include <cmath>
 #include <stdexcept>
 #include <string>
 
@@ -183,6 +184,74 @@ void attention_bwd(float* dq, float* dk, float* dv, const float* q, const float*
           "attention_bwd");
 }
 
+size_t row_bytes4(int cols) { return (size_t)kb_quant4_row_bytes(cols); }
+size_t scale_bytes4(int rows, int cols, int fmt) { return kb_quant4_scale_bytes(rows, cols, fmt); }
+
+void pack4(uint8_t* codes, uint8_t* scales, const void* w, int dtype, int rows, int cols, int fmt, int exp) {
+    check(kb_quant4(codes, (int)row_bytes4(cols), scales, w, cols, dtype, rows, cols, fmt, exp, g_ctx.stream), "pack4");
+}
+
+namespace {
+size_t bytes4(int rows, int cols, int fmt) { return align256((size_t)rows * row_bytes4(cols)) + align256(scale_bytes4(rows, cols, fmt)); }
+// room of a 4-bit matrix at `at` of the context's workspace
+Weight4 scratch4(int rows, int cols, int fmt, size_t at, const char* what) {
+    if (!g_ctx.workspace || g_ctx.workspace_bytes < at + bytes4(rows, cols, fmt)) throw std::runtime_error(std::string(what) + ": the workspace is too small for the 4-bit activations");
+    Weight4 m;
+    m.codes = static_cast<uint8_t*>(g_ctx.workspace) + at;
+    m.scales = m.codes + align256((size_t)rows * row_bytes4(cols));
+    m.rows = rows; m.cols = cols; m.fmt = fmt;
+    return m;
+}
+Weight4 activations4(const __half* x16, int T, int cols, int fmt, size_t at, const char* what) {
+    const Weight4 m = scratch4(T, cols, fmt, at, what);
+    pack4(const_cast<uint8_t*>(m.codes), const_cast<uint8_t*>(m.scales), x16, KB_F16, T, cols, fmt, 0);
+    return m;
+}
+void product4(void* y, int ldy, void* y_scales, const Weight4& x, const Weight4& W, int epi, const float* gate, const char* what) {
+    check(kb_linear4(y, ldy, y_scales, x.codes, (int)row_bytes4(x.cols), x.scales, W.codes, (int)row_bytes4(W.cols), W.scales, x.rows, W.rows, W.cols, W.fmt, epi,
+                     std::ldexp(1.f, x.exp + W.exp), gate, g_ctx.stream),
+          what);
+}
+}  // namespace
+
+size_t linear4_workspace(int T, int in, int fmt) { return bytes4(T, in, fmt); }
+size_t mlp4_workspace(int T, int in, int hidden, int fmt) { return bytes4(T, in, fmt) + bytes4(T, hidden, fmt); }
+
+void linear4(void* y, int ldy, const __half* x16, int T, const Weight4& W, Epi16 epi, const float* gate) {
+    if (T == 0) return;
+    product4(y, ldy, nullptr, activations4(x16, T, W.cols, W.fmt, 0, "linear4"), W, (int)epi, gate, "linear4");
+}
+
+void mlp4(float* y, int ldy, const __half* x16, int T, const Weight4& up, const Weight4& down, const float* gate) {
+    if (down.cols != up.rows || down.fmt != up.fmt) throw std::runtime_error("mlp4: the two weights do not follow one another");
+    if (T == 0) return;
+    const Weight4 h = scratch4(T, up.rows, up.fmt, bytes4(T, up.cols, up.fmt), "mlp4");
+    product4(const_cast<uint8_t*>(h.codes), (int)row_bytes4(h.cols), const_cast<uint8_t*>(h.scales), activations4(x16, T, up.cols, up.fmt, 0, "mlp4"), up, KB_EPI_GELU4, nullptr,
+             "mlp4");
+    product4(y, ldy, nullptr, h, down, KB_EPI_RESID, gate, "mlp4");
+}
+
+void linear4_dx(float* dx, const __half* dy16, int T, const Weight4& W) {
+    if (T == 0) return;
+    check(kb_linear4_dx(dx, W.cols, KB_F32, dy16, W.rows, W.codes, (int)row_bytes4(W.cols), W.scales, T, W.rows, W.cols, W.fmt, W.exp, g_ctx.workspace, g_ctx.workspace_bytes,
+                        g_ctx.stream),
+          "linear4_dx");
+}
+
+void rope_positions(float* q, float* k, int T, int H, int Dh, int rot, bool interleaved, const int* pos, int axes, const double* freq, const int* axis, float amplitude,
+                    bool inverse) {
+    void* const io[2] = {q, k};
+    const void* const in[2] = {q, k};
+    const int ld[2] = {H * Dh, H * Dh}, heads[2] = {H, H};
+    check(kb_rope(k ? 2 : 1, io, ld, in, ld, heads, KB_F32, T, Dh, rot, interleaved ? KB_ROPE_INTERLEAVED : KB_ROPE_HALF, pos, T > 0 ? T : 1, axes, axes, freq, axis, amplitude,
+                  inverse, g_ctx.stream),
+          "rope_positions");
+}
+
+void lora_dropout(__half* y, const __half* x, int rows, int cols, double p, const unsigned long long* rng) {
+    check(kb_dropout(y, cols, KB_F16, x, cols, KB_F16, nullptr, 0, rows, cols, p, rng, g_ctx.stream), "lora_dropout");
+}
+
 }  // namespace kiln_b200
 
 // C trampolines so the shim can be exercised from the test-suite without a C++ test runner:
@@ -333,5 +402,41 @@ double kbh_enqueue_cost_us(void* out, const void* q, const void* k, const void* 
     const auto t1 = std::chrono::steady_clock::now();
     cudaStreamSynchronize(nullptr);
     return std::chrono::duration<double, std::micro>(t1 - t0).count() / n;
+}
+struct W4 { void* y; int ldy; const void* x; int T; const void *c, *s; int rows, cols; const void *c2, *s2; int rows2, fmt, exp, what; const float* gate; };
+static kiln_b200::Weight4 weight4(const void* c, const void* s, int rows, int cols, int fmt, int exp) {
+    kiln_b200::Weight4 w;
+    w.codes = (const uint8_t*)c; w.scales = (const uint8_t*)s; w.rows = rows; w.cols = cols; w.fmt = fmt; w.exp = exp;
+    return w;
+}
+// what: 0..3 linear4 with that epilogue, 4 mlp4 (c2, s2 = the down-projection [rows2, rows]), 5 linear4_dx (x = dy), 6 pack4 (x = the fp32 weight, y = codes, c2 = scales)
+int kbh_base4(void* y, int ldy, const void* x, int T, const void* codes, const void* scales, int rows, int cols, const void* codes2, const void* scales2, int rows2, int fmt,
+              int exp, int what, const float* gate, char* err, int n) {
+    W4 a{y, ldy, x, T, codes, scales, rows, cols, codes2, scales2, rows2, fmt, exp, what, gate};
+    return guard(err, n, [](void* p) {
+        W4& a = *(W4*)p;
+        const kiln_b200::Weight4 w = weight4(a.c, a.s, a.rows, a.cols, a.fmt, a.exp);
+        if (a.what < 4) kiln_b200::linear4(a.y, a.ldy, (const __half*)a.x, a.T, w, (kiln_b200::Epi16)a.what, a.gate);
+        else if (a.what == 4) kiln_b200::mlp4((float*)a.y, a.ldy, (const __half*)a.x, a.T, w, weight4(a.c2, a.s2, a.rows2, a.rows, a.fmt, a.exp), a.gate);
+        else if (a.what == 5) kiln_b200::linear4_dx((float*)a.y, (const __half*)a.x, a.T, w);
+        else kiln_b200::pack4((uint8_t*)a.y, (uint8_t*)const_cast<void*>(a.c2), a.x, 2, a.rows, a.cols, a.fmt, a.exp);
+    }, &a);
+}
+size_t kbh_base4_workspace(int T, int in, int hidden, int fmt) {
+    return hidden ? kiln_b200::mlp4_workspace(T, in, hidden, fmt) : kiln_b200::linear4_workspace(T, in, fmt);
+}
+struct RP { float *q, *k; int T, H, Dh, rot, inter; const int* pos; int axes; const double* f; const int* ax; float amp; int inv; };
+int kbh_rope_positions(float* q, float* k, int T, int H, int Dh, int rot, int interleaved, const int* pos, int axes, const double* freq, const int* axis, float amplitude,
+                       int inverse, char* err, int n) {
+    RP a{q, k, T, H, Dh, rot, interleaved, pos, axes, freq, axis, amplitude, inverse};
+    return guard(err, n, [](void* p) {
+        RP& a = *(RP*)p;
+        kiln_b200::rope_positions(a.q, a.k, a.T, a.H, a.Dh, a.rot, a.inter != 0, a.pos, a.axes, a.f, a.ax, a.amp, a.inv != 0);
+    }, &a);
+}
+struct LD { void* y; const void* x; int rows, cols; double p; const unsigned long long* rng; };
+int kbh_lora_dropout(void* y, const void* x, int rows, int cols, double p, const unsigned long long* rng, char* err, int n) {
+    LD a{y, x, rows, cols, p, rng};
+    return guard(err, n, [](void* q) { LD& a = *(LD*)q; kiln_b200::lora_dropout((__half*)a.y, (const __half*)a.x, a.rows, a.cols, a.p, a.rng); }, &a);
 }
 }

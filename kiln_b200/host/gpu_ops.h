@@ -108,4 +108,32 @@ void cross_kv16(__half* k16, __half* v16, int ldy, const float* ctx, int L, cons
 void attention_bwd(float* dq, float* dk, float* dv, const float* q, const float* k, const float* v, const float* dout, int Tq, int Tk, int npad,
                    int H = 16);
 
+// ---- A 4-bit base (no counterpart in the engine, whose weights are bf16 / fp16): a weight quantised once, and the linear layers over it.
+// Block formats and layout: kb_quant4 in include/kiln_b200.h.
+struct Weight4 {
+    const uint8_t* codes = nullptr;  // [rows, row_bytes4(cols)]
+    const uint8_t* scales = nullptr; // scale_bytes4(rows, cols, fmt) bytes
+    int rows = 0, cols = 0;          // out, in
+    int fmt = 1, exp = 0;            // KB_MX4 / KB_NV4, and the power of two of an NV4 matrix
+};
+size_t row_bytes4(int cols);
+size_t scale_bytes4(int rows, int cols, int fmt);
+// Fills codes and scales (device buffers of the caller) from a row-major weight of KB_F16 / KB_BF16 / KB_F32 on the context's stream.
+void pack4(uint8_t* codes, uint8_t* scales, const void* w, int dtype, int rows, int cols, int fmt, int exp);
+// y = epi(x16 [T, in] . W^T): x16 is quantised to W's format at the start of the context's workspace (linear4_workspace bytes). Epilogues as linear16's.
+size_t linear4_workspace(int T, int in, int fmt);
+void linear4(void* y, int ldy, const __half* x16, int T, const Weight4& W, Epi16 epi, const float* gate = nullptr);
+// The block's MLP (engine/src/dit.cu:488-493) on 4-bit weights: y [T, ldy] fp32 += gate * (gelu(x16 . up^T) . down^T); the hidden activations are 4 bits as well.
+size_t mlp4_workspace(int T, int in, int hidden, int fmt);
+void mlp4(float* y, int ldy, const __half* x16, int T, const Weight4& up, const Weight4& down, const float* gate);
+// dx [T, in] fp32 = dy16 [T, out] . W, with 2 * out * in bytes of the context's workspace: what a LoRA trainer's backward needs of a frozen 4-bit weight
+void linear4_dx(float* dx, const __half* dy16, int T, const Weight4& W);
+
+// Rotary positions of q and k [T, H * Dh] fp32 in place, from integer positions pos [T, axes] on the device (frame, row, column of a patch) and host arrays
+// freq / axis of rot / 2 entries (kb_rope_freqs fills freq); inverse: the gradient's rotation. k may be null.
+void rope_positions(float* q, float* k, int T, int H, int Dh, int rot, bool interleaved, const int* pos, int axes, const double* freq, const int* axis, float amplitude,
+                    bool inverse);
+// y = dropout(x) over [rows, cols] fp16 (y may be x), rng = seed and offset on the device; the same call on dy is the gradient
+void lora_dropout(__half* y, const __half* x, int rows, int cols, double p, const unsigned long long* rng);
+
 }  // namespace kiln_b200

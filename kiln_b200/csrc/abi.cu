@@ -1063,6 +1063,18 @@ int make_tmap_scales(CUtensorMap* tm, const void* ptr, int rows, int cols, int f
     return r == CUDA_SUCCESS ? KB_OK : KB_ERR_CUDA;
 }
 
+// output [M, N]: box 64 bytes x 32 rows, as an epilogue warp stores it
+int make_tmap_out4(CUtensorMap* tm, void* ptr, int rows, int cols, int ld, bool f32) {
+    const cuuint64_t esz = f32 ? 4 : 2;
+    const cuuint64_t dims[3] = {(cuuint64_t)cols, (cuuint64_t)rows, 1};
+    const cuuint64_t strides[2] = {(cuuint64_t)ld * esz, (cuuint64_t)rows * (cuuint64_t)ld * esz};
+    const cuuint32_t box[3] = {(cuuint32_t)(64 / esz), 32, 1};
+    const cuuint32_t estr[3] = {1, 1, 1};
+    CUresult r = g_encode(tm, f32 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 3, ptr, dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                          CU_TENSOR_MAP_SWIZZLE_64B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    return r == CUDA_SUCCESS ? KB_OK : KB_ERR_CUDA;
+}
+
 template <int EPI, int FMT, bool PAIR>
 int launch_gemm4_shape(DeviceState* st, const Gemm4Maps& maps, Gemm4Params p, cudaStream_t stream) {
     constexpr int TILE = PAIR ? 256 : 128, CTAS = PAIR ? 2 : 1;
@@ -1074,7 +1086,7 @@ int launch_gemm4_shape(DeviceState* st, const Gemm4Maps& maps, Gemm4Params p, cu
     cudaLaunchAttribute cluster;
     cluster.id = cudaLaunchAttributeClusterDimension;
     cluster.val.clusterDim.x = CTAS; cluster.val.clusterDim.y = 1; cluster.val.clusterDim.z = 1;
-    return launch_dependent(gemm4_kernel<EPI, FMT, PAIR>, dim3((unsigned)(groups * CTAS)), dim3(G_THREADS), G4_SMEM, stream, PAIR ? &cluster : nullptr, maps, p);
+    return launch_dependent(gemm4_kernel<EPI, FMT, PAIR>, dim3((unsigned)(groups * CTAS)), dim3(G4_THREADS), G4_SMEM, stream, PAIR ? &cluster : nullptr, maps, p);
 }
 
 template <int EPI, int FMT>
@@ -1178,7 +1190,7 @@ int kb_linear4(void* C, int ldc, void* C_scales, const void* A, int lda, const v
     memset(&maps, 0, sizeof(maps));
     if ((rc = make_tmap_codes(&maps.a, A, M, K, lda)) || (rc = make_tmap_codes(&maps.w, W, N, K, ldw)) ||
         (rc = make_tmap_scales(&maps.sa, A_scales, M, K, fmt)) || (rc = make_tmap_scales(&maps.sw, W_scales, N, K, fmt)) ||
-        (!out4 && (rc = make_tmap_out(&maps.c, C, M, N, ldc, out32, false, false))))
+        (!out4 && (rc = make_tmap_out4(&maps.c, C, M, N, ldc, out32))))
         return rc;
     Gemm4Params p = {};
     p.M = M; p.N = N; p.K = K; p.alpha = alpha; p.C = C; p.ldc = ldc; p.gate = gate; p.status = st->status;

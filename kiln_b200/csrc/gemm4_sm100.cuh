@@ -2,7 +2,7 @@
 // codes and the scales as they lie in memory: tcgen05.mma kind::mxf4 (MX4, a scale per 32) and kind::mxf4nvf4 (NV4, a scale per 16) multiply
 // the 64 products of a k step by their blocks' scales and sum in fp32 in TMEM. Every product and its scaling is exact; only the sums round.
 //
-// The schedule is that of the fp16 product next door (gemm_sm100.cuh): persistent CTAs, one warp loads by TMA, one issues, eight run the epilogue of one
+// The schedule is that of the fp16 product next door (gemm_sm100.cuh): persistent CTAs, one warp loads by TMA, one issues, sixteen run the epilogue of one
 // tile under the main loop of the next. What differs: a k step in shared memory holds 256 columns (128 bytes) of each operand, plus their scales
 // (2 KB per 128 rows for NV4, 1 KB for MX4), which tcgen05.cp copies to TMEM in front of the step's products, four lanes' quarters at a time.
 //
@@ -27,8 +27,11 @@ constexpr int G4_K = 256;                                  // columns of a k ste
 constexpr int G4_STAGES = 5;
 constexpr int G4_SF_OFF = 32768;                           // scales of a stage: A's 128 rows, then W's
 constexpr int G4_STAGE_BYTES = G4_SF_OFF + 6144;
-constexpr int G4_STAGING_WARP = 4096;
-constexpr int G4_SMEM = G4_STAGES * G4_STAGE_BYTES + G_EPI_WARPS * G4_STAGING_WARP + 1024 + 1024;
+// Sixteen epilogue warps, four per TMEM lane quarter, with 32 columns at a time: GELU and quantisation are ~17 instructions per element, and eight warps kept the
+// issue slots 42 % busy (M 4096, N 8192, K 2048 into GELU in 4 bits: 8 warps 44.0 us, 16 T16 us).
+constexpr int G4_EPI_WARPS = 16, G4_THREADS = 32 * (G4_EPI_WARPS + 4);   // last warpgroup: MMA issue, TMA loads, two idle
+constexpr int G4_STAGING_WARP = 2048;                      // a box of 32 rows x 64 bytes on its way out
+constexpr int G4_SMEM = G4_STAGES * G4_STAGE_BYTES + G4_EPI_WARPS * G4_STAGING_WARP + 1024 + 1024;
 static_assert(G4_SMEM <= 232448, "shared memory of a thread block");
 
 struct Gemm4Params {
@@ -91,27 +94,26 @@ __device__ __forceinline__ void gemm4_tile(int w, const Gemm4Params& p, int& tm,
     tn = in_g / gsz;
 }
 
-// gelu() of gemm_sm100.cuh on a packed pair, the same arithmetic to the bit: (v + |v|) / 2 is max(v, 0) that keeps a NaN, and halving commutes with the
-// last rounding
+// The GELU of gemm_sm100.cuh on a packed pair, two instructions less: with a = -min(|v|, 7) it is max(v, 0) + a 2^(a Q(-a) - 1). max keeps a NaN.
 __device__ __forceinline__ uint64_t gelu2(uint64_t v) {
     float v0, v1;
     unpack2(v, v0, v1);
-    const uint64_t a = pack2(fminf(fabsf(v0), 7.f), fminf(fabsf(v1), 7.f));
+    const uint64_t a = pack2(fmaxf(-fabsf(v0), -7.f), fmaxf(-fabsf(v1), -7.f));
     auto both = [](float c) { return pack2(c, c); };
-    uint64_t q = both(2.5095840960887017e-09f);                           // the polynomial with its sign turned
+    uint64_t q = both(-2.5095840960887017e-09f);
     q = fma2(q, a, both(-9.659256505756275e-08f));
-    q = fma2(q, a, both(1.6297367437800858e-06f));
+    q = fma2(q, a, both(-1.6297367437800858e-06f));
     q = fma2(q, a, both(-1.5769759556860663e-05f));
-    q = fma2(q, a, both(9.427715122001246e-05f));
+    q = fma2(q, a, both(-9.427715122001246e-05f));
     q = fma2(q, a, both(-3.198326739948243e-04f));
-    q = fma2(q, a, both(5.3875570301897824e-05f));
+    q = fma2(q, a, both(-5.3875570301897824e-05f));
     q = fma2(q, a, both(6.906468421220779e-03f));
-    q = fma2(q, a, both(-5.242638662457466e-02f));
+    q = fma2(q, a, both(5.242638662457466e-02f));
     q = fma2(q, a, both(-0.4592227637767792f));
-    q = fma2(q, a, both(-1.151104211807251f));
+    q = fma2(q, a, both(1.151104211807251f));
     float t0, t1;
-    unpack2(mul2(q, a), t0, t1);
-    return fma2(mul2(a, both(-0.5f)), pack2(ex2(t0), ex2(t1)), pack2(max0_nan(v0), max0_nan(v1)));
+    unpack2(fma2(q, a, both(-1.f)), t0, t1);
+    return fma2(a, pack2(ex2(t0), ex2(t1)), pack2(max0_nan(v0), max0_nan(v1)));
 }
 
 // Codes and scales of 32 neighbouring columns of a row (two blocks of NV4, one of MX4), packed pairs: 16 bytes, and the scale bytes from bit 0 on
@@ -138,7 +140,7 @@ __device__ __forceinline__ void quant32(const uint64_t* v, uint4& codes, uint32_
 }
 
 template <int EPI, int FMT, bool PAIR>
-__global__ void __launch_bounds__(G_THREADS, 1)
+__global__ void __launch_bounds__(G4_THREADS, 1)
 gemm4_kernel(const __grid_constant__ Gemm4Maps maps, const Gemm4Params p) {
     constexpr int BN = PAIR ? 256 : 128, TILE_M = PAIR ? 256 : 128;
     constexpr int BUF_COLS = 128, ACC_SF = BUF_COLS + BN;                 // TMEM: the second accumulator begins at BUF_COLS, the scales behind it
@@ -149,15 +151,15 @@ gemm4_kernel(const __grid_constant__ Gemm4Maps maps, const Gemm4Params p) {
     static_assert(ACC_SF + SF_BUFS * SF_COLS <= (int)TMEM_ALL_COLUMNS, "TMEM");
     constexpr uint32_t STAGE_TX = 32768 + PIECES * 512 * (1 + W_BLOCKS);
     constexpr bool OUT32 = EPI == EPI_F32 || EPI == EPI_RESID;
-    constexpr int CW = 64, NCH = BN / CW;                                 // columns per chunk of the epilogue, which a warp has NCH / 2 of
-    constexpr int BOX_COLS = OUT32 ? 32 : CW, BOXES = CW / BOX_COLS;      // a chunk leaves as one or two boxes of 32 rows x 128 bytes
+    constexpr int CW = 32, NCH = BN / CW;                                 // columns per chunk of the epilogue, which a warp has NCH / 4 of
+    constexpr int BOX_COLS = OUT32 ? 16 : CW, BOXES = CW / BOX_COLS;      // a chunk leaves as one or two boxes of 32 rows x 64 bytes
 
     extern __shared__ uint8_t smem_raw[];
     const uint32_t raw = smem_u32(smem_raw);
     const uint32_t base = (raw + 1023u) & ~1023u;
     uint8_t* const smem = smem_raw + (base - raw);
     uint8_t* const stage_out = smem + G4_STAGES * G4_STAGE_BYTES;
-    uint8_t* const ctrl = stage_out + G_EPI_WARPS * G4_STAGING_WARP;
+    uint8_t* const ctrl = stage_out + G4_EPI_WARPS * G4_STAGING_WARP;
     const uint32_t bars = smem_u32(ctrl);
     uint32_t* const tmem_slot = reinterpret_cast<uint32_t*>(ctrl + 512);
     volatile uint32_t* const abort_flag = reinterpret_cast<volatile uint32_t*>(ctrl + 516);
@@ -169,13 +171,13 @@ gemm4_kernel(const __grid_constant__ Gemm4Maps maps, const Gemm4Params p) {
     const int n_tiles = p.tiles_m * p.tiles_n, ksteps = (p.K + G4_K - 1) / G4_K;
 
     if (tid == 0) {
-        for (int i = 0; i < G4BAR_COUNT; i++) mbar_init(bar(i), i >= G4BAR_ACC_EMPTY ? (PAIR ? 2u : 1u) * G_EPI_WARPS : 1u);   // acc_empty: one arrival per epilogue warp of the group
+        for (int i = 0; i < G4BAR_COUNT; i++) mbar_init(bar(i), i >= G4BAR_ACC_EMPTY ? (PAIR ? 2u : 1u) * G4_EPI_WARPS : 1u);   // acc_empty: one arrival per epilogue warp of the group
         *abort_flag = 0u;
         mbar_fence_init();
         fence_proxy_async_smem();
     }
-    if (warp == G_EPI_WARPS + 1 && lane == 0) { tma_prefetch_desc(&maps.a); tma_prefetch_desc(&maps.w); tma_prefetch_desc(&maps.sa); tma_prefetch_desc(&maps.sw); }
-    if (warp == G_EPI_WARPS) {
+    if (warp == G4_EPI_WARPS + 1 && lane == 0) { tma_prefetch_desc(&maps.a); tma_prefetch_desc(&maps.w); tma_prefetch_desc(&maps.sa); tma_prefetch_desc(&maps.sw); }
+    if (warp == G4_EPI_WARPS) {
         tmem_alloc(smem_u32(tmem_slot), TMEM_ALL_COLUMNS);
         tmem_relinquish();
     }
@@ -186,9 +188,9 @@ gemm4_kernel(const __grid_constant__ Gemm4Maps maps, const Gemm4Params p) {
     constexpr uint32_t tmem_base = 0u;                                    // see TMEM_ALL_COLUMNS
     pdl_wait();
 
-    if (warp < G_EPI_WARPS) {
-        setmaxnreg_inc<224>();
-        const int quarter = warp & 3, half = warp >> 2;                   // TMEM lanes [32 quarter, +32); every other chunk of columns
+    if (warp < G4_EPI_WARPS) {
+        setmaxnreg_inc<104>();
+        const int quarter = warp & 3, part = warp >> 2;                   // TMEM lanes [32 quarter, +32); every fourth chunk of columns
         const uint32_t lane_base = (uint32_t)(quarter * 32) << 16;
         uint8_t* const my_stage = stage_out + warp * G4_STAGING_WARP;
         uint32_t use[2] = {0, 0};
@@ -203,33 +205,31 @@ gemm4_kernel(const __grid_constant__ Gemm4Maps maps, const Gemm4Params p) {
             if (!ok) break;
             tc_fence_after();
             const int row = m0 + quarter * 32 + lane, nrow = p.M - (m0 + quarter * 32);
-#pragma unroll 1
-            for (int i = 0; i < NCH / 2; i++) {
-                const int ch = half + 2 * (PAIR ? i ^ buf ^ 1 : i);       // PAIR: the columns that both accumulators own first
-                uint64_t v[CW / 2];
-                {
-                    uint32_t a[CW / 32][32];
+            // PAIR: the columns that both accumulators own first; the other chunk's load is under way while the first one is worked on
+            uint32_t acc[NCH / 4][32];
+            auto column = [&](int i) { return (part + 4 * (PAIR ? i ^ buf ^ 1 : i)) * CW; };
+            tmem_ld32(tmem_base + lane_base + (uint32_t)(buf * BUF_COLS + column(0)), acc[0]);
+            tmem_wait_ld();
+            reg_fence32(acc[0]);
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) {                                              // what the next tile's products overwrite is in registers
+                const uint32_t b = bar(G4BAR_ACC_EMPTY + (PAIR ? 0 : buf));
+                if (PAIR && rank != 0) mbar_arrive_cluster_relaxed(mapa_u32(b, 0));
+                else mbar_arrive(b);
+            }
+            if constexpr (PAIR) tmem_ld32(tmem_base + lane_base + (uint32_t)(buf * BUF_COLS + column(1)), acc[NCH / 4 - 1]);
 #pragma unroll
-                    for (int q = 0; q < CW / 32; q++) tmem_ld32(tmem_base + lane_base + (uint32_t)(buf * BUF_COLS + ch * CW + 32 * q), a[q]);
+            for (int i = 0; i < NCH / 4; i++) {
+                if (i == 1) {
                     tmem_wait_ld();
-#pragma unroll
-                    for (int q = 0; q < CW / 32; q++) reg_fence32(a[q]);
-                    if (i == 0) {                                         // what the next tile's products overwrite is in registers
-                        tc_fence_before();
-                        __syncwarp();
-                        if (lane == 0) {
-                            const uint32_t b = bar(G4BAR_ACC_EMPTY + (PAIR ? 0 : buf));
-                            if (PAIR && rank != 0) mbar_arrive_cluster(mapa_u32(b, 0));
-                            else mbar_arrive(b);
-                        }
-                    }
-                    const uint64_t alpha = pack2(p.alpha, p.alpha);
-#pragma unroll
-                    for (int q = 0; q < CW / 32; q++)
-#pragma unroll
-                        for (int e = 0; e < 16; e++) v[16 * q + e] = mul2(pack2u(a[q][2 * e], a[q][2 * e + 1]), alpha);
+                    reg_fence32(acc[NCH / 4 - 1]);
                 }
-                const int c0 = n0 + ch * CW;
+                uint64_t v[CW / 2];
+                const uint64_t alpha = pack2(p.alpha, p.alpha);
+#pragma unroll
+                for (int e = 0; e < 16; e++) v[e] = mul2(pack2u(acc[i][2 * e], acc[i][2 * e + 1]), alpha);
+                const int c0 = n0 + column(i);
                 if constexpr (EPI == EPI_GELU16 || EPI == EPI_GELU4) {
 #pragma unroll
                     for (int c = 0; c < CW / 2; c++) v[c] = gelu2(v[c]);
@@ -300,17 +300,17 @@ gemm4_kernel(const __grid_constant__ Gemm4Maps maps, const Gemm4Params p) {
                         if (lane == 0) tma_store_wait_read();             // the box that was here has been read
                         __syncwarp();
 #pragma unroll
-                        for (int c = 0; c < 8; c++) {
+                        for (int c = 0; c < 4; c++) {
                             uint4 pk;
                             if constexpr (OUT32) {
-                                const uint64_t* const u = v + b * 16 + 2 * c;
+                                const uint64_t* const u = v + b * 8 + 2 * c;
                                 pk = make_uint4((uint32_t)u[0], (uint32_t)(u[0] >> 32), (uint32_t)u[1], (uint32_t)(u[1] >> 32));
                             } else {
                                 const uint64_t* const u = v + 4 * c;
                                 auto two = [](uint64_t w) { float lo, hi; unpack2(w, lo, hi); return pack16<DT_F16>(lo, hi); };
                                 pk = make_uint4(two(u[0]), two(u[1]), two(u[2]), two(u[3]));
                             }
-                            *reinterpret_cast<uint4*>(my_stage + lane * 128 + ((c ^ (lane & 7)) << 4)) = pk;
+                            *reinterpret_cast<uint4*>(my_stage + lane * 64 + ((c ^ ((lane >> 1) & 3)) << 4)) = pk;
                         }
                         fence_proxy_async_smem();
                         __syncwarp();
@@ -324,7 +324,7 @@ gemm4_kernel(const __grid_constant__ Gemm4Maps maps, const Gemm4Params p) {
             }
         }
         if (lane == 0) tma_store_wait_read();
-    } else if (warp == G_EPI_WARPS) {
+    } else if (warp == G4_EPI_WARPS) {
         setmaxnreg_dec<56>();
         if (rank == 0 && elect_one()) {
             // the products of a step take the pipe 0.3 us, little more than what this thread spends on one: counters instead of remainders
@@ -378,7 +378,7 @@ gemm4_kernel(const __grid_constant__ Gemm4Maps maps, const Gemm4Params p) {
         __syncwarp();
     } else {
         setmaxnreg_dec<56>();
-        if (warp == G_EPI_WARPS + 1 && elect_one()) {
+        if (warp == G4_EPI_WARPS + 1 && elect_one()) {
             uint32_t ring = 0;
             bool good = true;
             for (int w = group; w < n_tiles && good; w += n_groups) {
@@ -422,7 +422,7 @@ gemm4_kernel(const __grid_constant__ Gemm4Maps maps, const Gemm4Params p) {
     }
     tc_fence_before();
     if (PAIR) { cluster_arrive(); cluster_wait(); } else __syncthreads();
-    if (warp == G_EPI_WARPS) {
+    if (warp == G4_EPI_WARPS) {
         if (lane == 0 && *abort_flag) atomicOr(p.status, ST_TIMEOUT);
         tc_fence_after();
         tmem_dealloc(tmem_base, TMEM_ALL_COLUMNS);

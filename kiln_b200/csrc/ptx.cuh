@@ -272,6 +272,11 @@ __device__ __forceinline__ float4 ld_cluster_v4(uint32_t cluster_addr) {
 __device__ __forceinline__ void mbar_arrive_cluster(uint32_t cluster_bar) {
     asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(cluster_bar) : "memory");
 }
+// The same without the release: for a thread that has nothing in memory to publish, only reads that are done (TMEM values in registers behind tcgen05.wait::ld). The
+// release waits until all of the thread's earlier stores have been performed, behind a tile's output ~1500 clocks.
+__device__ __forceinline__ void mbar_arrive_cluster_relaxed(uint32_t cluster_bar) {
+    asm volatile("mbarrier.arrive.relaxed.cluster.shared::cluster.b64 _, [%0];" ::"r"(cluster_bar) : "memory");
+}
 // 3-D tiled load into this CTA's shared memory whose byte count completes on an mbarrier of either CTA of the pair
 __device__ __forceinline__ void tma_load_3d_pair(uint32_t dst, const void* tmap, uint32_t cluster_bar, int c0, int c1, int c2) {
     asm volatile(

@@ -9,12 +9,13 @@
 // Two shapes. Single: one CTA per 128 x 128 tile. PAIR: two CTAs on a 256 x 256 tile (cta_group::2): each loads its 128 rows of A, half of the W rows, the
 // scales of its rows and of ALL columns of the tile, and keeps its half of the accumulator. Two accumulators of 256 columns fill TMEM and leave no
 // room for scales, so they overlap: the first lies in columns [0, 256), the second in [128, 384), the scales behind them. The epilogue drains the 128
-// columns that both own first, and then the next tile's products begin; until then the tensor pipe waits, about 1.5 us per tile. (Pairs on 192 columns, which
-// have two whole accumulators beside the scales, wait for their loads instead: N 8192, K 2048, M 4096 37.3 us against 36.0, K 8192, N 2048 32.6 against 28.6.)
+// columns that both own first, and then the next tile's products begin; until then the tensor pipe waits, some 1000 clocks per tile. (Pairs on 192 columns, which
+// have two whole accumulators beside the scales, wait for their loads instead: with eight epilogue warps N 8192, K 2048, M 4096
+// took 37.3 us against 36.0, K 8192, N 2048 32.6 against 28.6.)
 //
 // What bounds it: a step of a pair takes the products' 512 clocks (490-510 from one to the next by the clock counter), so a long k range runs at the pipe's rate
 // for the clock that the power cap leaves: 8192^3 back to back 229 us at 1.36 GHz and 990 W (4.8 PFLOP/s; 199 us, 5.5, before the clock falls), M 4096, N 2048,
-// K 8192 28.6 us. Short ranges add the waits between tiles: M 4096, N 8192, K 2048 35.5 us, of which the products take 24 at 1.65 GHz.
+// K 8192 28.6 us. Short ranges add the waits between tiles: M 4096, N 8192, K 2048 32.4 us, of which the products take 24 at 1.65 GHz.
 #pragma once
 #include "gemm_sm100.cuh"   // gelu, elect_one, pack16
 #include "quant4.cuh"
@@ -28,7 +29,7 @@ constexpr int G4_STAGES = 5;
 constexpr int G4_SF_OFF = 32768;                           // scales of a stage: A's 128 rows, then W's
 constexpr int G4_STAGE_BYTES = G4_SF_OFF + 6144;
 // Sixteen epilogue warps, four per TMEM lane quarter, with 32 columns at a time: GELU and quantisation are ~17 instructions per element, and eight warps kept the
-// issue slots 42 % busy (M 4096, N 8192, K 2048 into GELU in 4 bits: 8 warps 44.0 us, 16 T16 us).
+// issue slots 42 % busy (M 4096, N 8192, K 2048 into GELU in 4 bits: 8 warps 44.0 us, 16, with both chunks' loads in front, 41.7).
 constexpr int G4_EPI_WARPS = 16, G4_THREADS = 32 * (G4_EPI_WARPS + 4);   // last warpgroup: MMA issue, TMA loads, two idle
 constexpr int G4_STAGING_WARP = 2048;                      // a box of 32 rows x 64 bytes on its way out
 constexpr int G4_SMEM = G4_STAGES * G4_STAGE_BYTES + G4_EPI_WARPS * G4_STAGING_WARP + 1024 + 1024;
@@ -94,23 +95,23 @@ __device__ __forceinline__ void gemm4_tile(int w, const Gemm4Params& p, int& tm,
     tn = in_g / gsz;
 }
 
-// The GELU of gemm_sm100.cuh on a packed pair, two instructions less: with a = -min(|v|, 7) it is max(v, 0) + a 2^(a Q(-a) - 1). max keeps a NaN.
+// v Phi(v) on a packed pair, in the form of gemm_sm100.cuh: with a = -min(|v|, 7), erfc(|v| / sqrt 2) = 2^(a Q(-a)) and v Phi(v) = max(v, 0) + a 2^(a Q(-a) - 1); max
+// keeps a NaN. Here GELU is what bounds the epilogue, so Q has degree 7 and not 10: fitted to -log2(erfc(x / sqrt 2)) / x on [0, 7] (2000 Chebyshev nodes, least squares
+// reweighted by the error of erfc times sqrt(erfc) + 1e-3). Largest error against float64 in fp32 2.4e-7, as with degree 10, relative 8e-6 within |v| < 3 and 6e-4 where
+// the value is below 1e-5.
 __device__ __forceinline__ uint64_t gelu2(uint64_t v) {
     float v0, v1;
     unpack2(v, v0, v1);
     const uint64_t a = pack2(fmaxf(-fabsf(v0), -7.f), fmaxf(-fabsf(v1), -7.f));
     auto both = [](float c) { return pack2(c, c); };
-    uint64_t q = both(-2.5095840960887017e-09f);
-    q = fma2(q, a, both(-9.659256505756275e-08f));
-    q = fma2(q, a, both(-1.6297367437800858e-06f));
-    q = fma2(q, a, both(-1.5769759556860663e-05f));
-    q = fma2(q, a, both(-9.427715122001246e-05f));
-    q = fma2(q, a, both(-3.198326739948243e-04f));
-    q = fma2(q, a, both(-5.3875570301897824e-05f));
-    q = fma2(q, a, both(6.906468421220779e-03f));
-    q = fma2(q, a, both(5.242638662457466e-02f));
-    q = fma2(q, a, both(-0.4592227637767792f));
-    q = fma2(q, a, both(1.151104211807251f));
+    uint64_t q = both(-3.179015664045437e-07f);
+    q = fma2(q, a, both(-5.414401130110491e-06f));
+    q = fma2(q, a, both(-3.436955466895597e-06f));
+    q = fma2(q, a, both(0.0006369439070113003f));
+    q = fma2(q, a, both(0.007798188831657171f));
+    q = fma2(q, a, both(0.053058017045259476f));
+    q = fma2(q, a, both(-0.4590109884738922f));
+    q = fma2(q, a, both(1.151127815246582f));
     float t0, t1;
     unpack2(fma2(q, a, both(-1.f)), t0, t1);
     return fma2(a, pack2(ex2(t0), ex2(t1)), pack2(max0_nan(v0), max0_nan(v1)));

@@ -193,17 +193,17 @@ inline GemmShape gemm_shape(int M, int N, long long ksteps, int n_seg, bool any_
     return g;
 }
 
-// 4-bit product: a pair of CTAs on 256 x 256 tiles or one CTA on 128 x 128. A launch costs a start, and per round of tiles the k steps of 256 columns (0.24 us single,
-// 0.333 pair: four times the products) and what does not run under them: single a part of the epilogue, pair the wait for the accumulators' shared columns
-// and a longer epilogue, by what it does. Units of 10 ns, fitted to these, measured on B200 inside a CUDA graph, single / pair:
-//   N 2048, K 2048, fp16: M 512 4.9 / 7.4 us, 1536 7.5 / 8.1, 3456 11.5 / 12.7, 4096 13.7 / 12.9; K 8192: 1024 12.3 / 15.6, 1536 19.2 / 16.3, 4096 36.4 / 29.0
-//   N 8192, K 2048: fp16 512 9.5 / 9.5, 1536 20.1 / 17.7, 4096 41.3 / 35.5; GELU in 4 bits 512 9.5 / 11.0, 3456 37.9 / 42.7, 4096 43.6 / 44.0
+// 4-bit product: a pair of CTAs on 256 x 256 tiles or one CTA on 128 x 128. A launch costs a start, and per round of tiles the k steps of 256 columns (0.244 us single,
+// 0.33 pair: four times the products) and what does not run under them: single a part of the epilogue, pair the wait for the accumulators' shared columns
+// and a longer epilogue, by what it does. Units of 1 and 10 ns, fitted to these, measured on B200 inside a CUDA graph, single / pair:
+//   N 2048, K 2048, fp16: M 512 4.9 / 6.8 us, 1536 7.5 / 7.5, 3456 11.2 / 11.2, 4096 13.0 / 11.5; K 8192: 1024 12.0 / 14.9, 1536 18.5 / 15.5, 4096 36.0 / 28.0
+//   N 8192, K 2048: fp16 512 9.1 / 8.6, 1536 19.0 / 15.7, 4096 40.4 / 32.4; GELU in 4 bits 512 9.1 / 9.7, 3456 36.7 / 35.6, 4096 42.3 / 37.0
 // The rule is within 3 % of the better one in each of 41 such measurements (tests/test_routes4.py).
-constexpr int GEMM4_SINGLE[6] = {140, 85, 100, 210, 0, 110}, GEMM4_PAIR[6] = {290, 180, 225, 480, 0, 300};   // by epilogue: F32, F16, GELU16, RESID, -, GELU4
+constexpr int GEMM4_SINGLE[6] = {131, 74, 100, 256, 0, 98}, GEMM4_PAIR[6] = {250, 126, 224, 540, 0, 222};   // by epilogue: F32, F16, GELU16, RESID, -, GELU4
 inline bool gemm4_pair(int M, int N, int ksteps, int epi, int sm_count) {
     if (M <= 128) return false;
     const long long pairs = sm_count / 2, single = (long long)((M + 127) / 128) * ((N + 127) / 128), pair = (long long)((M + 255) / 256) * ((N + 255) / 256);
-    return 4600 + (pair + pairs - 1) / pairs * (333LL * ksteps + 10 * GEMM4_PAIR[epi]) < 3000 + (single + sm_count - 1) / sm_count * (240LL * ksteps + 10 * GEMM4_SINGLE[epi]);
+    return 3650 + (pair + pairs - 1) / pairs * (330LL * ksteps + 10 * GEMM4_PAIR[epi]) < 2560 + (single + sm_count - 1) / sm_count * (244LL * ksteps + 10 * GEMM4_SINGLE[epi]);
 }
 
 }  // namespace kb

@@ -11,47 +11,47 @@ from util_routes import CSRC, SMS
 EPI = {"f32": 0, "f16": 1, "gelu16": 2, "resid": 3, "gelu4": 5}
 # Device time (us) of one call on a B200 inside a CUDA graph, NV4: single CTAs, pairs
 MEASURED = [  # M, N, K, epilogue
-    (77, 2048, 1024, "f16", 3.82, 5.38),
-    (200, 2048, 2048, "f16", 4.79, 6.91),
-    (512, 2048, 2048, "f16", 4.86, 7.44),
-    (1000, 2048, 2048, "f32", 6.25, 8.96),
-    (1536, 2048, 2048, "f16", 7.50, 8.12),
-    (2048, 2048, 2048, "f16", 8.24, 8.74),
-    (3456, 2048, 2048, "f16", 11.50, 12.66),
-    (4096, 2048, 2048, "f16", 13.65, 12.91),
-    (4096, 2048, 2048, "f32", 15.72, 15.38),
-    (4096, 2048, 2048, "resid", 20.14, 21.29),
-    (512, 8192, 2048, "gelu4", 9.48, 11.01),
-    (1024, 8192, 2048, "gelu4", 15.06, 16.18),
-    (1536, 8192, 2048, "gelu4", 20.42, 21.81),
-    (2304, 8192, 2048, "gelu4", 26.24, 27.48),
-    (3456, 8192, 2048, "gelu4", 37.85, 42.66),
-    (4096, 8192, 2048, "gelu4", 43.59, 43.96),
-    (512, 8192, 2048, "gelu16", 9.72, 11.12),
-    (1024, 8192, 2048, "gelu16", 15.29, 15.47),
-    (1536, 8192, 2048, "gelu16", 20.74, 19.63),
-    (3456, 8192, 2048, "gelu16", 37.66, 37.16),
-    (4096, 8192, 2048, "gelu16", 43.43, 38.91),
-    (512, 8192, 2048, "f16", 9.47, 9.50),
-    (1024, 8192, 2048, "f16", 15.00, 13.51),
-    (1536, 8192, 2048, "f16", 20.14, 17.70),
-    (2304, 8192, 2048, "f16", 25.49, 22.36),
-    (4096, 8192, 2048, "f16", 41.33, 35.50),
-    (4096, 8192, 2048, "f32", 51.92, 45.93),
-    (512, 2048, 8192, "f16", 11.85, 15.19),
-    (1024, 2048, 8192, "f16", 12.28, 15.59),
-    (1536, 2048, 8192, "f16", 19.19, 16.29),
-    (2304, 2048, 8192, "f16", 20.49, 16.86),
-    (4096, 2048, 8192, "f16", 36.44, 28.95),
-    (4096, 2048, 8192, "f32", 39.59, 31.46),
-    (1536, 2048, 8192, "resid", 21.72, 18.35),
-    (4096, 2048, 8192, "resid", 42.24, 34.01),
-    (4096, 8192, 256, "f16", 16.28, 20.02),
-    (4096, 8192, 512, "f16", 19.51, 21.83),
-    (4096, 8192, 512, "f32", 28.43, 30.15),
-    (1100, 1000, 512, "f16", 4.18, 5.98),
-    (700, 5000, 700, "f16", 5.82, 6.92),
-    (8192, 8192, 8192, "f16", 257.34, 203.12),
+    (77, 2048, 1024, "f16", 3.84, 5.16),
+    (200, 2048, 2048, "f16", 4.78, 6.60),
+    (512, 2048, 2048, "f16", 4.88, 6.76),
+    (1000, 2048, 2048, "f32", 6.17, 8.54),
+    (1536, 2048, 2048, "f16", 7.51, 7.54),
+    (2048, 2048, 2048, "f16", 8.24, 8.05),
+    (3456, 2048, 2048, "f16", 11.23, 11.21),
+    (4096, 2048, 2048, "f16", 13.02, 11.47),
+    (4096, 2048, 2048, "f32", 15.16, 13.49),
+    (4096, 2048, 2048, "resid", 21.37, 21.01),
+    (512, 8192, 2048, "gelu4", 9.13, 9.74),
+    (1024, 8192, 2048, "gelu4", 14.68, 14.02),
+    (1536, 8192, 2048, "gelu4", 20.03, 18.30),
+    (2304, 8192, 2048, "gelu4", 25.64, 23.07),
+    (3456, 8192, 2048, "gelu4", 36.74, 35.55),
+    (4096, 8192, 2048, "gelu4", 42.28, 36.95),
+    (512, 8192, 2048, "gelu16", 9.77, 10.00),
+    (1024, 8192, 2048, "gelu16", 15.18, 14.11),
+    (1536, 8192, 2048, "gelu16", 20.04, 18.28),
+    (3456, 8192, 2048, "gelu16", 36.87, 34.48),
+    (4096, 8192, 2048, "gelu16", 42.83, 36.94),
+    (512, 8192, 2048, "f16", 9.05, 8.63),
+    (1024, 8192, 2048, "f16", 14.10, 12.15),
+    (1536, 8192, 2048, "f16", 19.02, 15.74),
+    (2304, 8192, 2048, "f16", 24.20, 20.19),
+    (4096, 8192, 2048, "f16", 40.35, 32.44),
+    (4096, 8192, 2048, "f32", 49.67, 42.23),
+    (512, 2048, 8192, "f16", 11.53, 14.57),
+    (1024, 2048, 8192, "f16", 11.96, 14.92),
+    (1536, 2048, 8192, "f16", 18.53, 15.54),
+    (2304, 2048, 8192, "f16", 20.37, 16.22),
+    (4096, 2048, 8192, "f16", 35.96, 28.02),
+    (4096, 2048, 8192, "f32", 38.45, 30.42),
+    (1536, 2048, 8192, "resid", 21.79, 18.55),
+    (4096, 2048, 8192, "resid", 43.90, 34.40),
+    (4096, 8192, 256, "f16", 16.37, 14.94),
+    (4096, 8192, 512, "f16", 19.34, 16.67),
+    (4096, 8192, 512, "f32", 27.42, 25.32),
+    (1100, 1000, 512, "f16", 3.95, 5.52),
+    (700, 5000, 700, "f16", 5.65, 6.50),
+    (8192, 8192, 8192, "f16", 256.34, 197.77),
 ]
 
 

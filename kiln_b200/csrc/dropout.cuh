@@ -44,8 +44,9 @@ struct DropoutParams {
 };
 
 // A thread keeps its eight columns and goes down the rows, the next row's load under the ten rounds of this one's. Of 16-bit numbers the integer work bounds
-// it, and one round of thread blocks is best; of fp32 numbers the memory, and many short thread blocks keep more loads under way. Measured on B200, 4096 x 8192,
-// a thread block per row -> one round: bf16 34.9 -> 31.7 us, with a residual 45.1 -> 36.3; fp32 41.5 -> 57.8 (so not taken there).
+// it (180 instructions per eight elements; the issue slots 58 % busy, half of them waiting for the multiplier), and one round of thread blocks that keep the rounds' keys is
+// best; of fp32 numbers the memory, and many short thread blocks keep more loads under way. Measured on B200, 4096 x 8192, a thread block per row -> one round: bf16 34.9
+// -> 31.4 us, with a residual 45.1 -> 35.3 (5.7 TB/s); fp32 42.5 (6.3 TB/s) -> 57.8, so not taken there.
 constexpr int DROP_THREADS_LOG2 = 8, DROP_THREADS = 1 << DROP_THREADS_LOG2;
 template <typename InT, typename OutT> __host__ __device__ constexpr bool drop_one_round() { return sizeof(InT) == 2 && sizeof(OutT) == 2; }
 template <typename InT, typename OutT, bool RESID> __host__ __device__ constexpr int drop_blocks_per_sm() {   // as many as hold without spills

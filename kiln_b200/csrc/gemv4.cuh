@@ -4,8 +4,8 @@
 // A warp takes four rows of W that are 32 apart (their scales lie side by side in one 16-byte word of a piece), a lane 32 columns at a time, the next 32 on
 // their way. The codes of both sides become fp16 (each value is one of its numbers) and are multiplied in pairs there: the products are multiples of 1/4
 // up to 36 and a block of 16 gives each half of a pair eight of them, multiples of 1/4 up to 288, which eleven bits hold exactly. So a block's sum is exact; it
-// is scaled and summed over the blocks in fp32. What bounds it from some thousand rows on is the conversion of codes (a quarter of the rate of arithmetic
-// at best), not memory. Measured on B200, device time, tensor cores -> this: N 2048, K 2048, NV4 4.3 -> 2.5 us, N 8192 5.6 -> 3.8, MX4 5.4 -> 4.0, N 2048, K 8192 9.1 -> 6.2.
+// is scaled and summed over the blocks in fp32. What bounds it is latency: with N 8192, K 2048 a lane has two pieces of 32 columns, the issue slots are 42 % busy and memory is at 16 %.
+// Measured on B200, device time, tensor cores -> this: N 2048, K 2048, NV4 4.3 -> 2.5 us, N 8192 5.6 -> 3.8, MX4 5.4 -> 4.0, N 2048, K 8192 9.1 -> 6.2, 8192 x 8192 18.8 -> 11.8.
 // (Two tokens in this form: as long as the tensor cores take for up to 128.)
 #pragma once
 #include "gemm_sm100.cuh"   // gelu

@@ -285,7 +285,8 @@ dequant4_kernel(const Quant4Params p) {
 }
 
 // The transpose [cols, ld_x], through shared memory in tiles of 128 rows x 64 columns: a thread decodes sixteen columns (one scale) of two rows side by side, which
-// become sixteen pairs along rows of the transpose. What the gradient of a projection's input multiplies with.
+// become sixteen pairs along rows of the transpose. What the gradient of a projection's input multiplies with. 8192 x 2048 to fp16 11.3 us (3.8 TB/s), 4096 x 8192 19.4;
+// in tiles of 64 x 64 with eight columns per thread 14.0 and 25.8.
 constexpr int Q4_TILE_R = 128, Q4_TILE_C = 64, Q4_TILE_LD = Q4_TILE_R + 8;      // a tile row in shared memory starts on 16 bytes, four banks further
 template <typename T, int FMT>
 __global__ void __launch_bounds__(256)

@@ -403,3 +403,71 @@ def test_captured_and_on_another_stream(built_lib):
         assert torch.equal(out, other) and torch.equal(dx, odx)
         a = quantise(xs.double().numpy(), NV4)[2]
         assert (np.abs(out.double().cpu().numpy() - a @ held(W).T) <= _sum_bounds(a, held(W), K)).all()
+
+
+@gpu
+def test_binding_errors_on_the_gpu(built_lib):
+    """What the library refuses becomes KilnError with its code, what the tensors do not fit a ValueError; a tensor elsewhere never reaches a kernel."""
+    import kiln_b200 as kb
+    from kiln_b200 import ops
+    x = _x(1, 5, 64).cuda()
+    with pytest.raises(kb.KilnError) as e:
+        ops.quant4(x, MX4, exp=1)
+    assert e.value.code == -1
+    with pytest.raises(kb.KilnError) as e:
+        ops.dropout(torch.empty_like(x), x, torch.zeros(2, dtype=torch.int64, device="cuda"), 1.0)
+    assert e.value.code == -1
+    A, W = ops.quant4(x, NV4), ops.quant4(_x(2, 24, 64).cuda(), NV4)
+    for bad in (lambda: ops.quant4(x.cpu(), NV4), lambda: ops.quant4(x.double(), NV4), lambda: ops.quant4(x[:, ::2], NV4), lambda: ops.quant4(x, 7),
+                lambda: ops.quant4(x, NV4, out=ops.quant4_empty(5, 65, NV4, "cuda")), lambda: ops.dequant4(torch.empty(5, 63, device="cuda"), A),
+                lambda: ops.linear4(torch.empty(5, 24, device="cuda"), A, W, ops.EPI_F16), lambda: ops.linear4(torch.empty(5, 25, device="cuda"), A, W, ops.EPI_F32),
+                lambda: ops.linear4(torch.empty(5, 24), A, W, ops.EPI_F32), lambda: ops.linear4(x, A, W, ops.EPI_GELU4),
+                lambda: ops.linear4(ops.quant4_empty(5, 24, MX4, "cuda"), A, W, ops.EPI_GELU4),
+                lambda: ops.linear4(torch.empty(5, 24, device="cuda"), A, W, ops.EPI_RESID, gate=torch.ones(23, device="cuda")),
+                lambda: ops.linear4(torch.empty(5, 24, device="cuda"), A, x, ops.EPI_F32), lambda: ops.linear4_dx(torch.empty(5, 64, device="cuda"), x[:, :24], W)):
+        with pytest.raises(ValueError):
+            bad()
+    assert kb.check_status() == 0
+
+
+@gpu
+def test_rows_of_any_stride(built_lib):
+    """A single row whose stride says nothing, an empty matrix, one column."""
+    from kiln_b200 import ops
+    row = _x(3, 1, 96)[0].cuda()
+    for x in (row.expand(1, 96), torch.as_strided(row, (1, 96), (5, 1))):
+        q = ops.quant4(x, NV4)
+        assert np.array_equal(held(q), quantise(row[None].double().cpu().numpy(), NV4)[2])
+        W = ops.quant4(_x(4, 40, 96).cuda(), NV4)
+        want = ops.linear4(torch.empty(1, 40, device="cuda"), q, W, ops.EPI_F32)
+        assert torch.equal(ops.linear4(torch.as_strided(torch.empty(40, device="cuda"), (1, 40), (3, 1)), q, W, ops.EPI_F32), want)
+    e = ops.quant4(torch.empty(0, 96, device="cuda"), NV4)
+    assert ops.linear4(torch.empty(0, 40, device="cuda"), e, W, ops.EPI_F32).shape == (0, 40) and ops.dequant4(torch.empty(0, 96, device="cuda"), e).numel() == 0
+    c = _x(5, 7, 1).cuda()
+    assert np.array_equal(held(ops.quant4(c, MX4)), quantise(c.double().cpu().numpy(), MX4)[2])
+
+
+@gpu
+def test_two_threads_on_two_streams(built_lib):
+    """Calls from two host threads, each on its own stream, at the same time."""
+    import threading
+    from kiln_b200 import ops
+    W = ops.quant4(_x(1, 512, 256, "f32", 0.1).cuda(), NV4, -5)
+    xs = [_x(2 + i, 300 + 100 * i, 256, "f16").cuda() for i in range(2)]
+    want = [ops.linear4(torch.empty(len(x), 512, device="cuda"), ops.quant4(x, NV4), W, ops.EPI_F32) for x in xs]
+    torch.cuda.synchronize()
+    bad = []
+
+    def work(i):
+        s = torch.cuda.Stream()
+        with torch.cuda.stream(s):
+            for _ in range(50):
+                y = ops.linear4(torch.empty(len(xs[i]), 512, device="cuda"), ops.quant4(xs[i], NV4), W, ops.EPI_F32)
+                s.synchronize()
+                if not torch.equal(y, want[i]):
+                    bad.append(i)
+
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(2)]
+    [t.start() for t in threads]
+    [t.join() for t in threads]
+    assert not bad

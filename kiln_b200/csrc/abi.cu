@@ -1262,7 +1262,7 @@ int launch_dropout_r(DeviceState* st, const DropoutParams& p, unsigned across, c
     const long long block_rows = DROP_THREADS >> p.width_log2, down = ((long long)p.rows + block_rows - 1) / block_rows;
     long long grid = down;
     if (drop_one_round<InT, OutT>()) {                    // each thread block on its share of the rows (see the kernel)
-        const long long room = (long long)drop_blocks_per_sm<InT, OutT, RESID>() * st->sm_count / across;
+        const long long room = (long long)drop_blocks_per_sm<RESID>() * st->sm_count / across;
         grid = down <= room ? down : room > 1 ? room : 1;
     }
     return launch_dependent(dropout_kernel<InT, OutT, RESID>, dim3((unsigned)grid, across), dim3(DROP_THREADS), 0, stream, nullptr, p);

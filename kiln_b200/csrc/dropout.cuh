@@ -44,17 +44,16 @@ struct DropoutParams {
 };
 
 // A thread keeps its eight columns and goes down the rows, the next row's load under the ten rounds of this one's. Of 16-bit numbers the integer work bounds
-// it (180 instructions per eight elements; the issue slots 58 % busy, half of them waiting for the multiplier), and one round of thread blocks that keep the rounds' keys is
+// it (113 instructions per eight elements; the issue slots 52 % busy, the warps waiting for the multiplier), and one round of thread blocks that keep the rounds' keys is
 // best; of fp32 numbers the memory, and many short thread blocks keep more loads under way. Measured on B200, 4096 x 8192, a thread block per row -> one round: bf16 34.9
-// -> 31.4 us, with a residual 45.1 -> 35.3 (5.7 TB/s); fp32 42.5 (6.3 TB/s) -> 57.8, so not taken there.
+// -> 26.2 us (5.1 TB/s), with a residual 45.1 -> 35.3 (5.7); fp32 42.5 (6.3 TB/s) -> 57.8, so not taken there.
 constexpr int DROP_THREADS_LOG2 = 8, DROP_THREADS = 1 << DROP_THREADS_LOG2;
 template <typename InT, typename OutT> __host__ __device__ constexpr bool drop_one_round() { return sizeof(InT) == 2 && sizeof(OutT) == 2; }
-template <typename InT, typename OutT, bool RESID> __host__ __device__ constexpr int drop_blocks_per_sm() {   // as many as hold without spills
-    return drop_one_round<InT, OutT>() ? (RESID ? 4 : 5) : (RESID ? 4 : 6);
-}
+// Thread blocks of one round, by the registers: 45 without a residual, 56 with one. (Compiled with a launch bound of 5 blocks, the kernel without a residual takes 31.4 us.)
+template <bool RESID> __host__ __device__ constexpr int drop_blocks_per_sm() { return RESID ? 4 : 5; }
 
 template <typename InT, typename OutT, bool RESID>
-__global__ void __launch_bounds__(DROP_THREADS, drop_blocks_per_sm<InT, OutT, RESID>())
+__global__ void __launch_bounds__(DROP_THREADS, drop_one_round<InT, OutT>() || RESID ? 4 : 6)
 dropout_kernel(const DropoutParams p) {
     pdl_launch();
     pdl_wait();

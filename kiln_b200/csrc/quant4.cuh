@@ -170,6 +170,7 @@ quant4_kernel(const Quant4Params p) {
     const int lane = threadIdx.x & 31, c0 = (int)blockIdx.y * (SEGS * 256) + lane * 8;
     const T* const src = static_cast<const T*>(p.x) + (size_t)row * p.ld_x;
     const float down = pow2f(-p.exp), up = pow2f(p.exp);
+    const uint32_t limit = __float_as_uint(8192.f * up);       // beyond 6 x 448 2^exp all is 6 times the largest scale; |x| 2^-exp itself might not be an fp32 number
     Raw8<T> raw[SEGS];
 #pragma unroll
     for (int i = 0; i < SEGS; i++) raw[i] = load8_raw(src, c0 + i * 256, p.cols, p.wide);
@@ -177,13 +178,18 @@ quant4_kernel(const Quant4Params p) {
     for (int i = 0; i < SEGS; i++) {
         const int c = c0 + i * 256;
         if (c - lane * 8 >= p.cols) break;                     // the whole warp is behind the last column (a piece never begins there)
-        const F8 f = Io<T>::f8(raw[i]);
+        F8 f = Io<T>::f8(raw[i]);
         float big = max3_abs_nan(f.v[0], f.v[1], f.v[2]);
         big = max3_abs_nan(big, f.v[3], f.v[4]);
         big = max3_abs_nan(big, f.v[5], f.v[6]);
         uint32_t top = __float_as_uint(max3_abs_nan(big, f.v[7], 0.f)) & 0x7fffffffu;
         top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
         if (FMT == FMT_MX4) top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
+        if (FMT == FMT_NV4 && !std::is_same<T, __half>::value && top > limit && top < 0x7f800000u) {      // (an fp16 number is below 2^16)
+            top = limit;
+#pragma unroll
+            for (int e = 0; e < 8; e++) f.v[e] = fminf(fmaxf(f.v[e], -__uint_as_float(limit)), __uint_as_float(limit));
+        }
         const BlockScale<FMT> bs(top, down, up);
         uint64_t v[4];
 #pragma unroll

@@ -177,6 +177,21 @@ def test_quantise_extremes(built_lib, fmt):
 
 
 @gpu
+@pytest.mark.parametrize("exp", [-64, -40, -9, 64])
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+def test_quantise_beyond_the_largest_scale(built_lib, dtype, exp):
+    """|x| 2^-exp beyond what 32 bits hold: the scale stays at 448, the codes at 6 with their sign, and smaller elements of the block keep theirs."""
+    from kiln_b200 import ops
+    big = torch.tensor([3e38, -3e38, 1e30, -1e30, 2.0 ** 64, -2.0 ** 63, 0.0, -0.0]).double()
+    small = torch.tensor([2688.0, -1344.0, 448.0, 112.0, -560.0, 2.0 ** 13, -2.0 ** 13, 9000.0]).double() * 2.0 ** exp
+    x = torch.cat([torch.cat([big, small]), torch.cat([small, -small]), torch.cat([small, big / 4])])[None].to(TYPES[dtype])
+    assert torch.isfinite(x.double()).all()
+    code, s, val = quantise(x.double().numpy(), NV4, exp)
+    q = ops.quant4(x.cuda(), NV4, exp)
+    assert np.array_equal(held(q), val)
+
+
+@gpu
 @pytest.mark.parametrize("dtype", ["bf16", "f32"])
 def test_quantise_strides(built_lib, dtype):
     """Rows that start anywhere, codes in wider rows, the bytes between and behind left as they were."""

@@ -1247,8 +1247,10 @@ int kb_rope_freqs(double* freq, int rot_dim, double base, int scaling, double fa
 namespace {
 
 template <typename T>
-int launch_rope_t(const RopeParams& p, bool half, bool vec, unsigned blocks, cudaStream_t stream) {
+int launch_rope_t(const RopeParams& p, bool half, int way, unsigned blocks, cudaStream_t stream) {
     const dim3 grid(blocks), block(ROPE_THREADS);
+    const bool vec = way == ROPE_PIECES;
+    if (way == ROPE_SHIFTED) return launch_dependent(rope_shifted_kernel<T>, grid, block, 0, stream, nullptr, p);
     if (half) {
         if (vec) return launch_dependent(rope_kernel<T, true, true>, grid, block, 0, stream, nullptr, p);
         return launch_dependent(rope_kernel<T, true, false>, grid, block, 0, stream, nullptr, p);
@@ -1316,13 +1318,14 @@ int kb_rope(int n, void* const* out, const int* ld_out, const void* const* in, c
     if (rows == 0) return KB_OK;
     p.pos = pos; p.n = n; p.rows = rows; p.pos_rows = pos_rows; p.ld_pos = ld_pos; p.dim = head_dim; p.rot = rot_dim; p.inverse = inverse != 0;
     p.amplitude = amplitude;
-    const bool half = layout == KB_ROPE_HALF, vec = wide && (!half || rot_dim % 16 == 0);
-    p.block_rows = rope_block_rows(half, vec, head_dim, rot_dim, p.heads);
+    const bool half = layout == KB_ROPE_HALF;
+    const int way = rope_way(wide, half, rot_dim);
+    p.block_rows = rope_block_rows(way, half, head_dim, rot_dim, p.heads);
     const unsigned blocks = (unsigned)(((long long)rows + p.block_rows - 1) / p.block_rows);
     ProfScope ps(st, KB_PROF_NORM_ROPE, stream);
-    if (dtype == KB_F16) return launch_rope_t<__half>(p, half, vec, blocks, stream);
-    if (dtype == KB_BF16) return launch_rope_t<__nv_bfloat16>(p, half, vec, blocks, stream);
-    return launch_rope_t<float>(p, half, vec, blocks, stream);
+    if (dtype == KB_F16) return launch_rope_t<__half>(p, half, way, blocks, stream);
+    if (dtype == KB_BF16) return launch_rope_t<__nv_bfloat16>(p, half, way, blocks, stream);
+    return launch_rope_t<float>(p, half, way, blocks, stream);
 }
 
 int kb_dropout(void* out, int ld_out, int out_dtype, const void* in, int ld_in, int in_dtype, const void* resid, int ld_resid, int rows, int cols, double p_drop,

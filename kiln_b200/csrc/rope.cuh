@@ -9,7 +9,7 @@
 // Bound by memory. The sines of a row serve all of its heads of all tensors: a thread block takes a row (several where they are short), fills shared memory
 // with one (cos, sin) per pair while its first loads are under way, and every thread keeps those of its eight elements as it goes from head to head.
 // Measured on B200, device time: q and k of 1536 rows, 16 heads of 128 each, half, fp32 10.3 us (4.9 TB/s), fp16 6.1; 4096 rows fp16 half 12.5 (5.4), interleaved 12.8; 8190 rows, 16 + 4
-// heads, 96 of 128 interleaved, bf16 19.4 (4.3); 126 of 128 half, where no piece of eight is whole, 4096 rows, 16 + 4 heads 23 us.
+// heads, 96 of 128 interleaved, bf16 19.4 (4.3).
 #pragma once
 #include "quant4.cuh"   // to_f32, from_f32
 
@@ -40,15 +40,66 @@ __host__ __device__ inline RopeUnits rope_units(bool half, int dim, int rot) {
     const int pairs = rot / 2, each = half ? 8 : 4, turned = (pairs + each - 1) / each;
     return {half ? turned + (dim - rot) / 8 : dim / 8, turned, turned * each};
 }
-inline int rope_block_rows(bool half, bool vec, int dim, int rot, int heads) {
-    if (!vec) return 1;
-    const RopeUnits u = rope_units(half, dim, rot);
-    const int n = ROPE_THREADS / (u.per_head * heads);
+enum { ROPE_ELEMENTS, ROPE_PIECES, ROPE_SHIFTED };       // see the two kernels
+inline int rope_way(bool wide, bool half, int rot) { return !wide ? ROPE_ELEMENTS : half && rot % 16 ? ROPE_SHIFTED : ROPE_PIECES; }
+inline int rope_block_rows(int way, bool half, int dim, int rot, int heads) {
+    if (way == ROPE_ELEMENTS) return 1;
+    const int per_head = way == ROPE_SHIFTED ? dim / 8 : rope_units(half, dim, rot).per_head, n = ROPE_THREADS / (per_head * heads);
     return n > 1 ? n : 1;
 }
 
-// VEC: in pieces of eight elements, where every row starts on 16 bytes and a head (HALF: either side of the pairs too) is whole pieces; else a warp takes a head,
-// element by element.
+// (cos, sin) of the rows of a thread block, a row's `stride` apart; a thread keeps its pair, so that it fetches one frequency. each > 1: the pairs of a unit of `each`
+// lie `turned` apart, those of neighbouring units side by side, so that neighbouring lanes read neighbouring words
+__device__ __forceinline__ void rope_sines(const RopeParams& p, float2* cs, unsigned row0, int rows, int stride, int each, int turned) {
+    const int pairs = p.rot >> 1, per = ROPE_THREADS / pairs, f = threadIdx.x % pairs;
+    int r = threadIdx.x / pairs;
+    if (r >= per) return;
+    const unsigned long long freq = p.freq[f];
+    const int axis = p.axis[f];
+    float2* const at = cs + (f % each) * turned + f / each;
+    for (; r < rows; r += per) {
+        const int pos = p.pos[(size_t)((row0 + (unsigned)r) % (unsigned)p.pos_rows) * p.ld_pos + axis];
+        const unsigned long long turn = (unsigned long long)(long long)pos * freq;
+        float sn, cn;
+        sincospif((float)(int)(turn >> 32) * 0x1p-31f, &sn, &cn);     // in half turns, [-1, 1)
+        at[r * stride] = make_float2(cn * p.amplitude, (p.inverse ? -sn : sn) * p.amplitude);
+    }
+}
+// where head v of a row lies
+template <typename T>
+__device__ __forceinline__ void rope_head(const RopeParams& p, unsigned row, int v, const T*& src, T*& dst) {
+    const RopeTensor* t = &p.t[0];
+#pragma unroll
+    for (int k = 1; k < ROPE_MAX_TENSORS; k++)
+        if (k < p.n && v >= p.t[k].first) t = &p.t[k];
+    src = static_cast<const T*>(t->x) + (size_t)row * t->ld_x + (v - t->first) * p.dim;
+    dst = static_cast<T*>(t->y) + (size_t)row * t->ld_y + (v - t->first) * p.dim;
+}
+// Which unit of which head of which of the block's rows a thread takes, and how many heads on its next one is (the same for the whole block); the units of a head are neighbouring threads'
+struct RopePlace {
+    int r, v, s, step;
+    bool busy;
+    __device__ __forceinline__ RopePlace(const RopeParams& p, int per_head, int rows) {
+        if (p.block_rows == 1) {
+            r = 0;
+            step = ROPE_THREADS / per_head;
+            v = threadIdx.x / per_head;
+            s = threadIdx.x - v * per_head;
+            busy = v < step && v < p.heads;
+        } else {                                       // every thread has one unit of one head of one row
+            const int all = per_head * p.heads;
+            r = threadIdx.x / all;
+            const int j = threadIdx.x - r * all;
+            v = j / per_head;
+            s = j - v * per_head;
+            step = p.heads;
+            busy = r < rows;
+        }
+    }
+};
+
+// VEC (ROPE_PIECES): in pieces of eight elements, where every row starts on 16 bytes and a head (HALF: either side of the pairs too) is whole pieces; else
+// (ROPE_ELEMENTS) a warp takes a head, element by element.
 template <typename T, bool HALF, bool VEC>
 __global__ void __launch_bounds__(ROPE_THREADS)
 rope_kernel(const __grid_constant__ RopeParams p) {
@@ -61,49 +112,10 @@ rope_kernel(const __grid_constant__ RopeParams p) {
     const int stride = VEC ? un.slots : pairs;
     const unsigned row0 = blockIdx.x * (unsigned)p.block_rows;
     const int rows = (int)min((unsigned)p.block_rows, (unsigned)p.rows - row0);
-    // (cos, sin) of the block's rows; a thread keeps its pair, so that it fetches one frequency
-    auto fill = [&]() {
-        const int per = ROPE_THREADS / pairs, f = threadIdx.x % pairs;
-        int r = threadIdx.x / pairs;
-        if (r < per) {
-            const unsigned long long freq = p.freq[f];
-            const int axis = p.axis[f];
-            // VEC: a unit's pairs apart, those of neighbouring units side by side, so that neighbouring lanes read neighbouring words
-            float2* const at = cs + (VEC ? (f % EACH) * un.turned + f / EACH : f);
-            for (; r < rows; r += per) {
-                const int pos = p.pos[(size_t)((row0 + (unsigned)r) % (unsigned)p.pos_rows) * p.ld_pos + axis];
-                const unsigned long long turn = (unsigned long long)(long long)pos * freq;
-                float sn, cn;
-                sincospif((float)(int)(turn >> 32) * 0x1p-31f, &sn, &cn);     // in half turns, [-1, 1)
-                at[r * stride] = make_float2(cn * p.amplitude, (p.inverse ? -sn : sn) * p.amplitude);
-            }
-        }
-    };
-    auto head = [&](unsigned row, int v, const T*& src, T*& dst) {
-        const RopeTensor* t = &p.t[0];
-#pragma unroll
-        for (int k = 1; k < ROPE_MAX_TENSORS; k++)
-            if (k < p.n && v >= p.t[k].first) t = &p.t[k];
-        src = static_cast<const T*>(t->x) + (size_t)row * t->ld_x + (v - t->first) * p.dim;
-        dst = static_cast<T*>(t->y) + (size_t)row * t->ld_y + (v - t->first) * p.dim;
-    };
     if constexpr (VEC) {
-        int r = 0, v, s, step;
-        bool busy;
-        if (p.block_rows == 1) {
-            step = ROPE_THREADS / un.per_head;
-            v = threadIdx.x / un.per_head;
-            s = threadIdx.x - v * un.per_head;
-            busy = v < step && v < p.heads;
-        } else {                                       // every thread has one unit of one head of one row
-            const int all = un.per_head * p.heads;
-            r = threadIdx.x / all;
-            const int j = threadIdx.x - r * all;
-            v = j / un.per_head;
-            s = j - v * un.per_head;
-            step = p.heads;
-            busy = r < rows;
-        }
+        const RopePlace at(p, un.per_head, rows);
+        const int r = at.r, s = at.s, step = at.step;
+        int v = at.v;
         const unsigned row = row0 + (unsigned)r;
         const bool turns = s < un.turned;
         // Heads whose loads are under way together. Measured on B200, 16-bit, 2 and 4: 4096 x (16 + 16) heads of 128 half 12.5, 13.6 us, interleaved 14.1, 12.8; fp32 half, 1 and 2:
@@ -117,15 +129,15 @@ rope_kernel(const __grid_constant__ RopeParams p) {
             for (int i = 0; i < U; i++) {
                 if (v + i * step >= p.heads) break;
                 const T* src;
-                head(row, v + i * step, src, dst[i]);
+                rope_head(p, row, v + i * step, src, dst[i]);
                 a[i] = Io<T>::raw8(src + ca);
                 if (HALF && turns) b[i] = Io<T>::raw8(src + cb);
             }
         };
-        if (busy) load();                              // under the sines
-        fill();
+        if (at.busy) load();                           // under the sines
+        rope_sines(p, cs, row0, rows, stride, EACH, un.turned);
         __syncthreads();
-        if (!busy) return;
+        if (!at.busy) return;
         float2 z[EACH];
 #pragma unroll
         for (int e = 0; e < EACH; e++) {
@@ -162,13 +174,13 @@ rope_kernel(const __grid_constant__ RopeParams p) {
             load();
         }
     } else {
-        fill();
+        rope_sines(p, cs, row0, rows, stride, 1, 1);
         __syncthreads();
         const int lane = threadIdx.x & 31;
         for (int v = threadIdx.x >> 5; v < p.heads; v += ROPE_THREADS / 32) {
             const T* src;
             T* dst;
-            head(row0, v, src, dst);
+            rope_head(p, row0, v, src, dst);
             for (int s = lane; s < pairs; s += 32) {
                 const int ia = HALF ? s : 2 * s, ib = HALF ? pairs + s : 2 * s + 1;
                 const float2 z = cs[s];
@@ -177,6 +189,73 @@ rope_kernel(const __grid_constant__ RopeParams p) {
                 dst[ib] = from_f32<T>(y * z.x + x * z.y);
             }
             for (int c = p.rot + lane; c < p.dim; c += 32) dst[c] = src[c];
+        }
+    }
+}
+
+// Halves of pairs where no piece of eight begins with the second one (rot / 2 no multiple of eight): a thread takes eight elements of a head, and their partners one by one
+// out of shared memory, where the block's heads lie for the while. A block has read its heads before it writes one, so the output may be the input. Measured on
+// B200, a warp per head, element by element -> this: 4096 rows, 126 of 128, 16 + 4 heads, fp16 23.3 -> 14.7 us, fp32 29.3 -> 21.5 (3.9 TB/s); 34 of 128, 16 + 16 heads, fp16
+// 43.7 -> 17.2 (3.9). Partners as two pieces shifted by a run-time count: 37 us for the first. What bounds it is the instructions of a partner apiece.
+template <typename T>
+__global__ void __launch_bounds__(ROPE_THREADS, sizeof(T) == 2 ? 1 : 8)
+rope_shifted_kernel(const __grid_constant__ RopeParams p) {
+    constexpr int U = sizeof(T) == 2 ? 4 : 1;          // heads at a time (4 and 2: 14.7 and 15.6 us; fp32, 2 and 1: 22.6 and 21.5)
+    __shared__ float2 cs[ROPE_SLOTS];                  // a row has 8 turned <= dim of them, and block_rows * heads * dim / 8 <= ROPE_THREADS (or block_rows = 1, dim <= 256)
+    __shared__ Raw8<T> stage[U * ROPE_THREADS];
+    pdl_launch();
+    pdl_wait();
+    const int pairs = p.rot >> 1, per_head = p.dim >> 3, turned = (pairs + 7) >> 3;
+    const unsigned row0 = blockIdx.x * (unsigned)p.block_rows;
+    const int rows = (int)min((unsigned)p.block_rows, (unsigned)p.rows - row0);
+    const RopePlace at(p, per_head, rows);
+    const unsigned row = row0 + (unsigned)at.r;
+    const int c0 = 8 * at.s;
+    Raw8<T> a[U];
+    T* dst[U];
+    float2 z[8];
+    for (int first = 0; first < p.heads; first += U * at.step) {          // `first` and `step` are the same for the whole block
+        const int v = first + at.v;
+#pragma unroll
+        for (int i = 0; i < U; i++) {
+            if (!at.busy || v + i * at.step >= p.heads) break;
+            const T* src;
+            rope_head(p, row, v + i * at.step, src, dst[i]);
+            a[i] = Io<T>::raw8(src + c0);
+        }
+        if (first == 0) rope_sines(p, cs, row0, rows, 8 * turned, 8, turned);
+        else __syncthreads();                                             // the heads before are done with
+#pragma unroll
+        for (int i = 0; i < U; i++) {
+            if (!at.busy || v + i * at.step >= p.heads) break;
+            stage[i * ROPE_THREADS + threadIdx.x] = a[i];
+        }
+        __syncthreads();
+        if (!at.busy) continue;
+        const int left = p.rot - c0, low = pairs - c0;                    // elements of the piece that turn, those of the first half
+        if (first == 0) {
+#pragma unroll
+            for (int e = 0; e < 8; e++) {
+                const int f = min(c0 + e - (e < low ? 0 : pairs), pairs - 1);
+                z[e] = cs[at.r * 8 * turned + (f & 7) * turned + (f >> 3)];
+                z[e].y = e < low ? -z[e].y : z[e].y;
+            }
+        }
+#pragma unroll
+        for (int i = 0; i < U; i++) {
+            if (v + i * at.step >= p.heads) break;
+            F8 x = Io<T>::f8(a[i]);
+            if (left > 0) {
+                const T* const own = reinterpret_cast<const T*>(stage + i * ROPE_THREADS + threadIdx.x);
+                const T* const to = own + pairs;
+                const T* const from = own - pairs;
+#pragma unroll
+                for (int e = 0; e < 8; e++) {                             // a partner lies in the head whatever e; it is taken where e turns
+                    const float y = to_f32((e < low ? to : from)[e]), t = x.v[e] * z[e].x + y * z[e].y;
+                    x.v[e] = e < left ? t : x.v[e];
+                }
+            }
+            Io<T>::st8(dst[i] + c0, x);
         }
     }
 }

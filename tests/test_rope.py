@@ -98,6 +98,33 @@ def test_rotation(built_lib, dtype, half, rows, pos_rows, heads, dim, rot, axes,
             assert np.array_equal(got[:, rest], x[:, rest]) and torch.equal(o, i)
 
 
+SHIFTED = [  # heads of whole pieces of eight whose halves begin inside one
+    (21, 21, (16, 4), 128, 126, 1, 7), (5, 5, (33,), 256, 250, 2, 0), (40, 8, (1,), 8, 2, 1, 3), (19, 19, (1, 1), 32, 14, 1, 0), (6, 6, (40, 9, 2), 40, 36, 3, 0),
+    (3, 3, (13, 5), 248, 8, 1, 100), (17, 17, (2, 1), 128, 34, 1, 0), (2, 2, (64, 64), 64, 62, 1, 0)]
+
+
+@gpu
+@pytest.mark.parametrize("dtype", list(TYPES))
+@pytest.mark.parametrize("rows,pos_rows,heads,dim,rot,axes,start", SHIFTED)
+def test_shifted_halves(built_lib, dtype, rows, pos_rows, heads, dim, rot, axes, start):
+    test_rotation(built_lib, dtype, True, rows, pos_rows, heads, dim, rot, axes, start)
+
+
+@gpu
+def test_shifted_halves_keep_to_themselves(built_lib):
+    """Infinities and NaN spoil their own pair only; what does not turn is copied bit for bit, a negative zero too."""
+    from kiln_b200 import ops
+    x = _x(4, 6, 2 * 40, "f16")
+    x[:, 36:40], x[1, 3], x[2, 20], x[3, 77] = -0.0, float("inf"), float("nan"), float("inf")
+    pos, freq = torch.arange(6).int()[:, None].cuda(), ops.rope_freqs(34)
+    y = ops.rope([torch.empty_like(x).cuda()], [x.cuda()], [2], 40, pos, freq)[0].cpu()
+    bad = torch.zeros(6, 80, dtype=torch.bool)
+    bad[1, [3, 20]], bad[2, [3, 20]], bad[3, 77] = True, True, True
+    assert torch.isfinite(y[~bad]).all() and not torch.isfinite(y[bad]).any()
+    rest = torch.arange(80) % 40 >= 34
+    assert torch.equal(y[:, rest].view(torch.int16), x[:, rest].view(torch.int16))
+
+
 @gpu
 @pytest.mark.parametrize("half", [True, False], ids=["half", "interleaved"])
 def test_strides_and_alignment(built_lib, half):

@@ -1010,11 +1010,16 @@ dim3 quant4_grid(const Quant4Params& p) {
     return dim3((unsigned)(((long long)p.rows + WARPS - 1) / WARPS), (unsigned)((p.cols + COLS - 1) / COLS));
 }
 
+template <typename T, int FMT, bool WIDE>
+int launch_quant4_w(const Quant4Params& p, cudaStream_t stream) {
+    if constexpr (sizeof(T) == 2)
+        if ((long long)p.rows * p.cols >= Q4_LARGE) return launch_dependent(quant4_kernel<T, FMT, 4, WIDE>, quant4_grid<1024>(p), dim3(Q4_THREADS), 0, stream, nullptr, p);
+    return launch_dependent(quant4_kernel<T, FMT, 2, WIDE>, quant4_grid<512>(p), dim3(Q4_THREADS), 0, stream, nullptr, p);
+}
+
 template <typename T, int FMT>
 int launch_quant4_t(const Quant4Params& p, cudaStream_t stream) {
-    if constexpr (sizeof(T) == 2)
-        if ((long long)p.rows * p.cols >= Q4_LARGE) return launch_dependent(quant4_kernel<T, FMT, 4>, quant4_grid<1024>(p), dim3(Q4_THREADS), 0, stream, nullptr, p);
-    return launch_dependent(quant4_kernel<T, FMT, 2>, quant4_grid<512>(p), dim3(Q4_THREADS), 0, stream, nullptr, p);
+    return p.wide ? launch_quant4_w<T, FMT, true>(p, stream) : launch_quant4_w<T, FMT, false>(p, stream);
 }
 
 template <int FMT>
@@ -1260,26 +1265,28 @@ int launch_rope_t(const RopeParams& p, bool half, int way, unsigned blocks, cuda
 }
 
 template <typename InT, typename OutT, bool RESID>
-int launch_dropout_r(DeviceState* st, const DropoutParams& p, unsigned across, cudaStream_t stream) {
+int launch_dropout_r(DeviceState* st, const DropoutParams& p, bool wide, unsigned across, cudaStream_t stream) {
     const long long block_rows = DROP_THREADS >> p.width_log2, down = ((long long)p.rows + block_rows - 1) / block_rows;
     long long grid = down;
     if (drop_one_round<InT, OutT>()) {                    // each thread block on its share of the rows (see the kernel)
-        const long long room = (long long)drop_blocks_per_sm<RESID>() * st->sm_count / across;
+        const long long room = (long long)(wide ? drop_blocks_per_sm<RESID, true>() : drop_blocks_per_sm<RESID, false>()) * st->sm_count / across;
         grid = down <= room ? down : room > 1 ? room : 1;
     }
-    return launch_dependent(dropout_kernel<InT, OutT, RESID>, dim3((unsigned)grid, across), dim3(DROP_THREADS), 0, stream, nullptr, p);
+    const dim3 blocks((unsigned)grid, across);
+    if (wide) return launch_dependent(dropout_kernel<InT, OutT, RESID, true>, blocks, dim3(DROP_THREADS), 0, stream, nullptr, p);
+    return launch_dependent(dropout_kernel<InT, OutT, RESID, false>, blocks, dim3(DROP_THREADS), 0, stream, nullptr, p);
 }
 
 template <typename InT, typename OutT>
-int launch_dropout_t(DeviceState* st, const DropoutParams& p, unsigned across, cudaStream_t stream) {
-    return p.resid ? launch_dropout_r<InT, OutT, true>(st, p, across, stream) : launch_dropout_r<InT, OutT, false>(st, p, across, stream);
+int launch_dropout_t(DeviceState* st, const DropoutParams& p, bool wide, unsigned across, cudaStream_t stream) {
+    return p.resid ? launch_dropout_r<InT, OutT, true>(st, p, wide, across, stream) : launch_dropout_r<InT, OutT, false>(st, p, wide, across, stream);
 }
 
 template <typename InT>
-int launch_dropout(DeviceState* st, const DropoutParams& p, int out_dtype, unsigned across, cudaStream_t stream) {
-    if (out_dtype == KB_F16) return launch_dropout_t<InT, __half>(st, p, across, stream);
-    if (out_dtype == KB_BF16) return launch_dropout_t<InT, __nv_bfloat16>(st, p, across, stream);
-    return launch_dropout_t<InT, float>(st, p, across, stream);
+int launch_dropout(DeviceState* st, const DropoutParams& p, int out_dtype, bool wide, unsigned across, cudaStream_t stream) {
+    if (out_dtype == KB_F16) return launch_dropout_t<InT, __half>(st, p, wide, across, stream);
+    if (out_dtype == KB_BF16) return launch_dropout_t<InT, __nv_bfloat16>(st, p, wide, across, stream);
+    return launch_dropout_t<InT, float>(st, p, wide, across, stream);
 }
 
 }  // namespace
@@ -1348,16 +1355,16 @@ int kb_dropout(void* out, int ld_out, int out_dtype, const void* in, int ld_in, 
     p.rows = rows; p.cols = cols;
     p.ld_x = ld_in; p.ld_r = ld_resid; p.ld_y = ld_out;
     p.t = t; p.scale = (float)(65536.0 / (65536.0 - t));
-    p.wide = wide_rows(in, ld_in, in_dtype) && wide_rows(out, ld_out, out_dtype) && (!resid || wide_rows(resid, ld_resid, out_dtype));
+    const bool wide = wide_rows(in, ld_in, in_dtype) && wide_rows(out, ld_out, out_dtype) && (!resid || wide_rows(resid, ld_resid, out_dtype));
     // a row of a block's threads as wide as a row of the matrix, up to all of them
     const long long groups = ((long long)cols + 7) / 8;
     while (p.width_log2 < DROP_THREADS_LOG2 && 1LL << p.width_log2 < groups) ++p.width_log2;
     const long long across = (groups + (1LL << p.width_log2) - 1) >> p.width_log2;
     if (across > 65535) return KB_ERR_SHAPE;
     ProfScope ps(st, KB_PROF_LINEAR, stream);
-    if (in_dtype == KB_F16) return launch_dropout<__half>(st, p, out_dtype, (unsigned)across, stream);
-    if (in_dtype == KB_BF16) return launch_dropout<__nv_bfloat16>(st, p, out_dtype, (unsigned)across, stream);
-    return launch_dropout<float>(st, p, out_dtype, (unsigned)across, stream);
+    if (in_dtype == KB_F16) return launch_dropout<__half>(st, p, out_dtype, wide, (unsigned)across, stream);
+    if (in_dtype == KB_BF16) return launch_dropout<__nv_bfloat16>(st, p, out_dtype, wide, (unsigned)across, stream);
+    return launch_dropout<float>(st, p, out_dtype, wide, (unsigned)across, stream);
 }
 
 int kb_lora_pack(void* dst_f16, int ld, int col0, const void* src_bf16, int rows, int cols, float scale, void* stream) {

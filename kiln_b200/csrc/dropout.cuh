@@ -40,7 +40,6 @@ struct DropoutParams {
     int width_log2;                       // threads of a block side by side on a row
     unsigned t;                           // a 16-bit number below t drops its element
     float scale;
-    bool wide;                            // every row of every matrix starts on 16 bytes
 };
 
 // A thread keeps its eight columns and goes down the rows, the next row's load under the ten rounds of this one's. Of 16-bit numbers the integer work bounds
@@ -50,38 +49,52 @@ struct DropoutParams {
 constexpr int DROP_THREADS_LOG2 = 8, DROP_THREADS = 1 << DROP_THREADS_LOG2;
 template <typename InT, typename OutT> __host__ __device__ constexpr bool drop_one_round() { return sizeof(InT) == 2 && sizeof(OutT) == 2; }
 // Thread blocks of one round, by the registers: 45 without a residual, 56 with one. (Compiled with a launch bound of 5 blocks, the kernel without a residual takes 31.4 us.)
-template <bool RESID> __host__ __device__ constexpr int drop_blocks_per_sm() { return RESID ? 4 : 5; }
+template <bool RESID, bool WIDE> __host__ __device__ constexpr int drop_blocks_per_sm() { return (RESID ? 4 : 5) - !WIDE; }
 
-template <typename InT, typename OutT, bool RESID>
-__global__ void __launch_bounds__(DROP_THREADS, drop_one_round<InT, OutT>() || RESID ? 4 : 6)
+// WIDE: every row of every matrix starts on 16 bytes. Else the lanes of a row (`width` of a warp's) read and write theirs across, see load_across.
+template <typename InT, typename OutT, bool RESID, bool WIDE>
+__global__ void __launch_bounds__(DROP_THREADS, !WIDE ? RESID ? 3 : 4 : drop_one_round<InT, OutT>() || RESID ? 4 : 6)
 dropout_kernel(const DropoutParams p) {
+    __shared__ Raw8<InT> tiles_x[WIDE ? 1 : DROP_THREADS];
+    __shared__ Raw8<OutT> tiles_y[WIDE ? 1 : DROP_THREADS], tiles_r[WIDE || !RESID ? 1 : DROP_THREADS];
     pdl_launch();
     pdl_wait();
     const unsigned block_rows = DROP_THREADS >> p.width_log2, step = gridDim.x * block_rows;
     unsigned row = blockIdx.x * block_rows + (threadIdx.x >> p.width_log2);
     const int g = (int)(blockIdx.y << p.width_log2) + (int)(threadIdx.x & ((1u << p.width_log2) - 1u)), c = g * 8;
-    if (row >= (unsigned)p.rows || c >= p.cols) return;
+    const int width = min(32, 1 << p.width_log2), lane = threadIdx.x & (width - 1), first = c - 8 * lane;
+    const unsigned place = threadIdx.x - lane;                         // of the lanes that share a row, the first
+    const unsigned above = WIDE ? 0u : (threadIdx.x & 31u) >> p.width_log2;      // rows of the warp above this one's; the warp stays together for the first one's sake
+    if (row - above >= (unsigned)p.rows || (WIDE ? c : first) >= p.cols) return;
+    const int cols = WIDE || row < (unsigned)p.rows ? p.cols : 0;      // of a row behind the last nothing is read or written
     const InT* x = static_cast<const InT*>(p.x) + (size_t)row * p.ld_x;
     const OutT* res = static_cast<const OutT*>(p.resid) + (RESID ? (size_t)row * p.ld_r : 0);
     OutT* y = static_cast<OutT*>(p.y) + (size_t)row * p.ld_y;
     const size_t dx = (size_t)step * p.ld_x, dr = (size_t)step * p.ld_r, dy = (size_t)step * p.ld_y;
-    Raw8<InT> in = load8_raw(x, c, p.cols, p.wide);
+    auto load = [&](const auto* from, int n) { return WIDE ? load8_raw(from, c, n) : load_across(from, first, n, lane, width); };
+    Raw8<InT> in = load(x, cols);
     Raw8<OutT> add;
-    if (RESID) add = load8_raw(res, c, p.cols, p.wide);
+    if (RESID) add = load(res, cols);
     const unsigned long long seed = p.rng[0], offset = p.rng[1];
     const uint32_t t = p.t << 16;
     PhiloxKeys keys(seed);
     if (drop_one_round<InT, OutT>()) keys.keep();
+    int now = cols;
     while (true) {
+        if (!WIDE) {
+            if (RESID) add = across_to_own(add, tiles_r + place, lane, width);
+            in = across_to_own(in, tiles_x + place, lane, width);
+        }
         const F8 v = Io<InT>::f8(in);
         F8 out;
         if (RESID) out = Io<OutT>::f8(add);
         const unsigned next = row + step;
-        const bool more = next > row && next < (unsigned)p.rows;       // (and not beyond 2^32)
+        const bool more = next > row && next - above < (unsigned)p.rows;       // (and not beyond 2^32)
+        const int then = WIDE || next < (unsigned)p.rows ? p.cols : 0;
         if (more) {
             x += dx;
-            in = load8_raw(x, c, p.cols, p.wide);
-            if (RESID) { res += dr; add = load8_raw(res, c, p.cols, p.wide); }
+            in = load(x, then);
+            if (RESID) { res += dr; add = load(res, then); }
         }
         const uint4 w = philox4x32(make_uint4((uint32_t)g, row, (uint32_t)offset, (uint32_t)(offset >> 32)), keys);
         const uint32_t words[4] = {w.x, w.y, w.z, w.w};
@@ -92,10 +105,17 @@ dropout_kernel(const DropoutParams p) {
             const float kept = r >= t ? __fmul_rn(v.v[e], p.scale) : 0.f;
             out.v[e] = RESID ? __fadd_rn(out.v[e], kept) : kept;       // product and sum rounded apart, with a residual and without
         }
-        store8(y, c, p.cols, p.wide, out);
+        if (WIDE) {
+            store8(y, c, p.cols, out);
+        } else {
+            Raw8<OutT> own;
+            Io<OutT>::st8(reinterpret_cast<OutT*>(own.u), out);
+            store_across(own, tiles_y + place, y, first, now, lane, width);
+        }
         if (!more) break;
         y += dy;
         row = next;
+        now = then;
     }
 }
 

@@ -117,26 +117,51 @@ template <> __device__ __forceinline__ float from_f32<float>(float v) { return v
 template <> __device__ __forceinline__ __half from_f32<__half>(float v) { return __float2half_rn(v); }
 template <> __device__ __forceinline__ __nv_bfloat16 from_f32<__nv_bfloat16>(float v) { return __float2bfloat16_rn(v); }
 
-// eight elements from column c of a row, zeros behind the last column; `wide`: every row starts on 16 bytes
+// Rows that do not start on 16 bytes. One thread's eight elements one by one would touch a different 16 bytes in every lane, eight times over; so a
+// warp (or `width` of its lanes) takes its width x 8 columns across, element j of a lane being column j * width + lane, and turns them round in shared memory.
+// Measured on B200, one by one -> across: 4001 x 8190 bf16 to NV4 30.2 -> 24.2 us, back to fp16 54.6 -> 18.8, transposed 94 -> 31; 4001 x 4099 fp32 to NV4 20.7 -> 15.9;
+// dropout (dropout.cuh) of 4000 x 8190 fp16 85.8 -> 42.7, 1000 x 2047 9.7 -> 4.2, 2000 x 4099 fp32 22.9 -> 17.0.
 template <typename T>
-__device__ __forceinline__ F8 load8(const T* row, int c, int cols, bool wide) {
-    if (wide && c + 8 <= cols) return Io<T>::ld8(row + c);
-    F8 f;
+__device__ __forceinline__ Raw8<T> load_across(const T* row, int first, int cols, int lane, int width) {      // zeros behind the last column
+    Raw8<T> r;
 #pragma unroll
-    for (int i = 0; i < 8; i++) f.v[i] = c + i < cols ? to_f32(row[c + i]) : 0.f;
-    return f;
+    for (int j = 0; j < 8; j++) {
+        const int c = first + j * width + lane;
+        reinterpret_cast<T*>(r.u)[j] = c < cols ? row[c] : from_f32<T>(0.f);
+    }
+    return r;
+}
+// `tile`: width places; the whole warp calls
+template <typename T>
+__device__ __forceinline__ Raw8<T> across_to_own(const Raw8<T>& r, Raw8<T>* tile, int lane, int width) {
+#pragma unroll
+    for (int j = 0; j < 8; j++) reinterpret_cast<T*>(tile)[j * width + lane] = reinterpret_cast<const T*>(r.u)[j];
+    __syncwarp();
+    return tile[lane];
 }
 template <typename T>
-__device__ __forceinline__ Raw8<T> load8_raw(const T* row, int c, int cols, bool wide) {
-    if (wide && c + 8 <= cols) return Io<T>::raw8(row + c);
+__device__ __forceinline__ void store_across(const Raw8<T>& own, Raw8<T>* tile, T* row, int first, int cols, int lane, int width) {
+    tile[lane] = own;
+    __syncwarp();
+#pragma unroll
+    for (int j = 0; j < 8; j++) {
+        const int c = first + j * width + lane;
+        if (c < cols) row[c] = reinterpret_cast<const T*>(tile)[j * width + lane];
+    }
+}
+
+// eight elements from column c of a row that starts on 16 bytes, zeros behind the last column
+template <typename T>
+__device__ __forceinline__ Raw8<T> load8_raw(const T* row, int c, int cols) {
+    if (c + 8 <= cols) return Io<T>::raw8(row + c);
     Raw8<T> r;
 #pragma unroll
     for (int i = 0; i < 8; i++) reinterpret_cast<T*>(r.u)[i] = c + i < cols ? row[c + i] : from_f32<T>(0.f);
     return r;
 }
 template <typename T>
-__device__ __forceinline__ void store8(T* row, int c, int cols, bool wide, const F8& f) {
-    if (wide && c + 8 <= cols) { Io<T>::st8(row + c, f); return; }
+__device__ __forceinline__ void store8(T* row, int c, int cols, const F8& f) {
+    if (c + 8 <= cols) { Io<T>::st8(row + c, f); return; }
 #pragma unroll
     for (int i = 0; i < 8; i++)
         if (c + i < cols) row[c + i] = from_f32<T>(f.v[i]);
@@ -160,7 +185,8 @@ struct Quant4Params {
 constexpr int Q4_THREADS = 128;
 constexpr long long Q4_LARGE = 12LL << 20;
 
-template <typename T, int FMT, int SEGS>
+// WIDE: every row of x starts on 16 bytes
+template <typename T, int FMT, int SEGS, bool WIDE>
 __global__ void __launch_bounds__(Q4_THREADS, SEGS == 2 ? 12 : 10)
 quant4_kernel(const Quant4Params p) {
     pdl_launch();
@@ -171,13 +197,18 @@ quant4_kernel(const Quant4Params p) {
     const T* const src = static_cast<const T*>(p.x) + (size_t)row * p.ld_x;
     const float down = pow2f(-p.exp), up = pow2f(p.exp);
     const uint32_t limit = __float_as_uint(8192.f * up);       // beyond 6 x 448 2^exp all is 6 times the largest scale; |x| 2^-exp itself might not be an fp32 number
+    __shared__ Raw8<T> tiles[WIDE ? 1 : Q4_THREADS];
     Raw8<T> raw[SEGS];
 #pragma unroll
-    for (int i = 0; i < SEGS; i++) raw[i] = load8_raw(src, c0 + i * 256, p.cols, p.wide);
+    for (int i = 0; i < SEGS; i++) raw[i] = WIDE ? load8_raw(src, c0 + i * 256, p.cols) : load_across(src, c0 - lane * 8 + i * 256, p.cols, lane, 32);
 #pragma unroll
     for (int i = 0; i < SEGS; i++) {
         const int c = c0 + i * 256;
         if (c - lane * 8 >= p.cols) break;                     // the whole warp is behind the last column (a piece never begins there)
+        if (!WIDE) {
+            if (i > 0) __syncwarp();
+            raw[i] = across_to_own(raw[i], tiles + threadIdx.x - lane, lane, 32);
+        }
         F8 f = Io<T>::f8(raw[i]);
         float big = max3_abs_nan(f.v[0], f.v[1], f.v[2]);
         big = max3_abs_nan(big, f.v[3], f.v[4]);
@@ -242,17 +273,8 @@ __device__ __forceinline__ Raw8<T> q4_values8(const Q4Raw& q, float up) {
     Io<T>::st8(reinterpret_cast<T*>(out.u), f);
     return out;
 }
-// an element of eight that lie in registers
-template <typename T>
-__device__ __forceinline__ T q4_pick(const Raw8<T>& r, int e) {
-    T v = reinterpret_cast<const T*>(r.u)[0];
-#pragma unroll
-    for (int i = 1; i < 8; i++) v = e == i ? reinterpret_cast<const T*>(r.u)[i] : v;
-    return v;
-}
-
-// A lane takes 16 bytes of output where rows start on 16 bytes (fp32: half of eight codes), so that every store of a warp is 512 bytes in a row; else a
-// column at a time. Measured on B200, fp16, 512 columns of a warp -> 1024: 4096 x 8192 18.5 -> 15.8 us, 8192 x 2048 10.0 -> 8.6, 1536 x 2048 3.0 -> 3.0; fp32 the
+// A lane takes 16 bytes of output (fp32: half of eight codes), so that every store of a warp is 512 bytes in a row, or where rows do not start on 16 bytes as many stores
+// of an element apiece as a lane has. Measured on B200, fp16, 512 columns of a warp -> 1024: 4096 x 8192 18.5 -> 15.8 us, 8192 x 2048 10.0 -> 8.6, 1536 x 2048 3.0 -> 3.0; fp32 the
 // other way: 1536 x 2048 4.6 -> 5.0, 8192 x 2048 14.2 -> 14.8.
 template <typename T> __host__ __device__ constexpr int deq_cols() { return sizeof(T) == 2 ? 1024 : 512; }   // columns of a warp
 template <typename T, int FMT>
@@ -266,23 +288,30 @@ dequant4_kernel(const Quant4Params p) {
     const int first = (int)blockIdx.y * COLS, lane = threadIdx.x & 31;
     T* const dst = static_cast<T*>(p.y) + (size_t)row * p.ld_x;
     const float up = pow2f(p.exp);
-    if (!p.wide) {
-        for (int c = first + lane; c < min(first + COLS, p.cols); c += 32) dst[c] = q4_pick(q4_values8<T, FMT>(q4_load8<FMT>(p, (int)row, c & ~7), up), c & 7);
-        return;
-    }
+    __shared__ uint4 tiles[Q4_THREADS];                       // of rows that do not start on 16 bytes
     Q4Raw q[N];
 #pragma unroll
     for (int i = 0; i < N; i++) {
         const int c = first + (i * 32 + lane) * EACH;
-        if (c < p.cols) q[i] = q4_load8<FMT>(p, (int)row, c & ~7);
+        q[i] = c < p.cols ? q4_load8<FMT>(p, (int)row, c & ~7) : Q4Raw{0u, 0u};
     }
 #pragma unroll
     for (int i = 0; i < N; i++) {
         const int c = first + (i * 32 + lane) * EACH;
-        if (c >= p.cols) break;
+        if (c - lane * EACH >= p.cols) break;
         const Raw8<T> v = q4_values8<T, FMT>(q[i], up);
         const uint4 out = EACH == 8 ? v.u[0] : (c & 4) ? v.u[sizeof(T) / 2 - 1] : v.u[0];
-        if (c + EACH <= p.cols) *reinterpret_cast<uint4*>(dst + c) = out;
+        if (!p.wide) {
+            uint4* const tile = tiles + (threadIdx.x - lane);
+            if (i > 0) __syncwarp();
+            tile[lane] = out;
+            __syncwarp();
+#pragma unroll
+            for (int j = 0; j < EACH; j++) {
+                const int col = c - lane * EACH + j * 32 + lane;
+                if (col < p.cols) dst[col] = reinterpret_cast<const T*>(tile)[j * 32 + lane];
+            }
+        } else if (c + EACH <= p.cols) *reinterpret_cast<uint4*>(dst + c) = out;
         else
 #pragma unroll
             for (int e = 0; e < EACH; e++)
@@ -323,6 +352,13 @@ dequant4_t_kernel(const Quant4Params p) {
         }
     }
     __syncthreads();
+    if (!p.wide) {
+        for (int i = threadIdx.x; i < Q4_TILE_C * Q4_TILE_R; i += 256) {
+            const int k = i / Q4_TILE_R, n = i % Q4_TILE_R;
+            if (k0 + k < p.cols && r0 + n < p.rows) static_cast<T*>(p.y)[(size_t)(k0 + k) * p.ld_x + r0 + n] = tile[k * Q4_TILE_LD + n];
+        }
+        return;
+    }
     constexpr int EACH = 16 / sizeof(T), ACROSS = Q4_TILE_R / EACH;    // elements of 16 bytes
 #pragma unroll
     for (int i = threadIdx.x; i < Q4_TILE_C * ACROSS; i += 256) {
@@ -330,7 +366,7 @@ dequant4_t_kernel(const Quant4Params p) {
         if (k0 + k >= p.cols || left <= 0) continue;
         T* const dst = static_cast<T*>(p.y) + (size_t)(k0 + k) * p.ld_x + r0 + n;
         const uint4 v = *reinterpret_cast<const uint4*>(&tile[k * Q4_TILE_LD + n]);
-        if (p.wide && left >= EACH) *reinterpret_cast<uint4*>(dst) = v;
+        if (left >= EACH) *reinterpret_cast<uint4*>(dst) = v;
         else
 #pragma unroll
             for (int e = 0; e < EACH; e++)

@@ -83,6 +83,34 @@ def test_mask_does_not_depend_on_type_stride_or_alignment(built_lib):
 
 
 @gpu
+@pytest.mark.parametrize("xt,yt", [("f16", "f16"), ("bf16", "f32"), ("f32", "bf16"), ("f32", "f32")])
+@pytest.mark.parametrize("rows,cols,off,ld", [(40001, 9, 0, 9), (20011, 100, 1, 103), (3000, 1001, 0, 1001), (700, 8190, 2, 8195), (3, 2049, 5, 2060), (31, 1, 0, 1)])
+def test_rows_of_any_alignment_agree(built_lib, xt, yt, rows, cols, off, ld):
+    """Rows that do not start on 16 bytes get what rows that do get, bit for bit, with a residual and in place too; nothing beside them is written."""
+    from kiln_b200 import ops
+    rng = _rng(cols, rows).cuda()
+    g = torch.Generator(device="cuda").manual_seed(cols)
+    x = torch.randn(rows, ld, generator=g, device="cuda").to(TYPES[xt])[:, off:off + cols]
+    res = torch.randn(rows, ld, generator=g, device="cuda").to(TYPES[yt])
+    wx, wr, want = (ops.padded_empty(rows, cols, t, "cuda") for t in (TYPES[xt], TYPES[yt], TYPES[yt]))
+    wx.copy_(x)
+    wr.copy_(res[:, off:off + cols])
+    for with_res in (False, True):
+        ops.dropout(want, wx, rng, 0.3, resid=wr if with_res else None)
+        big = torch.full((rows, ld), 7.0, dtype=TYPES[yt], device="cuda")
+        ops.dropout(big[:, off:off + cols], x, rng, 0.3, resid=res[:, off:off + cols] if with_res else None)
+        assert torch.equal(big[:, off:off + cols], want)
+        big[:, off:off + cols] = 7
+        assert (big == 7).all()
+    ops.dropout(res[:, off:off + cols], x, rng, 0.3, resid=res[:, off:off + cols])
+    assert torch.equal(res[:, off:off + cols], want)
+    if xt == yt:
+        y = x.clone() if ld == cols else x
+        ops.dropout(want, wx, rng, 0.3)
+        assert torch.equal(ops.dropout(y, y, rng, 0.3), want)
+
+
+@gpu
 def test_in_place_nan_and_gradient(built_lib):
     """In place; a dropped infinity or NaN is a zero; the gradient is the same call."""
     from kiln_b200 import ops

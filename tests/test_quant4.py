@@ -211,6 +211,29 @@ def test_quantise_strides(built_lib, dtype):
         assert np.array_equal(y[:, off:off + 190].double().cpu().numpy(), held(q)) and (y[:, :off] == 7).all() and (y[:, off + 190:] == 7).all()
 
 
+@gpu
+@pytest.mark.parametrize("fmt", FMTS)
+@pytest.mark.parametrize("dtype", list(TYPES))
+@pytest.mark.parametrize("rows,cols,off,ld", [(1700, 8191, 0, 8191), (300, 1030, 1, 1037), (5, 255, 3, 259), (129, 4097, 0, 4098)])
+def test_rows_of_any_alignment_agree(built_lib, fmt, dtype, rows, cols, off, ld):
+    """Rows that do not start on 16 bytes give what a copy that does gives, bit for bit, and so does decoding into such rows."""
+    from kiln_b200 import ops
+    g = torch.Generator(device="cuda").manual_seed(cols)
+    x = torch.randn(rows, ld, generator=g, device="cuda").to(TYPES[dtype])[:, off:off + cols]
+    wide = ops.padded_empty(rows, cols, TYPES[dtype], "cuda")
+    wide.copy_(x)
+    a, b = ops.quant4(x, fmt), ops.quant4(wide, fmt)
+    assert torch.equal(a.codes, b.codes)
+    assert np.array_equal(held(a), held(b)) if rows * cols < 1 << 20 else torch.equal(ops.dequant4(torch.empty(rows, cols, device="cuda"), a), ops.dequant4(torch.empty(rows, cols, device="cuda"), b))
+    ops.dequant4(wide, b)
+    for t in (False, True):
+        shape = (cols, rows) if t else (rows, cols)
+        big = torch.full((shape[0], shape[1] + 5), 7.0, dtype=TYPES[dtype], device="cuda")
+        ops.dequant4(big[:, 2:2 + shape[1]], b, t)
+        assert torch.equal(big[:, 2:2 + shape[1]], wide.T if t else wide)
+        assert (big[:, :2] == 7).all() and (big[:, 2 + shape[1]:] == 7).all()
+
+
 # ---------------------------------------------------------------- products
 def _sum_bounds(a, w, K):
     """What fp32 sums of exact products may be off by, per element: a k step of 64 columns adds 65 numbers, each cut to 2^-23 of the largest of them, which is no

@@ -1327,7 +1327,7 @@ int kb_rope(int n, void* const* out, const int* ld_out, const void* const* in, c
     p.amplitude = amplitude;
     const bool half = layout == KB_ROPE_HALF;
     const int way = rope_way(wide, half, rot_dim);
-    p.block_rows = rope_block_rows(way, half, head_dim, rot_dim, p.heads);
+    rope_split(way, half, (int)elem_size(dtype), head_dim, rot_dim, p.heads, rows, st->sm_count, p.block_rows, p.row_threads);
     const unsigned blocks = (unsigned)(((long long)rows + p.block_rows - 1) / p.block_rows);
     ProfScope ps(st, KB_PROF_NORM_ROPE, stream);
     if (dtype == KB_F16) return launch_rope_t<__half>(p, half, way, blocks, stream);

@@ -6,10 +6,10 @@
 // and a position an integer, so their product modulo 2^64 IS the fraction of the turn, exactly, in two integer multiplications: the
 // only rounding is that of the fraction to 32 bits (2^-32 of a turn) and the sine's own.
 //
-// Bound by memory. The sines of a row serve all of its heads of all tensors: a thread block takes a row (several where they are short), fills shared memory
+// Bound by memory. The sines of a row serve all of its heads of all tensors: a thread block takes a row or several (rope_split), fills shared memory
 // with one (cos, sin) per pair while its first loads are under way, and every thread keeps those of its eight elements as it goes from head to head.
 // Measured on B200, device time: q and k of 1536 rows, 16 heads of 128 each, half, fp32 10.3 us (4.9 TB/s), fp16 6.1; 4096 rows fp16 half 12.5 (5.4), interleaved 12.8; 8190 rows, 16 + 4
-// heads, 96 of 128 interleaved, bf16 19.4 (4.3).
+// heads, 96 of 128 interleaved, bf16 16.3 (5.1).
 #pragma once
 #include "quant4.cuh"   // to_f32, from_f32
 
@@ -28,7 +28,7 @@ struct RopeParams {
     unsigned long long freq[ROPE_MAX_PAIRS];           // turns per position, a 64-bit fraction
     unsigned char axis[ROPE_MAX_PAIRS];
     const int* pos;                                    // [pos_rows, ld_pos]; row r takes row r % pos_rows
-    int n, heads, rows, pos_rows, ld_pos, dim, rot, block_rows, inverse;
+    int n, heads, rows, pos_rows, ld_pos, dim, rot, block_rows, row_threads, inverse;
     float amplitude;
 };
 
@@ -42,10 +42,31 @@ __host__ __device__ inline RopeUnits rope_units(bool half, int dim, int rot) {
 }
 enum { ROPE_ELEMENTS, ROPE_PIECES, ROPE_SHIFTED };       // see the two kernels
 inline int rope_way(bool wide, bool half, int rot) { return !wide ? ROPE_ELEMENTS : half && rot % 16 ? ROPE_SHIFTED : ROPE_PIECES; }
-inline int rope_block_rows(int way, bool half, int dim, int rot, int heads) {
-    if (way == ROPE_ELEMENTS) return 1;
-    const int per_head = way == ROPE_SHIFTED ? dim / 8 : rope_units(half, dim, rot).per_head, n = ROPE_THREADS / (per_head * heads);
-    return n > 1 ? n : 1;
+// Heads whose loads a thread has under way together. Measured on B200, 16-bit, 2 and 4: 4096 x (16 + 16) heads of 128 half 12.5, 13.6 us, interleaved 14.1, 12.8; shifted, 126 of
+// 128, 16 + 4 heads, 15.6, 14.7. fp32 half, 1 and 2: 1536 rows 10.6, 10.3; shifted 21.5, 22.6
+__host__ __device__ constexpr int rope_together(int way, bool half, int elem) {
+    return way == ROPE_SHIFTED ? (elem == 2 ? 4 : 1) : elem == 2 && !half ? 4 : 2;
+}
+// Rows of a thread block and the threads of each. Where a row is short, as many as fit. Else 1, or 2 or 4 where more of the loads that the threads could have under way are
+// then real ones, and all SMs have eight blocks even so: with fewer, rows side by side instead of one behind the other are faster. Measured on B200, 1, 2 and 4 rows,
+// the fullest one marked: 8190 rows, 16 + 4 heads of 128 interleaved bf16 19.4, 18.0, 16.3*; 4096 rows, 16 + 16 heads of 64 half bf16 9.0, 7.4*, 8.0; 8 + 8 of 128 interleaved fp16
+// 10.7, 9.2*, 9.0, and 1024 such rows 4.4*, 5.8, 5.7; 16 + 16 of 128 12.8*, 13.1, 14.1.
+inline void rope_split(int way, bool half, int elem, int dim, int rot, int heads, long long rows, int sm_count, int& block_rows, int& row_threads) {
+    block_rows = 1;
+    row_threads = ROPE_THREADS;
+    if (way == ROPE_ELEMENTS) return;
+    const int per_head = way == ROPE_SHIFTED ? dim / 8 : rope_units(half, dim, rot).per_head, all = per_head * heads, together = rope_together(way, half, elem);
+    if (2 * all <= ROPE_THREADS) {
+        row_threads = all;
+        block_rows = ROPE_THREADS / all;
+        return;
+    }
+    long long best_of = 0, best_turns = 1;                 // all / turns: the share of real loads
+    for (int n = 1; n <= 4 && rows >= (n > 1 ? 8LL * n * sm_count : 0) && per_head * n <= ROPE_THREADS; n *= 2) {
+        const int threads = ROPE_THREADS / n, at_once = threads / per_head * together;
+        const long long turns = (long long)((heads + at_once - 1) / at_once) * together * threads;
+        if (all * best_turns > best_of * turns) { best_of = all; best_turns = turns; block_rows = n; row_threads = threads; }
+    }
 }
 
 // (cos, sin) of the rows of a thread block, a row's `stride` apart; a thread keeps its pair, so that it fetches one frequency. each > 1: the pairs of a unit of `each`
@@ -80,21 +101,12 @@ struct RopePlace {
     int r, v, s, step;
     bool busy;
     __device__ __forceinline__ RopePlace(const RopeParams& p, int per_head, int rows) {
-        if (p.block_rows == 1) {
-            r = 0;
-            step = ROPE_THREADS / per_head;
-            v = threadIdx.x / per_head;
-            s = threadIdx.x - v * per_head;
-            busy = v < step && v < p.heads;
-        } else {                                       // every thread has one unit of one head of one row
-            const int all = per_head * p.heads;
-            r = threadIdx.x / all;
-            const int j = threadIdx.x - r * all;
-            v = j / per_head;
-            s = j - v * per_head;
-            step = p.heads;
-            busy = r < rows;
-        }
+        r = threadIdx.x / p.row_threads;
+        const int j = threadIdx.x - r * p.row_threads;
+        v = j / per_head;
+        s = j - v * per_head;
+        step = p.row_threads / per_head;
+        busy = r < rows && v < step && v < p.heads;
     }
 };
 
@@ -118,9 +130,7 @@ rope_kernel(const __grid_constant__ RopeParams p) {
         int v = at.v;
         const unsigned row = row0 + (unsigned)r;
         const bool turns = s < un.turned;
-        // Heads whose loads are under way together. Measured on B200, 16-bit, 2 and 4: 4096 x (16 + 16) heads of 128 half 12.5, 13.6 us, interleaved 14.1, 12.8; fp32 half, 1 and 2:
-        // 1536 rows 10.6, 10.3 us
-        constexpr int U = sizeof(T) == 2 && !HALF ? 4 : 2;
+        constexpr int U = rope_together(ROPE_PIECES, HALF, sizeof(T));
         const int ca = HALF && !turns ? p.rot + 8 * (s - un.turned) : 8 * s, cb = pairs + 8 * s;
         Raw8<T> a[U], b[U];
         T* dst[U];
@@ -200,7 +210,7 @@ rope_kernel(const __grid_constant__ RopeParams p) {
 template <typename T>
 __global__ void __launch_bounds__(ROPE_THREADS, sizeof(T) == 2 ? 1 : 8)
 rope_shifted_kernel(const __grid_constant__ RopeParams p) {
-    constexpr int U = sizeof(T) == 2 ? 4 : 1;          // heads at a time (4 and 2: 14.7 and 15.6 us; fp32, 2 and 1: 22.6 and 21.5)
+    constexpr int U = rope_together(ROPE_SHIFTED, true, sizeof(T));
     __shared__ float2 cs[ROPE_SLOTS];                  // a row has 8 turned <= dim of them, and block_rows * heads * dim / 8 <= ROPE_THREADS (or block_rows = 1, dim <= 256)
     __shared__ Raw8<T> stage[U * ROPE_THREADS];
     pdl_launch();

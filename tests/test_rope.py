@@ -111,6 +111,14 @@ def test_shifted_halves(built_lib, dtype, rows, pos_rows, heads, dim, rot, axes,
 
 
 @gpu
+@pytest.mark.parametrize("dtype", ["f16", "f32"])
+@pytest.mark.parametrize("half", [True, False], ids=["half", "interleaved"])
+@pytest.mark.parametrize("rows,rot", [(4739, 30), (2371, 32)])
+def test_several_rows_of_a_thread_block(built_lib, dtype, half, rows, rot):
+    test_rotation(built_lib, dtype, half, rows, 1000, (13, 7), 32, rot, 1, 11)
+
+
+@gpu
 def test_shifted_halves_keep_to_themselves(built_lib):
     """Infinities and NaN spoil their own pair only; what does not turn is copied bit for bit, a negative zero too."""
     from kiln_b200 import ops

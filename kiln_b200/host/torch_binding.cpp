@@ -123,8 +123,7 @@ at::Device to_device(PyObject* o) {
 struct Quant4 {
     PyObject_HEAD
     PyObject *codes, *scales, *both;    // `both`: the one buffer of a matrix made here, whose two views are made when they are asked for
-    int rows, cols, fmt, exp, ld, device;
-    unsigned long long codes_ptr, scales_ptr;
+    int rows, cols, fmt, exp;
 };
 PyTypeObject* quant4_type = nullptr;
 
@@ -135,6 +134,57 @@ int64_t scale_bytes(int rows, int cols, int fmt) {
 }
 void check_size(int rows, int cols, int fmt) {
     if (rows < 0 || rows > KB_MAX_Q4_ROWS || cols <= 0 || cols > KB_MAX_Q4_COLS || (fmt != KB_MX4 && fmt != KB_NV4)) refuse("no 4-bit matrix of %d x %d, format %d", rows, cols, fmt);
+}
+
+// Where a matrix lies. A tensor can be given another memory at any time (`codes.data = ...`, which is what moving a parameter to another device does, or
+// storage().resize_()), so this is asked for in every call and kept by none.
+struct Buffers {
+    void *codes, *scales;
+    int ld, device;                     // bytes of a row of codes; -1: the CPU
+};
+// bytes [first, first + n) of a tensor's storage exist
+bool exists(const at::Tensor& t, int64_t first, int64_t n) { return n <= 0 || (int64_t)t.storage().nbytes() >= first + n; }
+
+Buffers buffers(const Quant4& q, const char* name) {
+    const int wide = row_bytes(q.cols);
+    const int64_t n_codes = (int64_t)q.rows * wide, n_scales = scale_bytes(q.rows, q.cols, q.fmt);
+    Buffers b = {nullptr, nullptr, wide, -1};
+    const at::Tensor* both = q.both ? &THPVariable_Unpack(q.both) : nullptr;
+    at::Device codes_device(at::kCPU), scales_device(at::kCPU);
+    if (q.codes) {
+        const at::Tensor& t = THPVariable_Unpack(q.codes);
+        if (t.element_size() != 1 || t.dim() != 2) refuse("%s: codes are a [rows, bytes] matrix of bytes", name);
+        if (t.size(0) < q.rows || t.size(1) < wide || t.stride(1) != 1) refuse("%s: codes do not hold %d rows of %d columns", name, q.rows, q.cols);
+        const int64_t ld = q.rows <= 1 ? wide : t.stride(0);
+        if (ld > std::numeric_limits<int>::max()) refuse("%s: codes have a row stride beyond 32 bits", name);
+        if (!exists(t, t.storage_offset(), q.rows ? (q.rows - 1) * ld + wide : 0)) refuse("%s: the memory behind its codes is gone", name);
+        b.ld = (int)ld;
+        b.codes = t.data_ptr();
+        codes_device = t.device();
+    } else if (both) {
+        if (!exists(*both, both->storage_offset(), n_codes)) refuse("%s: the memory behind its codes is gone", name);
+        b.codes = both->data_ptr();
+        codes_device = both->device();
+    } else {
+        refuse("%s has no buffers", name);
+    }
+    if (q.scales) {
+        const at::Tensor& t = THPVariable_Unpack(q.scales);
+        if (t.element_size() != 1 || !t.is_contiguous()) refuse("%s: scales are contiguous bytes", name);
+        if (t.numel() < n_scales) refuse("%s: scales do not hold %d rows of %d columns", name, q.rows, q.cols);
+        if (!exists(t, t.storage_offset(), n_scales)) refuse("%s: the memory behind its scales is gone", name);
+        b.scales = t.data_ptr();
+        scales_device = t.device();
+    } else if (both) {
+        if (!exists(*both, both->storage_offset() + n_codes, n_scales)) refuse("%s: the memory behind its scales is gone", name);
+        b.scales = static_cast<char*>(both->data_ptr()) + n_codes;
+        scales_device = both->device();
+    } else {
+        refuse("%s has no buffers", name);
+    }
+    if (codes_device != scales_device) refuse("%s: codes and scales lie on one device", name);
+    b.device = codes_device.is_cuda() ? (int)codes_device.index() : -1;
+    return b;
 }
 
 Quant4* new_quant4() {
@@ -148,10 +198,7 @@ Quant4* make_quant4(int rows, int cols, int fmt, int exp, const at::Device& devi
     const int64_t codes = (int64_t)rows * row_bytes(cols);
     at::Tensor both = new_bytes(codes + scale_bytes(rows, cols, fmt), device);
     Quant4* q = new_quant4();
-    q->rows = rows; q->cols = cols; q->fmt = fmt; q->exp = exp; q->ld = row_bytes(cols);
-    q->device = both.is_cuda() ? (int)both.get_device() : -1;
-    q->codes_ptr = (unsigned long long)(uintptr_t)both.data_ptr();
-    q->scales_ptr = q->codes_ptr + (unsigned long long)codes;
+    q->rows = rows; q->cols = cols; q->fmt = fmt; q->exp = exp;
     q->both = THPVariable_Wrap(std::move(both));
     if (!q->both) { Py_DECREF(q); throw Refused(); }
     return q;
@@ -183,19 +230,14 @@ int quant4_init(PyObject* self, PyObject* args, PyObject* kwargs) {
     if (!PyArg_ParseTupleAndKeywords(args, kwargs, "OOiii|i", const_cast<char**>(names), &codes_o, &scales_o, &rows, &cols, &fmt, &exp)) return -1;
     try {
         check_size(rows, cols, fmt);
-        const at::Tensor &codes = tensor(codes_o, "codes"), &scales = tensor(scales_o, "scales");
-        if (codes.element_size() != 1 || scales.element_size() != 1 || codes.dim() != 2 || !scales.is_contiguous())
-            refuse("codes are a [rows, bytes] matrix of bytes, scales contiguous bytes");
-        if (codes.size(0) < rows || codes.size(1) < row_bytes(cols) || codes.stride(1) != 1) refuse("codes do not hold %d rows of %d columns", rows, cols);
-        if (scales.numel() < scale_bytes(rows, cols, fmt)) refuse("scales do not hold %d rows of %d columns", rows, cols);
-        const int64_t ld = rows <= 1 ? row_bytes(cols) : codes.stride(0);
-        if (ld > std::numeric_limits<int>::max()) refuse("codes have a row stride beyond 32 bits");
-        if (codes.device() != scales.device()) refuse("codes and scales lie on one device");
+        tensor(codes_o, "codes");
+        tensor(scales_o, "scales");
+        Quant4 fresh = {};                              // looked over before `self` changes
+        fresh.codes = codes_o; fresh.scales = scales_o;
+        fresh.rows = rows; fresh.cols = cols; fresh.fmt = fmt; fresh.exp = exp;
+        buffers(fresh, "Quant4");
         Quant4* q = reinterpret_cast<Quant4*>(self);
-        q->rows = rows; q->cols = cols; q->fmt = fmt; q->exp = exp; q->ld = (int)ld;
-        q->device = codes.is_cuda() ? (int)codes.get_device() : -1;
-        q->codes_ptr = (unsigned long long)(uintptr_t)codes.data_ptr();
-        q->scales_ptr = (unsigned long long)(uintptr_t)scales.data_ptr();
+        q->rows = rows; q->cols = cols; q->fmt = fmt; q->exp = exp;
         Py_INCREF(codes_o);
         Py_INCREF(scales_o);
         Py_XSETREF(q->codes, codes_o);
@@ -222,8 +264,8 @@ PyObject* view_of(Quant4* q, PyObject** slot, bool scales) {
         if (!*slot) {
             if (!q->both) refuse("this Quant4 has no buffers");
             const at::Tensor& both = THPVariable_Unpack(q->both);
-            const int64_t codes = (int64_t)q->rows * q->ld;
-            *slot = scales ? THPVariable_Wrap(both.narrow(0, codes, both.numel() - codes)) : THPVariable_Wrap(both.narrow(0, 0, codes).view({q->rows, q->ld}));
+            const int64_t wide = row_bytes(q->cols), codes = q->rows * wide;
+            *slot = scales ? THPVariable_Wrap(both.narrow(0, codes, both.numel() - codes)) : THPVariable_Wrap(both.narrow(0, 0, codes).view({q->rows, wide}));
         }
         Py_XINCREF(*slot);
         return *slot;
@@ -235,18 +277,37 @@ PyObject* view_of(Quant4* q, PyObject** slot, bool scales) {
 }
 PyObject* get_codes(PyObject* self, void*) { Quant4* q = reinterpret_cast<Quant4*>(self); return view_of(q, &q->codes, false); }
 PyObject* get_scales(PyObject* self, void*) { Quant4* q = reinterpret_cast<Quant4*>(self); return view_of(q, &q->scales, true); }
+enum { WHERE_CODES, WHERE_SCALES, WHERE_LD, WHERE_DEVICE };
+PyObject* get_where(PyObject* self, void* what) {
+    try {
+        const Buffers b = buffers(*reinterpret_cast<Quant4*>(self), "Quant4");
+        switch ((int)(intptr_t)what) {
+            case WHERE_CODES: return PyLong_FromUnsignedLongLong((uintptr_t)b.codes);
+            case WHERE_SCALES: return PyLong_FromUnsignedLongLong((uintptr_t)b.scales);
+            case WHERE_LD: return PyLong_FromLong(b.ld);
+            default: return PyLong_FromLong(b.device);
+        }
+    } catch (const Refused&) {
+    } catch (const std::exception& e) {
+        PyErr_SetString(PyExc_RuntimeError, e.what());
+    }
+    return nullptr;
+}
 
 PyMemberDef quant4_members[] = {
     {"rows", T_INT, offsetof(Quant4, rows), READONLY, nullptr},
     {"cols", T_INT, offsetof(Quant4, cols), READONLY, nullptr},
     {"fmt", T_INT, offsetof(Quant4, fmt), READONLY, "MX4 or NV4"},
     {"exp", T_INT, offsetof(Quant4, exp), 0, "the whole matrix is times 2^exp"},
-    {"ld", T_INT, offsetof(Quant4, ld), READONLY, "bytes from a row of codes to the next"},
-    {"device", T_INT, offsetof(Quant4, device), READONLY, "index of the GPU, -1 for the CPU"},
-    {"codes_ptr", T_ULONGLONG, offsetof(Quant4, codes_ptr), READONLY, nullptr},
-    {"scales_ptr", T_ULONGLONG, offsetof(Quant4, scales_ptr), READONLY, nullptr},
     {nullptr, 0, 0, 0, nullptr}};
-PyGetSetDef quant4_getset[] = {{"codes", get_codes, nullptr, "uint8 [rows, ld]", nullptr}, {"scales", get_scales, nullptr, "uint8, flat", nullptr}, {nullptr, nullptr, nullptr, nullptr, nullptr}};
+PyGetSetDef quant4_getset[] = {
+    {"codes", get_codes, nullptr, "uint8 [rows, ld]", nullptr},
+    {"scales", get_scales, nullptr, "uint8, flat", nullptr},
+    {"ld", get_where, nullptr, "bytes from a row of codes to the next", (void*)(intptr_t)WHERE_LD},
+    {"device", get_where, nullptr, "index of the GPU, -1 for the CPU", (void*)(intptr_t)WHERE_DEVICE},
+    {"codes_ptr", get_where, nullptr, "where the codes lie now", (void*)(intptr_t)WHERE_CODES},
+    {"scales_ptr", get_where, nullptr, "where the scales lie now", (void*)(intptr_t)WHERE_SCALES},
+    {nullptr, nullptr, nullptr, nullptr, nullptr}};
 PyType_Slot quant4_slots[] = {
     {Py_tp_doc, const_cast<char*>("Quant4(codes, scales, rows, cols, fmt, exp=0): a matrix [rows, cols] of 4-bit numbers in blocks (kb_quant4): codes uint8 [rows, >= 16 ceil(cols / 32)], "
                                   "scales uint8, fmt MX4 or NV4, all of it times 2^exp.")},
@@ -290,8 +351,9 @@ PyObject* py_quant4(PyObject* const* a, Py_ssize_t n) {            // x, fmt, ex
     try {
         const Here here;
         here.have(x.device, "x");
-        here.have(q->device, "out");
-        if (x.rows) check(f_quant4(ptr(q->codes_ptr), q->ld, ptr(q->scales_ptr), x.p, x.ld, x.dtype, x.rows, x.cols, fmt, exp, here.stream), "kb_quant4");
+        const Buffers out = buffers(*q, "out");
+        here.have(out.device, "out");
+        if (x.rows) check(f_quant4(out.codes, out.ld, out.scales, x.p, x.ld, x.dtype, x.rows, x.cols, fmt, exp, here.stream), "kb_quant4");
     } catch (...) {
         Py_DECREF(q);
         throw;
@@ -306,9 +368,10 @@ PyObject* py_dequant4(PyObject* const* a, Py_ssize_t n) {          // y, q, tran
     const bool t = to_bool(a[2]);
     if (y.rows != (t ? q.cols : q.rows) || y.cols != (t ? q.rows : q.cols)) refuse("y is %d x %d for a matrix of %d x %d", y.rows, y.cols, q.rows, q.cols);
     const Here here;
+    const Buffers b = buffers(q, "q");
     here.have(y.device, "y");
-    here.have(q.device, "q");
-    if (q.rows) check(f_dequant4(y.p, y.ld, y.dtype, ptr(q.codes_ptr), q.ld, ptr(q.scales_ptr), q.rows, q.cols, q.fmt, q.exp, t, here.stream), "kb_dequant4");
+    here.have(b.device, "q");
+    if (q.rows) check(f_dequant4(y.p, y.ld, y.dtype, b.codes, b.ld, b.scales, q.rows, q.cols, q.fmt, q.exp, t, here.stream), "kb_dequant4");
     return same(a[0]);
 }
 
@@ -316,13 +379,15 @@ PyObject* py_linear4(PyObject* const* a, Py_ssize_t n) {           // C, A, W, e
     expect(n, 6);
     const Quant4 &A = quant4_arg(a[1], "A"), &W = quant4_arg(a[2], "W");
     const int M = A.rows, N = W.rows, K = A.cols, epi = to_int(a[3]);
+    const Buffers ab = buffers(A, "A"), wb = buffers(W, "W");
     if (W.cols != K || W.fmt != A.fmt) refuse("A and W have to agree in columns and format");
     void *out, *scales = nullptr;
     int ldc, where;
     if (epi == KB_EPI_GELU4) {
         const Quant4& C = quant4_arg(a[0], "C of EPI_GELU4");
         if (C.rows != M || C.cols != N || C.fmt != A.fmt || C.exp != 0) refuse("EPI_GELU4 goes into a Quant4 [M, N] of the operands' format with exp 0");
-        out = ptr(C.codes_ptr); scales = ptr(C.scales_ptr); ldc = C.ld; where = C.device;
+        const Buffers cb = buffers(C, "C");
+        out = cb.codes; scales = cb.scales; ldc = cb.ld; where = cb.device;
     } else {
         const Mat C = matrix(tensor(a[0], "C"), "C");
         if (C.rows != M || C.cols != N || C.dtype != (epi == KB_EPI_F32 || epi == KB_EPI_RESID ? KB_F32 : KB_F16)) refuse("C is [M, N] of its epilogue's type");
@@ -337,10 +402,10 @@ PyObject* py_linear4(PyObject* const* a, Py_ssize_t n) {           // C, A, W, e
         gate = static_cast<const float*>(g.data_ptr());
     }
     here.have(where, "C");
-    here.have(A.device, "A");
-    here.have(W.device, "W");
+    here.have(ab.device, "A");
+    here.have(wb.device, "W");
     const double alpha = std::ldexp(to_double(a[5]), A.exp + W.exp);
-    if (M) check(f_linear4(out, ldc, scales, ptr(A.codes_ptr), A.ld, ptr(A.scales_ptr), ptr(W.codes_ptr), W.ld, ptr(W.scales_ptr), M, N, K, A.fmt, epi, (float)alpha, gate,
+    if (M) check(f_linear4(out, ldc, scales, ab.codes, ab.ld, ab.scales, wb.codes, wb.ld, wb.scales, M, N, K, A.fmt, epi, (float)alpha, gate,
                            here.stream), "kb_linear4");
     return same(a[0]);
 }
@@ -354,7 +419,8 @@ PyObject* py_linear4_dx(PyObject* const* a, Py_ssize_t n) {        // dx, dy, W,
     const Here here;
     here.have(dx.device, "dx");
     here.have(dy.device, "dy");
-    here.have(W.device, "W");
+    const Buffers wb = buffers(W, "W");
+    here.have(wb.device, "W");
     if (!dy.rows) return same(a[0]);
     at::Tensor made;
     const bool given = a[3] != Py_None;
@@ -362,7 +428,7 @@ PyObject* py_linear4_dx(PyObject* const* a, Py_ssize_t n) {        // dx, dy, W,
     const at::Tensor& ws = given ? tensor(a[3], "workspace") : made;
     if (given) here.have(ws.is_cuda() ? (int)ws.get_device() : -1, "workspace");
     if (!ws.is_contiguous()) refuse("the workspace is contiguous");
-    check(f_linear4_dx(dx.p, dx.ld, dx.dtype, dy.p, dy.ld, ptr(W.codes_ptr), W.ld, ptr(W.scales_ptr), dy.rows, W.rows, W.cols, W.fmt, W.exp, ws.data_ptr(), ws.nbytes(),
+    check(f_linear4_dx(dx.p, dx.ld, dx.dtype, dy.p, dy.ld, wb.codes, wb.ld, wb.scales, dy.rows, W.rows, W.cols, W.fmt, W.exp, ws.data_ptr(), ws.nbytes(),
                        here.stream), "kb_linear4_dx");
     return same(a[0]);
 }

@@ -317,7 +317,9 @@ int kb_linear4(void* C, int ldc, void* C_scales, const void* A, int lda, const v
 
 /* The gradient of kb_linear4's input (A taken as the values that it was quantised from): dx [M, K] = dy [M, N] . W [N, K], dy fp16, dx fp16 or fp32.
  * W is decoded, transposed, to fp16 in the workspace (kb_linear4_dx_workspace_bytes(N, K), always required), then multiplied as kb_linear16 does.
- * N a multiple of 64, K of 8. Frozen weights have no gradient. */
+ * Those values leave out 2^exp, which the sums are multiplied with, so every exp that kb_quant4 takes is as good as 0. They are exact for KB_NV4, and for blocks of
+ * KB_MX4 whose scale lies in [2^-23, 2^13] (max |x| from 2^-21 up to 2^15); elements of other blocks round to fp16, at most 2^-25 off, or from 65520 on to
+ * infinity, and KB_STATUS_RANGE is set. N a multiple of 64, K of 8. Frozen weights have no gradient. */
 size_t kb_linear4_dx_workspace_bytes(int N, int K);
 int kb_linear4_dx(void* dx, int ld_dx, int out_dtype, const void* dy_f16, int ld_dy, const void* W, int ldw, const void* W_scales, int M, int N, int K, int fmt,
                   int exp, void* workspace, size_t workspace_bytes, void* stream);
@@ -356,7 +358,8 @@ int kb_lora_pack(void* dst_f16, int ld, int col0, const void* src_bf16, int rows
 
 /* Read and clear the device status word of the current device (synchronises the device).
  * *status_bits = 0 when every kernel since the last call finished normally; returns KB_ERR_TIMEOUT
- * when a kernel gave up on a bounded wait. */
+ * when a kernel gave up on a bounded wait. KB_STATUS_RANGE alone is no error: kb_linear4_dx rounded elements of a KB_MX4 weight, see there. */
+enum { KB_STATUS_TIMEOUT = 1, KB_STATUS_RANGE = 2 };
 int kb_status(unsigned* status_bits);
 
 /* Per-category kernel timing, the counterpart of the engine's ProfScope / prof_report

@@ -723,7 +723,7 @@ struct SecondProduct {
 // shared body of kb_linear16 (one weight matrix) and kb_linear16_qkv (three, one launch)
 int linear16_segments(void* const* C, int ldc, const void* A, int lda, const void* const* W, int ldw, int n_seg, int M, int N, int K, int epi,
                       const float* gate, const void* const* head_w, const int* rope_on, const float* rope_cos, const float* rope_sin,
-                      int rope_T, float eps, cudaStream_t stream, const SecondProduct& sp = SecondProduct()) {
+                      int rope_T, float eps, cudaStream_t stream, const SecondProduct& sp = SecondProduct(), float alpha = 1.f) {
     if (!A || M < 0 || N <= 0 || K <= 0 || n_seg < 1 || n_seg > 3) return KB_ERR_ARG;
     if (epi < KB_EPI_F32 || epi > KB_EPI_HEADS16) return KB_ERR_ARG;
     if ((rope_cos == nullptr) != (rope_sin == nullptr)) return KB_ERR_ARG;
@@ -778,6 +778,7 @@ int linear16_segments(void* const* C, int ldc, const void* A, int lda, const voi
     }
     p.C = C[0]; p.ldc = ldc; p.M = M; p.N = N; p.K = K;
     p.gate = gate;
+    p.alpha = alpha;
     p.rope_cos = rope_cos; p.rope_sin = rope_sin; p.rope_T = rope_T > 0 ? rope_T : 1; p.eps = eps;
     p.status = st->status;
     switch (epi) {
@@ -1117,6 +1118,26 @@ int launch_gemv4(const Gemv4Params& p, cudaStream_t stream) {
     return launch_dependent(gemv4_kernel<FMT>, grid, block, 0, stream, nullptr, p);
 }
 
+// kb_dequant4; tell: report a value that T does not hold (transposed, to fp16) to kb_status
+int dequant4(void* y, int ld_y, int out_dtype, const void* codes, int ld_codes, const void* scales, int rows, int cols, int fmt, int exp, int transpose, bool tell,
+             cudaStream_t stream) {
+    if (!y || rows < 0 || cols <= 0 || !valid_in_dtype(out_dtype) || !valid_q4(fmt, exp)) return KB_ERR_ARG;
+    if (cols > KB_MAX_Q4_COLS || rows > KB_MAX_Q4_ROWS || ld_y < (transpose ? rows : cols)) return KB_ERR_SHAPE;
+    if (reinterpret_cast<uintptr_t>(y) % elem_size(out_dtype)) return KB_ERR_ALIGN;
+    int rc;
+    if ((rc = check_q4(codes, ld_codes, scales, cols))) return rc;
+    DeviceState* st;
+    if ((rc = get_state(&st))) return rc;
+    if (rows == 0) return KB_OK;
+    Quant4Params p = {};
+    p.y = y; p.codes = static_cast<uint8_t*>(const_cast<void*>(codes)); p.scales = static_cast<uint8_t*>(const_cast<void*>(scales));
+    p.rows = rows; p.cols = cols; p.ld_x = ld_y; p.ld = ld_codes; p.pieces = q4_pieces(cols, fmt); p.exp = exp;
+    p.wide = wide_rows(y, ld_y, out_dtype);
+    p.status = tell ? st->status : nullptr;
+    ProfScope ps(st, KB_PROF_LINEAR, stream);
+    return fmt == KB_MX4 ? launch_dequant4<FMT_MX4>(p, out_dtype, transpose != 0, stream) : launch_dequant4<FMT_NV4>(p, out_dtype, transpose != 0, stream);
+}
+
 }  // namespace
 
 extern "C" {
@@ -1147,22 +1168,8 @@ int kb_quant4(void* codes, int ld_codes, void* scales, const void* x, int ld_x, 
 }
 
 int kb_dequant4(void* y, int ld_y, int out_dtype, const void* codes, int ld_codes, const void* scales, int rows, int cols, int fmt, int exp,
-                int transpose, void* stream_) {
-    cudaStream_t stream = static_cast<cudaStream_t>(stream_);
-    if (!y || rows < 0 || cols <= 0 || !valid_in_dtype(out_dtype) || !valid_q4(fmt, exp)) return KB_ERR_ARG;
-    if (cols > KB_MAX_Q4_COLS || rows > KB_MAX_Q4_ROWS || ld_y < (transpose ? rows : cols)) return KB_ERR_SHAPE;
-    if (reinterpret_cast<uintptr_t>(y) % elem_size(out_dtype)) return KB_ERR_ALIGN;
-    int rc;
-    if ((rc = check_q4(codes, ld_codes, scales, cols))) return rc;
-    DeviceState* st;
-    if ((rc = get_state(&st))) return rc;
-    if (rows == 0) return KB_OK;
-    Quant4Params p = {};
-    p.y = y; p.codes = static_cast<uint8_t*>(const_cast<void*>(codes)); p.scales = static_cast<uint8_t*>(const_cast<void*>(scales));
-    p.rows = rows; p.cols = cols; p.ld_x = ld_y; p.ld = ld_codes; p.pieces = q4_pieces(cols, fmt); p.exp = exp;
-    p.wide = wide_rows(y, ld_y, out_dtype);
-    ProfScope ps(st, KB_PROF_LINEAR, stream);
-    return fmt == KB_MX4 ? launch_dequant4<FMT_MX4>(p, out_dtype, transpose != 0, stream) : launch_dequant4<FMT_NV4>(p, out_dtype, transpose != 0, stream);
+                int transpose, void* stream) {
+    return dequant4(y, ld_y, out_dtype, codes, ld_codes, scales, rows, cols, fmt, exp, transpose, false, static_cast<cudaStream_t>(stream));
 }
 
 int kb_linear4(void* C, int ldc, void* C_scales, const void* A, int lda, const void* A_scales, const void* W, int ldw, const void* W_scales, int M,
@@ -1216,14 +1223,15 @@ int kb_linear4_dx(void* dx, int ld_dx, int out_dtype, const void* dy_f16, int ld
     if (M == 0) return KB_OK;
     if (!workspace || workspace_bytes < kb_linear4_dx_workspace_bytes(N, K)) return KB_ERR_WORKSPACE;
     if (!aligned16(workspace)) return KB_ERR_ALIGN;
-    // the transposed weight in fp16 (4-bit values with their scales are fp16 numbers, see the header), then the fp16 product
-    if ((rc = kb_dequant4(workspace, N, KB_F16, W, ldw, W_scales, N, K, fmt, exp, 1, stream_))) return rc;
+    // The transposed weight in fp16, then the fp16 product, whose sums take 2^exp. Without it NV4 numbers lie in 2^-10 ... 2688, multiples of 2^-10 with six
+    // significant bits, so every one is an fp16 number. Of MX4 those of scales from 2^-23 to 2^13 are; others round, and kb_status says so.
+    if ((rc = dequant4(workspace, N, KB_F16, W, ldw, W_scales, N, K, fmt, 0, 1, true, stream))) return rc;
     void* const cs[1] = {dx};
     const void* const ws[1] = {workspace};
     const void* const hw[1] = {nullptr};
     const int rope_on[1] = {0};
     return linear16_segments(cs, ld_dx, dy_f16, ld_dy, ws, N, 1, M, K, N, out_dtype == KB_F32 ? KB_EPI_F32 : KB_EPI_F16, nullptr, hw, rope_on, nullptr, nullptr,
-                             0, 0.f, stream);
+                             0, 0.f, stream, SecondProduct(), ldexpf(1.f, exp));
 }
 
 // ------------------------------------------------------------------------------------------- rotary positions, dropout

@@ -103,7 +103,7 @@ constexpr int attn_smem(int mode) { return mode == MODE_PAIR ? ATTN_SMEM_PAIR : 
 static_assert(ATTN_SMEM_NAG <= 232448, "shared memory per thread block on sm_100");
 
 // error bits written to the status word
-constexpr uint32_t ST_TIMEOUT = 1u;
+constexpr uint32_t ST_TIMEOUT = 1u, ST_RANGE = 2u;
 
 constexpr int MAX_PEERS = 8;
 

@@ -72,6 +72,7 @@ struct GemmParams {
     // belongs to segment tn / tiles_n_seg, which has its own W and C tensor maps and its own head epilogue settings.
     int tiles_n_seg;               // column tiles per segment (= tiles_n for a single matrix)
     const float* gate;             // EPI_RESID: C[r, c] += gate[c] * acc (null = 1)
+    float alpha;                   // EPI_F32, EPI_F16: C = alpha * acc, the power of two of a 4-bit weight whose operand here is without it; else 1
     const __nv_bfloat16* head_w[3];   // EPI_HEADS16: RMSNorm weight[128] of the segment, or null
     int rope_on[3];                // EPI_HEADS16: the segment's heads are rotated (tables below)
     const float* rope_cos;         // EPI_HEADS16: tables [rope_T, 64] or null; row r uses table row r % rope_T
@@ -424,6 +425,12 @@ gemm16_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ G
                         if (lane == 0) {
                             if (PAIR && rank != 0) mbar_arrive_cluster(mapa_u32(bar(GBAR_ACC_EMPTY + buf), lead));
                             else mbar_arrive(bar(GBAR_ACC_EMPTY + buf));
+                        }
+                    }
+                    if constexpr (EPI == EPI_F32 || EPI == EPI_F16) {
+                        if (p.alpha != 1.f) {
+#pragma unroll
+                            for (int c = 0; c < CW; c++) v[c] *= p.alpha;
                         }
                     }
                     if constexpr (EPI == EPI_GELU16) {

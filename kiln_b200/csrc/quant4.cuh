@@ -15,6 +15,7 @@
 #include <cuda_fp16.h>
 #include <stdint.h>
 
+#include "attn_sm100.cuh"   // ST_RANGE
 #include "prep.cuh"   // Io
 #include "ptx.cuh"
 
@@ -176,6 +177,7 @@ struct Quant4Params {
     int pieces;                  // of a row block
     int exp;
     bool wide;
+    uint32_t* status;            // dequant transposed to fp16: set ST_RANGE where a value is not one of fp16's (null: not asked)
 };
 
 // A lane takes eight columns, so that a block is two (NV4) or four (MX4) lanes, which meet by shuffles; a warp 256 columns side by side, SEGS times, its loads
@@ -335,12 +337,15 @@ dequant4_t_kernel(const Quant4Params p) {
     const float up = pow2f(p.exp);
     uint2 codes[2];
     uint32_t scale[2];
+    bool rounded = false;
 #pragma unroll
     for (int i = 0; i < 2; i++) {
         const int r = r0 + 2 * pair + i, b = c / q4_block(FMT);
         const bool in = r < p.rows && c < p.cols;
         codes[i] = in ? *reinterpret_cast<const uint2*>(p.codes + (size_t)r * p.ld + (c >> 1)) : make_uint2(0u, 0u);
         scale[i] = in ? p.scales[q4_scale_at(r, b >> 2, p.pieces) + (b & 3)] : 0u;
+        // a half of the scale down to 2^-24, six of it up to 49152; a NaN is one of fp16 as well, and zeros are whatever their scale
+        rounded |= FMT == FMT_MX4 && (scale[i] < 127u - 23u || scale[i] > 127u + 13u) && scale[i] != 255u && ((codes[i].x | codes[i].y) & 0x77777777u) != 0u;
     }
 #pragma unroll
     for (int h = 0; h < 2; h++) {
@@ -351,7 +356,9 @@ dequant4_t_kernel(const Quant4Params p) {
             *reinterpret_cast<Two*>(&tile[(16 * kg + 8 * h + e) * Q4_TILE_LD + 2 * pair]) = two;
         }
     }
-    __syncthreads();
+    if (std::is_same<T, __half>::value && FMT == FMT_MX4 && p.status) {
+        if (__syncthreads_or(rounded) && threadIdx.x == 0) atomicOr(p.status, ST_RANGE);
+    } else __syncthreads();
     if (!p.wide) {
         for (int i = threadIdx.x; i < Q4_TILE_C * Q4_TILE_R; i += 256) {
             const int k = i / Q4_TILE_R, n = i % Q4_TILE_R;

@@ -9,6 +9,7 @@ import ctypes
 import os
 
 KB_F16, KB_BF16, KB_F32 = 0, 1, 2
+STATUS_RANGE = 2
 
 _PKG = os.path.dirname(os.path.abspath(__file__))
 _LIB_PATH = os.environ.get("KILN_B200_LIB") or os.path.join(_PKG, "lib", "libkiln_b200.so")   # override: an alternative build of the same ABI
@@ -403,7 +404,8 @@ def linear4(C, A, W, epi, gate=None, alpha=1.0):
 
 
 def linear4_dx(dx, dy, W, workspace=None):
-    """dx [M, K] (fp16 or fp32) = dy [M, N] @ W for a 4-bit W [N, K]: the gradient of linear4's input. dy fp16. workspace: 2 N K bytes, made here if None."""
+    """dx [M, K] (fp16 or fp32) = dy [M, N] @ W for a 4-bit W [N, K]: the gradient of linear4's input. dy fp16. workspace: 2 N K bytes, made here if None.
+    W's power of two may be any; blocks of an MX4 weight with a scale outside [2^-23, 2^13] round to fp16, which check_status tells (STATUS_RANGE)."""
     return (_binding or _b()).linear4_dx(dx, dy, W, workspace)
 
 
@@ -432,7 +434,8 @@ def dropout(out, x, rng, p, resid=None):
 
 
 def check_status():
-    """Synchronise and raise if any kernel since the last call gave up on a bounded wait."""
+    """Synchronise and raise if any kernel since the last call gave up on a bounded wait. Returns the other status bits: STATUS_RANGE where linear4_dx has
+    rounded elements of an MX4 weight to fp16 (see there)."""
     bits = ctypes.c_uint(0)
     _check(lib().kb_status(ctypes.byref(bits)), "kb_status")
     return bits.value

@@ -86,6 +86,9 @@ __device__ __forceinline__ void rope_sines(const RopeParams& p, float2* cs, unsi
         at[r * stride] = make_float2(cn * p.amplitude, (p.inverse ? -sn : sn) * p.amplitude);
     }
 }
+// A pair turned, written out down to which product the sum is fused with, so that pieces and elements give the same bits whatever stands around them
+__device__ __forceinline__ float rope_a(float a, float b, float2 z) { return fmaf(a, z.x, -__fmul_rn(b, z.y)); }
+__device__ __forceinline__ float rope_b(float a, float b, float2 z) { return fmaf(a, z.y, __fmul_rn(b, z.x)); }
 // where head v of a row lies
 template <typename T>
 __device__ __forceinline__ void rope_head(const RopeParams& p, unsigned row, int v, const T*& src, T*& dst) {
@@ -148,12 +151,10 @@ rope_kernel(const __grid_constant__ RopeParams p) {
         rope_sines(p, cs, row0, rows, stride, EACH, un.turned);
         __syncthreads();
         if (!at.busy) return;
+        const int mine = HALF ? EACH : pairs - EACH * s;       // pairs of the unit that turn: interleaved, the last one that turns may hold others, which are copied
         float2 z[EACH];
 #pragma unroll
-        for (int e = 0; e < EACH; e++) {
-            const bool in = turns && (HALF || EACH * s + e < pairs);   // interleaved: the last unit that turns may hold pairs that do not
-            z[e] = in ? cs[r * stride + e * un.turned + s] : make_float2(1.f, 0.f);
-        }
+        for (int e = 0; e < EACH; e++) z[e] = turns && e < mine ? cs[r * stride + e * un.turned + s] : make_float2(1.f, 0.f);
         while (true) {
 #pragma unroll
             for (int i = 0; i < U; i++) {
@@ -165,16 +166,16 @@ rope_kernel(const __grid_constant__ RopeParams p) {
 #pragma unroll
                     for (int e = 0; e < 8; e++) {
                         const float t = x.v[e];
-                        x.v[e] = t * z[e].x - y.v[e] * z[e].y;
-                        y.v[e] = y.v[e] * z[e].x + t * z[e].y;
+                        x.v[e] = rope_a(t, y.v[e], z[e]);
+                        y.v[e] = rope_b(t, y.v[e], z[e]);
                     }
                     Io<T>::st8(dst[i] + cb, y);
                 } else {
 #pragma unroll
                     for (int e = 0; e < 4; e++) {
                         const float t = x.v[2 * e], u = x.v[2 * e + 1];
-                        x.v[2 * e] = t * z[e].x - u * z[e].y;
-                        x.v[2 * e + 1] = u * z[e].x + t * z[e].y;
+                        x.v[2 * e] = e < mine ? rope_a(t, u, z[e]) : t;
+                        x.v[2 * e + 1] = e < mine ? rope_b(t, u, z[e]) : u;
                     }
                 }
                 Io<T>::st8(dst[i] + ca, x);
@@ -195,8 +196,8 @@ rope_kernel(const __grid_constant__ RopeParams p) {
                 const int ia = HALF ? s : 2 * s, ib = HALF ? pairs + s : 2 * s + 1;
                 const float2 z = cs[s];
                 const float x = to_f32(src[ia]), y = to_f32(src[ib]);
-                dst[ia] = from_f32<T>(x * z.x - y * z.y);
-                dst[ib] = from_f32<T>(y * z.x + x * z.y);
+                dst[ia] = from_f32<T>(rope_a(x, y, z));
+                dst[ib] = from_f32<T>(rope_b(x, y, z));
             }
             for (int c = p.rot + lane; c < p.dim; c += 32) dst[c] = src[c];
         }
@@ -261,7 +262,7 @@ rope_shifted_kernel(const __grid_constant__ RopeParams p) {
                 const T* const from = own - pairs;
 #pragma unroll
                 for (int e = 0; e < 8; e++) {                             // a partner lies in the head whatever e; it is taken where e turns
-                    const float y = to_f32((e < low ? to : from)[e]), t = x.v[e] * z[e].x + y * z[e].y;
+                    const float y = to_f32((e < low ? to : from)[e]), t = fmaf(x.v[e], z[e].x, __fmul_rn(y, z[e].y));
                     x.v[e] = e < left ? t : x.v[e];
                 }
             }

@@ -6,10 +6,13 @@ nvcc cross-compiles without a GPU. The library links the CUDA runtime statically
 one driver entry point it needs (cuTensorMapEncodeTiled) at run time, so it loads on a machine
 without a driver; every launch entry point then fails with KB_ERR_DEVICE.
 """
+import importlib.util
 import os
+import re
 import shutil
 import subprocess
 import sys
+import sysconfig
 
 PKG = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(PKG, "csrc")
@@ -43,10 +46,14 @@ def build(force=False, verbose=False, defines=(), out=None):
     out = out or LIB
     os.makedirs(os.path.dirname(out), exist_ok=True)
     deps = _sources([CSRC, INCLUDE], (".cu", ".cuh", ".h"))
+    if force or _stale(out, deps):
+        _compile(out, verbose, defines)
     if out == LIB:
         build_binding()                            # ops.py binds some of the library's calls with it
-    if not force and not _stale(out, deps):
-        return out
+    return out
+
+
+def _compile(out, verbose, defines):
     cmd = ["nvcc"] + NVCC_FLAGS + (["-Xptxas", "-v"] if verbose else []) + ["-D" + d for d in defines] + \
           ["-o", out, os.path.join(CSRC, "abi.cu")]
     r = subprocess.run(cmd, capture_output=True, text=True)
@@ -54,7 +61,6 @@ def build(force=False, verbose=False, defines=(), out=None):
         sys.stderr.write(r.stderr)
     if r.returncode != 0:
         raise RuntimeError("nvcc failed:\n" + r.stderr[-6000:])
-    return out
 
 
 def build_host(force=False):
@@ -71,18 +77,34 @@ def build_host(force=False):
     return HOST_LIB
 
 
+def torch_tag(torch_dir):
+    """What the binding is compiled for: it takes the layout of torch's and Python's structures from their headers."""
+    with open(os.path.join(torch_dir, "version.py")) as f:
+        version = re.search(r"^__version__\s*=\s*['\"]([^'\"]+)", f.read(), flags=re.M).group(1)
+    return f"torch {version}, {sysconfig.get_config_var('SOABI')}"
+
+
+def _built_for(path, tag):
+    with open(path, "rb") as f:
+        return f"[{tag}]".encode() in f.read()
+
+
 def build_binding(force=False):
-    """Compile the binding of the 4-bit, rotary and dropout calls for torch tensors (a CPython module, no device code); returns its path."""
-    import importlib.util
-    import sysconfig
+    """Compile the binding of the 4-bit, rotary and dropout calls for torch tensors (a CPython module, no device code); returns its path, or None where
+    there is no torch: the library and the C++ shim need none, and without the binding those calls of ops.py refuse."""
+    spec = importlib.util.find_spec("torch")
+    if spec is None or not spec.origin:
+        sys.stderr.write("kiln_b200: no torch here, so its binding is not built\n")
+        return None
     src = os.path.join(PKG, "host", "torch_binding.cpp")
-    if not force and not _stale(BINDING, [src, os.path.join(INCLUDE, "kiln_b200.h")]):
+    torch_dir = os.path.dirname(spec.origin)
+    tag = torch_tag(torch_dir)
+    if not force and not _stale(BINDING, [src, os.path.join(INCLUDE, "kiln_b200.h")]) and _built_for(BINDING, tag):
         return BINDING
-    os.makedirs(LIB_DIR, exist_ok=True)
-    torch_dir = os.path.dirname(importlib.util.find_spec("torch").origin)
+    os.makedirs(os.path.dirname(BINDING), exist_ok=True)
     inc = os.path.join(torch_dir, "include")
     cuda = os.path.dirname(os.path.dirname(shutil.which("nvcc") or "/usr/local/cuda/bin/nvcc"))
-    cmd = ["g++", "-O2", "-std=c++17", "-fPIC", "-shared", "-w", "-I" + inc, "-I" + os.path.join(inc, "torch", "csrc", "api", "include"),
+    cmd = ["g++", "-O2", "-std=c++17", "-fPIC", "-shared", "-w", f'-DKB_BUILT_FOR="{tag}"', "-I" + inc, "-I" + os.path.join(inc, "torch", "csrc", "api", "include"),
            "-I" + os.path.join(cuda, "include"), "-I" + sysconfig.get_paths()["include"], "-o", BINDING + ".new", src, "-L" + os.path.join(torch_dir, "lib"),
            "-lc10", "-lc10_cuda", "-ltorch_cpu", "-ltorch_python"]
     r = subprocess.run(cmd, capture_output=True, text=True)
@@ -96,4 +118,5 @@ if __name__ == "__main__":
     print(build(force="--force" in sys.argv, verbose="--verbose" in sys.argv))
     if os.path.exists(os.path.join(PKG, "host", "gpu_ops.cpp")):
         print(build_host(force="--force" in sys.argv))
-    print(build_binding(force="--force" in sys.argv))
+    if build_binding(force="--force" in sys.argv):
+        print(BINDING)

@@ -547,6 +547,9 @@ PyMODINIT_FUNC PyInit__kiln_torch() {
     PyObject* m = PyModule_Create(&module_def);
     if (!m) return nullptr;
     quant4_type = reinterpret_cast<PyTypeObject*>(PyType_FromSpec(&quant4_spec));
+    // in brackets in the file as well, where the build looks for it
+    static const char built_for[] = "[" KB_BUILT_FOR "]";
+    if (PyModule_AddObject(m, "built_for", PyUnicode_FromStringAndSize(built_for + 1, sizeof(built_for) - 3)) < 0) { Py_DECREF(m); return nullptr; }
     if (!quant4_type || PyModule_AddObjectRef(m, "Quant4", reinterpret_cast<PyObject*>(quant4_type)) < 0) { Py_DECREF(m); return nullptr; }
     return m;
 }

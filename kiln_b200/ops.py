@@ -354,13 +354,17 @@ def _b():
     if _binding is None:
         import importlib.machinery
         import importlib.util
-        import torch                                   # noqa: F401  (its libraries, which the module links against)
+        import torch                                   # its libraries, which the module links against
         L = lib()
         if not os.path.exists(_BINDING_PATH):
             raise FileNotFoundError(f"{_BINDING_PATH} is missing: run `python -m kiln_b200.build`")
         loader = importlib.machinery.ExtensionFileLoader("_kiln_torch", _BINDING_PATH)
         m = importlib.util.module_from_spec(importlib.util.spec_from_loader("_kiln_torch", loader))
         loader.exec_module(m)
+        from .build import torch_tag
+        here = torch_tag(os.path.dirname(torch.__file__))
+        if m.built_for != here:
+            raise ImportError(f"{_BINDING_PATH} was built for {m.built_for} and this is {here}: run `python -m kiln_b200.build`")
         m.bind(KilnError, *[ctypes.cast(f, ctypes.c_void_p).value for f in (L.kb_quant4, L.kb_dequant4, L.kb_linear4, L.kb_linear4_dx, L.kb_rope, L.kb_dropout)])
         _binding = m
     return _binding

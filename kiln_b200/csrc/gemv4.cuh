@@ -42,6 +42,15 @@ __device__ __forceinline__ float2 gv4_scales(uint32_t word, int chunk) {
 }
 __device__ __forceinline__ __half2 gv4_h2(uint32_t v) { return *reinterpret_cast<const __half2*>(&v); }
 
+// acc + sa sw sum. The product of two of NV4's scales lies in 2^-18 ... 2^18. Of MX4's it may leave fp32 where the term does not (the block's sum may be 0): scales
+// on the same side of 1 are therefore multiplied with one after the other, so that what overflows or vanishes on the way does so in the term as well.
+template <int FMT>
+__device__ __forceinline__ float gv4_add(float sa, float sw, float sum, float acc) {
+    if (FMT == FMT_NV4) return fmaf(sa * sw, sum, acc);
+    const bool apart = (sa < 1.f) == (sw < 1.f);
+    return fmaf(apart ? sw : sa * sw, apart ? sum * sa : sum, acc);
+}
+
 template <int FMT>
 __global__ void __launch_bounds__(32 * GV4_WARPS)
 gemv4_kernel(const Gemv4Params p) {
@@ -87,7 +96,7 @@ gemv4_kernel(const Gemv4Params p) {
                 for (int i = 1; i < 8; i++) s = __hfma2(gv4_h2(a[i]), gv4_h2(w[i]), s);
                 const float2 f = __half22float2(s), fw = gv4_scales<FMT>(sws[j], c);
                 // exact but for the sum: 8 bits of scales, 12 of the block. Rows that do not exist may have scales of anything
-                if (j < real) acc[j] = fmaf((b ? fa.y : fa.x) * (b ? fw.y : fw.x), f.x + f.y, acc[j]);
+                if (j < real) acc[j] = gv4_add<FMT>(b ? fa.y : fa.x, b ? fw.y : fw.x, f.x + f.y, acc[j]);
             }
         }
     }

@@ -193,6 +193,10 @@ void pack4(uint8_t* codes, uint8_t* scales, const void* w, int dtype, int rows, 
 
 namespace {
 size_t bytes4(int rows, int cols, int fmt) { return align256((size_t)rows * row_bytes4(cols)) + align256(scale_bytes4(rows, cols, fmt)); }
+// what kb_quant4 makes; kb_linear4 has only the factor of both sides
+void check_exp(const Weight4& W, const char* what) {
+    if (W.fmt == KB_MX4 ? W.exp != 0 : W.exp < -64 || W.exp > 64) throw std::runtime_error(std::string(what) + ": a power of two that no 4-bit weight has");
+}
 // room of a 4-bit matrix at `at` of the context's workspace
 Weight4 scratch4(int rows, int cols, int fmt, size_t at, const char* what) {
     if (!g_ctx.workspace || g_ctx.workspace_bytes < at + bytes4(rows, cols, fmt)) throw std::runtime_error(std::string(what) + ": the workspace is too small for the 4-bit activations");
@@ -218,12 +222,15 @@ size_t linear4_workspace(int T, int in, int fmt) { return bytes4(T, in, fmt); }
 size_t mlp4_workspace(int T, int in, int hidden, int fmt) { return bytes4(T, in, fmt) + bytes4(T, hidden, fmt); }
 
 void linear4(void* y, int ldy, const __half* x16, int T, const Weight4& W, Epi16 epi, const float* gate) {
+    check_exp(W, "linear4");
     if (T == 0) return;
     product4(y, ldy, nullptr, activations4(x16, T, W.cols, W.fmt, 0, "linear4"), W, (int)epi, gate, "linear4");
 }
 
 void mlp4(float* y, int ldy, const __half* x16, int T, const Weight4& up, const Weight4& down, const float* gate) {
     if (down.cols != up.rows || down.fmt != up.fmt) throw std::runtime_error("mlp4: the two weights do not follow one another");
+    check_exp(up, "mlp4");
+    check_exp(down, "mlp4");
     if (T == 0) return;
     const Weight4 h = scratch4(T, up.rows, up.fmt, bytes4(T, up.cols, up.fmt), "mlp4");
     product4(const_cast<uint8_t*>(h.codes), (int)row_bytes4(h.cols), const_cast<uint8_t*>(h.scales), activations4(x16, T, up.cols, up.fmt, 0, "mlp4"), up, KB_EPI_GELU4, nullptr,

@@ -16,6 +16,7 @@
 #include <torch/csrc/Dtype.h>
 #include <torch/csrc/autograd/python_variable.h>
 
+#include <cmath>
 #include <cstdarg>
 #include <limits>
 #include <string>
@@ -135,6 +136,12 @@ int64_t scale_bytes(int rows, int cols, int fmt) {
 void check_size(int rows, int cols, int fmt) {
     if (rows < 0 || rows > KB_MAX_Q4_ROWS || cols <= 0 || cols > KB_MAX_Q4_COLS || (fmt != KB_MX4 && fmt != KB_NV4)) refuse("no 4-bit matrix of %d x %d, format %d", rows, cols, fmt);
 }
+// The power of two of a whole matrix. quant4 takes 0 alone for MX4, but a product may carry one, and every product takes what a handle holds.
+constexpr int MOST_EXP = 64;
+int check_exp(int exp) {
+    if (exp < -MOST_EXP || exp > MOST_EXP) refuse("exp lies between %d and %d, not %d", -MOST_EXP, MOST_EXP, exp);
+    return exp;
+}
 
 // Where a matrix lies. A tensor can be given another memory at any time (`codes.data = ...`, which is what moving a parameter to another device does, or
 // storage().resize_()), so this is asked for in every call and kept by none.
@@ -195,6 +202,7 @@ Quant4* new_quant4() {
 
 Quant4* make_quant4(int rows, int cols, int fmt, int exp, const at::Device& device) {
     check_size(rows, cols, fmt);
+    check_exp(exp);
     const int64_t codes = (int64_t)rows * row_bytes(cols);
     at::Tensor both = new_bytes(codes + scale_bytes(rows, cols, fmt), device);
     Quant4* q = new_quant4();
@@ -230,6 +238,7 @@ int quant4_init(PyObject* self, PyObject* args, PyObject* kwargs) {
     if (!PyArg_ParseTupleAndKeywords(args, kwargs, "OOiii|i", const_cast<char**>(names), &codes_o, &scales_o, &rows, &cols, &fmt, &exp)) return -1;
     try {
         check_size(rows, cols, fmt);
+        check_exp(exp);
         tensor(codes_o, "codes");
         tensor(scales_o, "scales");
         Quant4 fresh = {};                              // looked over before `self` changes
@@ -294,15 +303,26 @@ PyObject* get_where(PyObject* self, void* what) {
     return nullptr;
 }
 
+PyObject* get_exp(PyObject* self, void*) { return PyLong_FromLong(reinterpret_cast<Quant4*>(self)->exp); }
+int set_exp(PyObject* self, PyObject* value, void*) {
+    try {
+        if (!value) refuse("exp cannot be deleted");
+        reinterpret_cast<Quant4*>(self)->exp = check_exp(to_int(value));
+        return 0;
+    } catch (const Refused&) {
+        return -1;
+    }
+}
+
 PyMemberDef quant4_members[] = {
     {"rows", T_INT, offsetof(Quant4, rows), READONLY, nullptr},
     {"cols", T_INT, offsetof(Quant4, cols), READONLY, nullptr},
     {"fmt", T_INT, offsetof(Quant4, fmt), READONLY, "MX4 or NV4"},
-    {"exp", T_INT, offsetof(Quant4, exp), 0, "the whole matrix is times 2^exp"},
     {nullptr, 0, 0, 0, nullptr}};
 PyGetSetDef quant4_getset[] = {
     {"codes", get_codes, nullptr, "uint8 [rows, ld]", nullptr},
     {"scales", get_scales, nullptr, "uint8, flat", nullptr},
+    {"exp", get_exp, set_exp, "the whole matrix is times 2^exp", nullptr},
     {"ld", get_where, nullptr, "bytes from a row of codes to the next", (void*)(intptr_t)WHERE_LD},
     {"device", get_where, nullptr, "index of the GPU, -1 for the CPU", (void*)(intptr_t)WHERE_DEVICE},
     {"codes_ptr", get_where, nullptr, "where the codes lie now", (void*)(intptr_t)WHERE_CODES},
@@ -310,7 +330,8 @@ PyGetSetDef quant4_getset[] = {
     {nullptr, nullptr, nullptr, nullptr, nullptr}};
 PyType_Slot quant4_slots[] = {
     {Py_tp_doc, const_cast<char*>("Quant4(codes, scales, rows, cols, fmt, exp=0): a matrix [rows, cols] of 4-bit numbers in blocks (kb_quant4): codes uint8 [rows, >= 16 ceil(cols / 32)], "
-                                  "scales uint8, fmt MX4 or NV4, all of it times 2^exp.")},
+                                  "scales uint8, fmt MX4 or NV4, all of it times 2^exp, exp from -64 to 64. quant4 makes MX4 matrices with 0 alone; "
+                                  "another one counts in products, and dequant4 and linear4_dx refuse it.")},
     {Py_tp_init, (void*)quant4_init}, {Py_tp_new, (void*)PyType_GenericNew}, {Py_tp_dealloc, (void*)quant4_dealloc},
     {Py_tp_members, quant4_members}, {Py_tp_getset, quant4_getset}, {0, nullptr}};
 PyType_Spec quant4_spec = {"kiln_b200.ops.Quant4", sizeof(Quant4), 0, Py_TPFLAGS_DEFAULT, quant4_slots};
@@ -405,6 +426,8 @@ PyObject* py_linear4(PyObject* const* a, Py_ssize_t n) {           // C, A, W, e
     here.have(ab.device, "A");
     here.have(wb.device, "W");
     const double alpha = std::ldexp(to_double(a[5]), A.exp + W.exp);
+    // within a rounding of 32 bits, which infinities, NaN and what vanishes are not
+    if (!(std::fabs((double)(float)alpha - alpha) <= 0x1p-24 * std::fabs(alpha))) refuse("alpha and both powers of two make a factor that 32 bits do not hold");
     if (M) check(f_linear4(out, ldc, scales, ab.codes, ab.ld, ab.scales, wb.codes, wb.ld, wb.scales, M, N, K, A.fmt, epi, (float)alpha, gate,
                            here.stream), "kb_linear4");
     return same(a[0]);

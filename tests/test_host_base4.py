@@ -100,3 +100,15 @@ def test_rope_and_dropout_match_the_calls(shim):
     y = torch.empty_like(x)
     assert _call(shim.kbh_lora_dropout, P(y), P(x), 40, 96, 0.2, P(rng)) == (0, "")
     assert torch.equal(y, ops.dropout(torch.empty_like(x), x, rng, 0.2))
+
+
+def test_powers_of_two_that_no_weight_has(shim):
+    """Refused before anything runs, by the product as by the gradient."""
+    buf = (ctypes.c_char * 65536)()
+    a = (ctypes.addressof(buf) + 255) & ~255
+    shim.kbh_set_context(None, a, 32768)
+    for fmt, exp in ((0, 1), (0, -1), (1, 65), (1, -65), (1, 1000)):
+        for what in (1, 5):
+            rc, msg = _call(shim.kbh_base4, a, 64, a, 4, a, a, 64, 64, None, None, 0, fmt, exp, what, None)
+            assert rc == -1 and "linear4" in msg and ("power of two" in msg or what == 5)
+    shim.kbh_set_context(None, None, 0)

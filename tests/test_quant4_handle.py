@@ -94,3 +94,39 @@ def test_a_weight_moved_off_the_gpu_and_back(built_lib):
     assert W.device == 0 and torch.equal(run(), want) and W.codes_ptr == codes.data_ptr() and held.numel()
     y = ops.dequant4(torch.empty(40, 256, device="cuda"), W)
     assert torch.equal(y, ops.dequant4(torch.empty(40, 256, device="cuda"), made))
+
+
+def test_powers_of_two(built_lib):
+    """-64 to 64 wherever a handle is made or changed; a factor of a product that 32 bits do not hold is refused."""
+    from kiln_b200 import ops
+    codes, scales, q = _made(fmt=NV4)
+    for good in (-64, 0, 64):
+        assert ops.Quant4(codes, scales, 4, 64, NV4, good).exp == good == ops.quant4_empty(4, 64, NV4, "cpu", good).exp
+        q.exp = good
+        assert q.exp == good
+    for bad in (-65, 65, 1000, -2 ** 31, 2 ** 40):
+        for make in (lambda: ops.Quant4(codes, scales, 4, 64, NV4, bad), lambda: ops.quant4_empty(4, 64, NV4, "cpu", bad), lambda: setattr(q, "exp", bad)):
+            with pytest.raises((ValueError, OverflowError)):
+                make()
+    with pytest.raises(TypeError):
+        q.exp = 1.5
+    with pytest.raises(ValueError):
+        del q.exp
+    assert q.exp == 64
+
+
+@gpu
+def test_factors_of_a_product(built_lib):
+    from kiln_b200 import ops
+    A, W = ops.quant4(torch.ones(3, 64).cuda(), NV4), ops.quant4(torch.ones(8, 64).cuda(), NV4)
+    run = lambda alpha=1.0: ops.linear4(torch.empty(3, 8, device="cuda"), A, W, ops.EPI_F32, alpha=alpha)
+    plain = run()
+    for ea, ew, alpha in [(64, 64, 2.0 ** -10), (-64, -64, 1.0), (64, -64, 1.0), (-64, -63, 2.0 ** 127)]:
+        A.exp, W.exp = ea, ew
+        assert torch.equal(run(alpha).double(), (plain.double() * 2.0 ** (ea + ew) * alpha).float().double())
+    for ea, ew, alpha in [(64, 64, 1.0), (64, 64, -4.0), (-64, -64, 1e-30), (0, 0, float("nan")), (0, 0, float("inf")), (0, 0, 1e300), (-64, -64, 1.0 / 3)]:
+        A.exp, W.exp = ea, ew
+        with pytest.raises(ValueError):
+            run(alpha)
+    A.exp = W.exp = 0
+    assert torch.equal(run(0.0), torch.zeros_like(plain))

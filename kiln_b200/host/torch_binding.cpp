@@ -286,6 +286,16 @@ PyObject* view_of(Quant4* q, PyObject** slot, bool scales) {
 }
 PyObject* get_codes(PyObject* self, void*) { Quant4* q = reinterpret_cast<Quant4*>(self); return view_of(q, &q->codes, false); }
 PyObject* get_scales(PyObject* self, void*) { Quant4* q = reinterpret_cast<Quant4*>(self); return view_of(q, &q->scales, true); }
+// copy, deepcopy and pickle: the type's own arguments
+PyObject* quant4_reduce(PyObject* self, PyObject*) {
+    const Quant4* q = reinterpret_cast<Quant4*>(self);
+    PyObject *codes = get_codes(self, nullptr), *scales = codes ? get_scales(self, nullptr) : nullptr;
+    PyObject* made = scales ? Py_BuildValue("O(OOiiii)", reinterpret_cast<PyObject*>(Py_TYPE(self)), codes, scales, q->rows, q->cols, q->fmt, q->exp) : nullptr;
+    Py_XDECREF(codes);
+    Py_XDECREF(scales);
+    return made;
+}
+PyMethodDef quant4_methods[] = {{"__reduce__", quant4_reduce, METH_NOARGS, nullptr}, {nullptr, nullptr, 0, nullptr}};
 enum { WHERE_CODES, WHERE_SCALES, WHERE_LD, WHERE_DEVICE };
 PyObject* get_where(PyObject* self, void* what) {
     try {
@@ -333,7 +343,7 @@ PyType_Slot quant4_slots[] = {
                                   "scales uint8, fmt MX4 or NV4, all of it times 2^exp, exp from -64 to 64. quant4 makes MX4 matrices with 0 alone; "
                                   "another one counts in products, and dequant4 and linear4_dx refuse it.")},
     {Py_tp_init, (void*)quant4_init}, {Py_tp_new, (void*)PyType_GenericNew}, {Py_tp_dealloc, (void*)quant4_dealloc},
-    {Py_tp_members, quant4_members}, {Py_tp_getset, quant4_getset}, {0, nullptr}};
+    {Py_tp_members, quant4_members}, {Py_tp_methods, quant4_methods}, {Py_tp_getset, quant4_getset}, {0, nullptr}};
 PyType_Spec quant4_spec = {"kiln_b200.ops.Quant4", sizeof(Quant4), 0, Py_TPFLAGS_DEFAULT, quant4_slots};
 
 inline void* ptr(unsigned long long p) { return reinterpret_cast<void*>((uintptr_t)p); }

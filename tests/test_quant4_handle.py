@@ -130,3 +130,30 @@ def test_factors_of_a_product(built_lib):
             run(alpha)
     A.exp = W.exp = 0
     assert torch.equal(run(0.0), torch.zeros_like(plain))
+
+
+def test_copies_and_pickles(built_lib):
+    """A copy shares the buffers, a deep copy and a pickled one have their own; a module with a 4-bit weight can be copied and saved."""
+    import copy
+    import io
+    import pickle
+    from kiln_b200 import ops
+    made = ops.quant4_empty(5, 70, NV4, "cpu", -7)
+    made.codes.copy_(torch.arange(5 * 48).view(5, 48) % 256)
+    made.scales.copy_(torch.arange(1024) % 120)
+    wide = torch.zeros(6, 100, dtype=torch.uint8)
+    own = ops.Quant4(wide[:, :64], torch.zeros(600, dtype=torch.uint8), 5, 70, MX4)
+    for q in (made, own, ops.quant4_empty(0, 70, MX4, "cpu")):
+        same = copy.copy(q)
+        assert same.codes.data_ptr() == q.codes.data_ptr() and same.scales.data_ptr() == q.scales.data_ptr()
+        for other in (same, copy.deepcopy(q), pickle.loads(pickle.dumps(q))):
+            assert (other.rows, other.cols, other.fmt, other.exp) == (q.rows, q.cols, q.fmt, q.exp) and type(other) is ops.Quant4
+            assert torch.equal(other.codes, q.codes) and torch.equal(other.scales, q.scales)
+            assert other is same or q.rows == 0 or (other.codes_ptr != q.codes_ptr and other.scales_ptr != q.scales_ptr)
+    layer = torch.nn.Module()
+    layer.weight = made
+    assert torch.equal(copy.deepcopy(layer).weight.codes, made.codes)
+    f = io.BytesIO()
+    torch.save(layer, f)
+    f.seek(0)
+    assert torch.equal(torch.load(f, weights_only=False).weight.scales, made.scales)

@@ -8,7 +8,7 @@
 // Measured on B200, device time, tensor cores -> this: N 2048, K 2048, NV4 4.3 -> 2.5 us, N 8192 5.6 -> 3.8, MX4 5.4 -> 4.0, N 2048, K 8192 9.1 -> 6.2, 8192 x 8192 18.8 -> 11.8.
 // (Two tokens in this form: as long as the tensor cores take for up to 128.)
 #pragma once
-#include "gemm_sm100.cuh"   // gelu
+#include "gemm4_sm100.cuh"   // gelu2
 #include "quant4.cuh"
 
 namespace kb {
@@ -109,7 +109,11 @@ gemv4_kernel(const Gemv4Params p) {
     const float v = (lane == 0 ? acc[0] : lane == 1 ? acc[1] : lane == 2 ? acc[2] : acc[3]) * p.alpha;
     if (p.epi == EPI_F32) static_cast<float*>(p.C)[n] = v;
     else if (p.epi == EPI_RESID) static_cast<float*>(p.C)[n] += p.gate ? p.gate[n] * v : v;
-    else static_cast<__half*>(p.C)[n] = __float2half_rn(p.epi == EPI_GELU16 ? gelu(v) : v);
+    else {
+        float g, same;
+        unpack2(gelu2(pack2(v, v)), g, same);                  // the GELU of the form for several rows
+        static_cast<__half*>(p.C)[n] = __float2half_rn(p.epi == EPI_GELU16 ? g : v);
+    }
 }
 
 }  // namespace kb

@@ -3,7 +3,7 @@ import numpy as np
 import pytest
 import torch
 
-from util_ops4 import MX4, held
+from util_ops4 import MX4, NV4, held
 
 pytestmark = pytest.mark.gpu
 
@@ -47,3 +47,22 @@ def test_overflow_and_bad_blocks(built_lib):
     y = ops.linear4(torch.empty(1, 8, device="cuda"), ops.quant4(x.cuda(), MX4), ops.quant4(w.cuda(), MX4), ops.EPI_F32).cpu()[0]
     inf = float("inf")
     assert y[[0, 1, 2, 4]].tolist() == [inf] * 4 and y[3] == -inf and torch.isnan(y[5]) and y[6] == 1.0 and y[7] == 0.0
+
+
+@pytest.mark.parametrize("fmt", [MX4, NV4], ids=["mx4", "nv4"])
+def test_gelu_as_in_a_batch(built_lib, fmt):
+    """Where the sums are exact (few enough bits between the scales) a token's GELU has the same bits alone as among others."""
+    from kiln_b200 import ops
+    g = torch.Generator().manual_seed(5)
+    x, w = torch.randn(9, 512, generator=g).half(), torch.randn(8192, 512, generator=g) / 16
+    exp = -8 if fmt == NV4 else 0
+    W = ops.quant4(w.cuda(), fmt, exp)
+    A = ops.quant4(x.cuda(), fmt)
+    rows = ops.linear4(torch.empty(9, 8192, device="cuda"), A, W, ops.EPI_F32)
+    many = ops.linear4(ops.padded_empty(9, 8192, torch.float16, "cuda"), A, W, ops.EPI_GELU16)
+    exact = torch.from_numpy(held(A) @ held(W).T).float()
+    for i in range(9):
+        one = ops.quant4(x[i:i + 1].cuda(), fmt)
+        sums = ops.linear4(torch.empty(1, 8192, device="cuda"), one, W, ops.EPI_F32)
+        assert torch.equal(sums, rows[i:i + 1]) and torch.equal(sums.cpu()[0], exact[i])
+        assert torch.equal(ops.linear4(ops.padded_empty(1, 8192, torch.float16, "cuda"), one, W, ops.EPI_GELU16), many[i:i + 1])

@@ -1268,6 +1268,7 @@ int launch_rope_t(const RopeParams& p, bool half, int way, unsigned blocks, cuda
         if (vec) return launch_dependent(rope_kernel<T, true, true>, grid, block, 0, stream, nullptr, p);
         return launch_dependent(rope_kernel<T, true, false>, grid, block, 0, stream, nullptr, p);
     }
+    if (vec && p.rot % 8) return launch_dependent(rope_kernel<T, false, true, true>, grid, block, 0, stream, nullptr, p);
     if (vec) return launch_dependent(rope_kernel<T, false, true>, grid, block, 0, stream, nullptr, p);
     return launch_dependent(rope_kernel<T, false, false>, grid, block, 0, stream, nullptr, p);
 }

@@ -42,11 +42,9 @@ __device__ __forceinline__ float2 gv4_scales(uint32_t word, int chunk) {
 }
 __device__ __forceinline__ __half2 gv4_h2(uint32_t v) { return *reinterpret_cast<const __half2*>(&v); }
 
-// acc + sa sw sum. The product of two of NV4's scales lies in 2^-18 ... 2^18. Of MX4's it may leave fp32 where the term does not (the block's sum may be 0): scales
-// on the same side of 1 are therefore multiplied with one after the other, so that what overflows or vanishes on the way does so in the term as well.
-template <int FMT>
-__device__ __forceinline__ float gv4_add(float sa, float sw, float sum, float acc) {
-    if (FMT == FMT_NV4) return fmaf(sa * sw, sum, acc);
+// acc + sa sw sum for MX4. The product of two scales may leave fp32 where the term does not (the block's sum may be 0): scales on the same side of 1 are therefore
+// multiplied with one after the other, so that what overflows or vanishes on the way does so in the term as well. (NV4's products lie in 2^-18 ... 2^18.)
+__device__ __forceinline__ float gv4_add_mx4(float sa, float sw, float sum, float acc) {
     const bool apart = (sa < 1.f) == (sw < 1.f);
     return fmaf(apart ? sw : sa * sw, apart ? sum * sa : sum, acc);
 }
@@ -81,6 +79,7 @@ gemv4_kernel(const Gemv4Params p) {
         if (c + 32 < chunks) next = load(c + 32);
         const uint32_t sws[GV4_ROWS] = {k.sw.x, k.sw.y, k.sw.z, k.sw.w};
         const float2 fa = gv4_scales<FMT>(k.sa, c);
+        float half[GV4_ROWS];                               // MX4: the first half of the block
 #pragma unroll
         for (int b = 0; b < 2; b++) {                       // 16 columns at a time: 8 bytes of codes
             uint32_t a[8];
@@ -95,8 +94,10 @@ gemv4_kernel(const Gemv4Params p) {
 #pragma unroll
                 for (int i = 1; i < 8; i++) s = __hfma2(gv4_h2(a[i]), gv4_h2(w[i]), s);
                 const float2 f = __half22float2(s), fw = gv4_scales<FMT>(sws[j], c);
-                // exact but for the sum: 8 bits of scales, 12 of the block. Rows that do not exist may have scales of anything
-                if (j < real) acc[j] = gv4_add<FMT>(b ? fa.y : fa.x, b ? fw.y : fw.x, f.x + f.y, acc[j]);
+                // exact but for the sum: 8 bits of scales, 12 of the block (MX4: 13). Rows that do not exist may have scales of anything
+                if (FMT == FMT_NV4) { if (j < real) acc[j] = fmaf((b ? fa.y : fa.x) * (b ? fw.y : fw.x), f.x + f.y, acc[j]); }
+                else if (b == 0) half[j] = f.x + f.y;
+                else if (j < real) acc[j] = gv4_add_mx4(fa.x, fw.x, half[j] + (f.x + f.y), acc[j]);
             }
         }
     }

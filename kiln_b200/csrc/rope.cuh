@@ -3,8 +3,9 @@
 // (2 i, 2 i + 1) (interleaved), the rest of the head is copied. The inverse turns by -t: it is the gradient.
 //
 // The angle of a far position turns thousands of times, and fp32 has lost its fraction by then. Here a frequency is a 64-bit fraction of a turn
-// and a position an integer, so their product modulo 2^64 IS the fraction of the turn, exactly, in two integer multiplications: the
-// only rounding is that of the fraction to 32 bits (2^-32 of a turn) and the sine's own.
+// and a position an integer, so their product modulo 2^64 IS the fraction of the turn, exactly, in two integer multiplications. What rounds is the
+// fraction on its way into an fp32 number of half turns in [-1, 1): by 2^-25 of a half turn at most (9.4e-8 rad; the 32 bits cut off before are 2^-32 of a turn), then
+// the sine and cosine themselves (2 units of fp32) and their product with the amplitude.
 //
 // Bound by memory. The sines of a row serve all of its heads of all tensors: a thread block takes a row or several (rope_split), fills shared memory
 // with one (cos, sin) per pair while its first loads are under way, and every thread keeps those of its eight elements as it goes from head to head.

@@ -126,7 +126,8 @@ void linear4(void* y, int ldy, const __half* x16, int T, const Weight4& W, Epi16
 // The block's MLP (engine/src/dit.cu:488-493) on 4-bit weights: y [T, ldy] fp32 += gate * (gelu(x16 . up^T) . down^T); the hidden activations are 4 bits as well.
 size_t mlp4_workspace(int T, int in, int hidden, int fmt);
 void mlp4(float* y, int ldy, const __half* x16, int T, const Weight4& up, const Weight4& down, const float* gate);
-// dx [T, in] fp32 = dy16 [T, out] . W, with 2 * out * in bytes of the context's workspace: what a LoRA trainer's backward needs of a frozen 4-bit weight
+// dx [T, in] fp32 = dy16 [T, out] . W, with 2 * out * in bytes of the context's workspace: what a LoRA trainer's backward needs of a frozen 4-bit weight.
+// out a multiple of 64, in of 8; the scales of a KB_MX4 weight in [2^-23, 2^13] (kb_linear4_dx says what happens to others).
 void linear4_dx(float* dx, const __half* dy16, int T, const Weight4& W);
 
 // Rotary positions of q and k [T, H * Dh] fp32 in place, from integer positions pos [T, axes] on the device (frame, row, column of a patch) and host arrays

@@ -3,7 +3,7 @@
 // The shortest of these calls take the GPU 2-5 us, and what Python and ctypes do for one - a buffer or two, a dozen tensor attributes, seventeen
 // converted arguments - took 6-9 us more: a projection of one token, quantisation and product, 22 us of host time for 6 us of device time. Here a call reads the
 // tensors' own structures and goes straight through the C ABI, whose addresses ops.py hands over once (bind), so both use one loaded library.
-// It checks what the C ABI cannot see: shapes, types, strides, and that every tensor lies on the current device.
+// It checks what the C ABI cannot see: shapes, types, strides, that a 4-bit matrix's buffers still hold it, and that every tensor lies on the current device.
 #define PY_SSIZE_T_CLEAN
 #include <Python.h>
 #include <structmember.h>
